@@ -6,7 +6,8 @@ reference names RationalTriton1DGroup / RationalTriton2D); and the reference pac
 `rational_kat_cu`'s front end rat_cuda (rational_kat_cu/__init__.py), the abs-after-sum
 variant of the activation on the same kernels; and its B-spline basis kernels with the
 FusedKANLinear layer (rational_kat_cu/bspline_basis.py).  `fused_gemm` holds the KAN block's
-fc1 -> act2 -> fc2 with the activation inside tcgen05 GEMM epilogues (KANMlpFused).
+fc1 -> act2 -> fc2 with the activation inside tcgen05 GEMM epilogues (KANMlpFused).  For
+training the model around the activation: the Muon optimizer (orthogonalised updates).
 """
 
 from . import fused_gemm
@@ -15,6 +16,7 @@ from .fused_gemm import KANMlpFused, kan_mlp_fused
 from .kat_1dgroup import KAT_Group
 from .kat_1dgroup_torch import KAT_Group_Torch, Rational_CUDA_A_1DGroup
 from .kat_2dgroup import KAT_Group2D
+from .muon import Muon, muon_step, orthogonalize
 from .rat_cuda import RatGroup, rat_cuda
 from .rational_cuda import (
     RationalCUDA1DGroup,
@@ -49,4 +51,7 @@ __all__ = [
     "fused_gemm",
     "KANMlpFused",
     "kan_mlp_fused",
+    "Muon",
+    "muon_step",
+    "orthogonalize",
 ]

@@ -1,5 +1,5 @@
 """ctypes binding of libkat_rational.so (the C ABI declared in include/kat_rational.h,
-include/kat_bspline.h and include/kat_gemm.h).
+include/kat_bspline.h, include/kat_gemm.h and include/kat_muon.h).
 
 The library is loaded once, on first use.  If it is missing the call fails with a
 RuntimeError naming the build command: there is no fallback implementation.
@@ -60,6 +60,10 @@ EXPORTED_SYMBOLS = (
     "kat_gemm_rational_bwd",
     "kat_gemm_device_status",
     "kat_gemm_set_test_stall",
+    "kat_muon_workspace_bytes",
+    "kat_orthogonalize",
+    "kat_muon_step",
+    "kat_muon_device_status",
 )
 
 KAT_SHARED_NUMERATOR = 0x100
@@ -194,6 +198,16 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.kat_rational_bwd_allreduce_formula.restype = i32
     lib.kat_rational_exchange_grads.argtypes = [vp, vp, i64, vp, vp]
     lib.kat_rational_exchange_grads.restype = i32
+    f32, c32 = ctypes.c_float, ctypes.c_int32
+    lib.kat_muon_workspace_bytes.argtypes = [c32, i64, i64]
+    lib.kat_muon_workspace_bytes.restype = ctypes.c_size_t
+    lib.kat_orthogonalize.argtypes = [vp, vp, c32, i64, i64, c32, c32, vp, ctypes.c_size_t, vp]
+    lib.kat_orthogonalize.restype = i32
+    lib.kat_muon_step.argtypes = [vp, vp, vp, c32, i64, i64, c32, f32, vp, f32, c32, f32, f32,
+                                  c32, vp, ctypes.c_size_t, vp]
+    lib.kat_muon_step.restype = i32
+    lib.kat_muon_device_status.argtypes = [i32, i32, ctypes.POINTER(ctypes.c_int)]
+    lib.kat_muon_device_status.restype = i32
     lib.kat_rational_exchange_destroy.argtypes = [vp]
     lib.kat_rational_exchange_destroy.restype = i32
 

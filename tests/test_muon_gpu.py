@@ -1,0 +1,214 @@
+"""Orthogonalised updates on the GPU against the iteration in 64 bits.
+
+Tolerance.  One step maps singular values by p(s) = a s + b s^3 + c s^5, and the change of its
+result by a change of its input is at most L = max(|p'|, |p(s)/s|) = 3.9 on [0, 1.21].  A step's own
+error is at most (|a| + 2 |b| s^2 + 3 |c| s^4) u |X|_F < 30 u |X|_F (s <= 1.21), u being the
+error of one product relative to its operands' Frobenius norms: 2^-22 from the two planes of each
+operand and sqrt(K) 2^-23 from adding K terms in fp32 (rounding or cutting).  So the result is within
+30 u sum_j L^j |X_(steps - j)|_F of the exact one, plus half a step of the output's type."""
+
+import math
+
+import pytest
+import torch
+
+import rational_kat_cu_b200 as kat
+from rational_kat_cu_b200 import muon
+
+pytestmark = pytest.mark.gpu
+
+A, B, C = 3.4445, -4.7750, 2.0315
+HALF = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.float16, torch.bfloat16)}
+
+
+def reference(u, steps=5):
+    """(result, error allowed for it before rounding) of a matrix in 64 bits."""
+    x = u.double()
+    flip = x.shape[0] > x.shape[1]
+    x = x.t() if flip else x
+    norm = x.norm()
+    x = x / norm if norm > 0 else x
+    unit = 2.0 ** -22 + math.sqrt(x.shape[1]) * 2.0 ** -23
+    allowed = 0.0
+    for _ in range(steps):
+        a = x @ x.t()
+        allowed = 3.9 * allowed + 30 * unit * float(x.norm())
+        x = A * x + (B * a + C * (a @ a)) @ x
+    return (x.t() if flip else x), allowed
+
+
+def assert_close(got, want, allowed, dtype):
+    assert got.dtype == dtype
+    off = float((got.double() - want).norm())
+    assert off <= allowed + HALF[dtype] * float(want.norm()) + 1e-30, (off, allowed)
+
+
+def normal(*shape, seed=0, dtype=torch.float32, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(dtype).to(device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 9), (7, 1), (8, 8), (33, 65), (128, 128),
+                                   (129, 127), (64, 520), (520, 64), (200, 333), (384, 1000)])
+def test_sizes(cuda_device, shape, dtype):
+    x = normal(*shape, dtype=dtype, seed=shape[0])
+    before = x.clone()
+    want, allowed = reference(x)
+    assert_close(kat.orthogonalize(x), want, allowed, dtype)
+    assert torch.equal(x, before) and muon.device_status() == 0
+
+
+def test_tiles_beyond_one_wave(cuda_device):
+    """More tiles than SMs: blocks take several tiles and both accumulators."""
+    x = normal(3, 1024, 1280, seed=5)
+    out = kat.orthogonalize(x)
+    for i in range(3):
+        want, allowed = reference(x[i])
+        assert_close(out[i], want, allowed, torch.float32)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 8])
+def test_steps(cuda_device, steps):
+    x = normal(96, 160)
+    want, allowed = reference(x, steps)
+    assert_close(kat.orthogonalize(x, steps=steps), want, allowed, torch.float32)
+
+
+def test_batches_and_strides(cuda_device):
+    x = normal(2, 3, 40, 72, seed=1)
+    out = kat.orthogonalize(x)
+    assert out.shape == x.shape
+    for i in range(2):
+        for j in range(3):
+            assert torch.equal(out[i, j], kat.orthogonalize(x[i, j]))
+    # transposed and strided inputs are the same matrices
+    assert torch.equal(kat.orthogonalize(x.transpose(-1, -2).contiguous().transpose(-1, -2)), out)
+    wide = normal(40, 144, seed=2)
+    assert torch.equal(kat.orthogonalize(wide[:, ::2]),
+                       kat.orthogonalize(wide[:, ::2].contiguous()))
+    assert kat.orthogonalize(x[:0]).shape == (0, 3, 40, 72)
+    assert kat.orthogonalize(torch.empty(3, 0, 5, device="cuda")).shape == (3, 0, 5)
+    # more matrices than a call takes
+    many = normal(70, 16, 24, seed=3)
+    out = kat.orthogonalize(many)
+    assert torch.equal(out[69], kat.orthogonalize(many[69]))
+
+
+def test_zero_tiny_huge_and_bad_values(cuda_device):
+    assert not kat.orthogonalize(torch.zeros(2, 20, 30, device="cuda")).any()
+    x = normal(50, 70)
+    base = kat.orthogonalize(x)
+    # a power of two does not change the normalised update: same bits
+    for e in (-100, 100):
+        assert torch.equal(kat.orthogonalize(x * 2.0 ** e), base)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        y = torch.stack([x, x])
+        y[1, 3, 5] = bad
+        out = kat.orthogonalize(y)
+        assert torch.equal(out[0], base) and out[1].isnan().all()
+
+
+def test_low_rank(cuda_device):
+    x = normal(100, 4) @ normal(4, 200, seed=1)
+    want, allowed = reference(x)
+    assert_close(kat.orthogonalize(x), want, allowed, torch.float32)
+    one = torch.zeros(64, 64, device="cuda")
+    one[3, 60] = -2.0
+    want, allowed = reference(one)
+    assert_close(kat.orthogonalize(one), want, allowed, torch.float32)
+
+
+def step_reference(w, g, m, lr, mu, nesterov, wd, steps=5):
+    m = mu * m.double() + g.double()
+    u = g.double() + mu * m if nesterov else m
+    o, allowed = reference(u, steps)
+    s = 0.2 * math.sqrt(max(w.shape))
+    return w.double() * (1 - lr * wd) - lr * s * o, m, lr * s * allowed
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_step(cuda_device, dtype, nesterov):
+    shapes = [(40, 72), (72, 40), (40, 72), (13, 9), (128, 256)]
+    ws = [normal(*s, seed=i, dtype=dtype) for i, s in enumerate(shapes)]
+    gs = [normal(*s, seed=10 + i, dtype=dtype) for i, s in enumerate(shapes)]
+    gs[2] = gs[2].t().contiguous().t()           # not contiguous
+    ms = [normal(*s, seed=20 + i) for i, s in enumerate(shapes)]
+    lr, mu, wd = 0.02, 0.9, 0.1
+    want = [step_reference(w, g, m, lr, mu, nesterov, wd) for w, g, m in zip(ws, gs, ms)]
+    kat.muon_step(ws, gs, ms, lr=lr, momentum=mu, nesterov=nesterov, weight_decay=wd)
+    for w, m, (rw, rm, allowed) in zip(ws, ms, want):
+        # m: one product and one sum of fp32; w: the same twice over before its rounding
+        assert (m.double() - rm).abs().max() <= 2.0 ** -23 * (rm.abs().max() + 5)
+        assert_close(w, rw, allowed + 2.0 ** -22 * float(rw.norm()), dtype)
+
+
+def test_step_refusals_leave_everything(cuda_device):
+    w, g, m = normal(8, 8), normal(8, 8, seed=1), normal(8, 8, seed=2)
+    before = w.clone(), m.clone()
+    half = torch.zeros(8, 8, device="cuda", dtype=torch.float16)
+    for ws, gs, ms in (([w, w], [g, g], [m, m.clone()]), ([w], [g], [w]), ([w], [half], [m]),
+                       ([w], [g], [half]), ([w.t()[:, :7]], [g[:, :7]], [m[:, :7]]),
+                       ([w], [g[:4]], [m]), ([w], [g.to_sparse()], [m])):
+        with pytest.raises((ValueError, TypeError)):
+            kat.muon_step(ws, gs, ms, lr=0.1)
+    for lr in (torch.zeros(2, device="cuda"), torch.zeros(1, device="cuda").half()):
+        with pytest.raises(ValueError, match="lr"):
+            kat.muon_step([w], [g], [m], lr=lr)
+    assert torch.equal(w, before[0]) and torch.equal(m, before[1])
+
+
+def test_version_counter(cuda_device):
+    w = normal(8, 8).requires_grad_()
+    y = (w * w).sum()
+    kat.muon_step([w.detach()], [normal(8, 8)], [torch.zeros(8, 8, device="cuda")], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_optimizer_streams_and_graph(cuda_device):
+    """A captured step with the step size on the device, replayed next to an eager one and beside
+    a second captured graph; a step on a side stream."""
+    def fresh():
+        p = torch.nn.Parameter(normal(96, 64, seed=4))
+        p.grad = normal(96, 64, seed=5)
+        return p
+
+    a, b, c, d = (fresh() for _ in range(4))
+    lr = torch.tensor(0.05, device="cuda")
+    opts = [kat.Muon([p], lr=lr, weight_decay=0.01) for p in (a, b, c)]
+    opts.append(kat.Muon([d], lr=0.05, weight_decay=0.01))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for o in opts:
+            o.step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for p in (b, c, d):
+        assert torch.equal(a, p)
+    graphs = []
+    for o in opts[1:3]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o.step()
+        graphs.append(graph)
+    assert torch.equal(a, b)        # capturing ran nothing
+    for value in (0.05, 0.01):
+        lr.fill_(value)
+        opts[3].param_groups[0]["lr"] = value
+        opts[0].step()
+        graphs[0].replay()
+        graphs[1].replay()
+        opts[3].step()
+        torch.cuda.synchronize()
+        for p in (b, c, d):
+            assert torch.equal(a, p)
+
+
+def test_repeatable(cuda_device):
+    x = normal(4, 300, 700, seed=9)
+    first = kat.orthogonalize(x)
+    for _ in range(5):
+        assert torch.equal(kat.orthogonalize(x), first)
