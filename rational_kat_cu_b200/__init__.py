@@ -7,12 +7,20 @@ reference names RationalTriton1DGroup / RationalTriton2D); and the reference pac
 variant of the activation on the same kernels; and its B-spline basis kernels with the
 FusedKANLinear layer (rational_kat_cu/bspline_basis.py).  `fused_gemm` holds the KAN block's
 fc1 -> act2 -> fc2 with the activation inside tcgen05 GEMM epilogues (KANMlpFused).  For
-training the model around the activation: the Muon optimizer (orthogonalised updates).
+training the model around the activation: the norm of queries and keys with the position
+rotation (qk_norm_rope) and the Muon optimizer (orthogonalised updates).
 """
 
 from . import fused_gemm
 from .bspline import BSplineBasis, FusedKANLinear, bspline_basis_bwd, bspline_basis_fwd
 from .fused_gemm import KANMlpFused, kan_mlp_fused
+from .head_norm import (
+    QKNormRope,
+    qk_norm_rope,
+    qkv_norm_rope,
+    rope_grid_table,
+    rope_table,
+)
 from .kat_1dgroup import KAT_Group
 from .kat_1dgroup_torch import KAT_Group_Torch, Rational_CUDA_A_1DGroup
 from .kat_2dgroup import KAT_Group2D
@@ -54,4 +62,9 @@ __all__ = [
     "Muon",
     "muon_step",
     "orthogonalize",
+    "QKNormRope",
+    "qk_norm_rope",
+    "qkv_norm_rope",
+    "rope_table",
+    "rope_grid_table",
 ]

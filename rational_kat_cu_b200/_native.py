@@ -1,5 +1,5 @@
 """ctypes binding of libkat_rational.so (the C ABI declared in include/kat_rational.h,
-include/kat_bspline.h, include/kat_gemm.h and include/kat_muon.h).
+include/kat_bspline.h, include/kat_gemm.h, include/kat_muon.h and include/kat_qk_norm_rope.h).
 
 The library is loaded once, on first use.  If it is missing the call fails with a
 RuntimeError naming the build command: there is no fallback implementation.
@@ -64,6 +64,9 @@ EXPORTED_SYMBOLS = (
     "kat_orthogonalize",
     "kat_muon_step",
     "kat_muon_device_status",
+    "kat_qk_norm_rope_fwd",
+    "kat_qk_norm_rope_bwd_workspace_bytes",
+    "kat_qk_norm_rope_bwd",
 )
 
 KAT_SHARED_NUMERATOR = 0x100
@@ -208,6 +211,12 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.kat_muon_step.restype = i32
     lib.kat_muon_device_status.argtypes = [i32, i32, ctypes.POINTER(ctypes.c_int)]
     lib.kat_muon_device_status.restype = i32
+    lib.kat_qk_norm_rope_fwd.argtypes = [vp, vp, c32, vp]
+    lib.kat_qk_norm_rope_fwd.restype = i32
+    lib.kat_qk_norm_rope_bwd_workspace_bytes.argtypes = [c32, c32, i32]
+    lib.kat_qk_norm_rope_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.kat_qk_norm_rope_bwd.argtypes = [vp, vp, c32, vp, ctypes.c_size_t, vp]
+    lib.kat_qk_norm_rope_bwd.restype = i32
     lib.kat_rational_exchange_destroy.argtypes = [vp]
     lib.kat_rational_exchange_destroy.restype = i32
 
