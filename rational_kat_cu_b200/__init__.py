@@ -8,7 +8,8 @@ variant of the activation on the same kernels; and its B-spline basis kernels wi
 FusedKANLinear layer (rational_kat_cu/bspline_basis.py).  `fused_gemm` holds the KAN block's
 fc1 -> act2 -> fc2 with the activation inside tcgen05 GEMM epilogues (KANMlpFused).  For
 training the model around the activation: the norm of queries and keys with the position
-rotation (qk_norm_rope) and the Muon optimizer (orthogonalised updates).
+rotation (qk_norm_rope), the learned relative position bias (distance_bias, index_bias) and
+the Muon optimizer (orthogonalised updates).
 """
 
 from . import fused_gemm
@@ -25,6 +26,15 @@ from .kat_1dgroup import KAT_Group
 from .kat_1dgroup_torch import KAT_Group_Torch, Rational_CUDA_A_1DGroup
 from .kat_2dgroup import KAT_Group2D
 from .muon import Muon, muon_step, orthogonalize
+from .position_bias import (
+    DistanceBuckets,
+    GridPositionBias,
+    IndexBuckets,
+    RelativePositionBias,
+    distance_bias,
+    grid_index,
+    index_bias,
+)
 from .rat_cuda import RatGroup, rat_cuda
 from .rational_cuda import (
     RationalCUDA1DGroup,
@@ -67,4 +77,11 @@ __all__ = [
     "qkv_norm_rope",
     "rope_table",
     "rope_grid_table",
+    "DistanceBuckets",
+    "IndexBuckets",
+    "distance_bias",
+    "index_bias",
+    "grid_index",
+    "RelativePositionBias",
+    "GridPositionBias",
 ]

@@ -22,12 +22,14 @@ SOURCES = [os.path.join(PKG_DIR, "csrc", "kat_rational.cu"),
            os.path.join(PKG_DIR, "csrc", "kat_bspline.cu"),
            os.path.join(PKG_DIR, "csrc", "kat_gemm.cu"),
            os.path.join(PKG_DIR, "csrc", "kat_muon.cu"),
-           os.path.join(PKG_DIR, "csrc", "kat_qk_norm_rope.cu")]
+           os.path.join(PKG_DIR, "csrc", "kat_qk_norm_rope.cu"),
+           os.path.join(PKG_DIR, "csrc", "kat_position_bias.cu")]
 HEADERS = [os.path.join(REPO_DIR, "include", "kat_rational.h"),
            os.path.join(REPO_DIR, "include", "kat_bspline.h"),
            os.path.join(REPO_DIR, "include", "kat_gemm.h"),
            os.path.join(REPO_DIR, "include", "kat_muon.h"),
            os.path.join(REPO_DIR, "include", "kat_qk_norm_rope.h"),
+           os.path.join(REPO_DIR, "include", "kat_position_bias.h"),
            os.path.join(PKG_DIR, "csrc", "kat_math.cuh"),
            os.path.join(PKG_DIR, "csrc", "kat_plan.h")]
 LIBRARY = os.path.join(PKG_DIR, "libkat_rational.so")

@@ -1,5 +1,6 @@
 """ctypes binding of libkat_rational.so (the C ABI declared in include/kat_rational.h,
-include/kat_bspline.h, include/kat_gemm.h, include/kat_muon.h and include/kat_qk_norm_rope.h).
+include/kat_bspline.h, include/kat_gemm.h, include/kat_muon.h, include/kat_qk_norm_rope.h and
+include/kat_position_bias.h).
 
 The library is loaded once, on first use.  If it is missing the call fails with a
 RuntimeError naming the build command: there is no fallback implementation.
@@ -67,6 +68,12 @@ EXPORTED_SYMBOLS = (
     "kat_qk_norm_rope_fwd",
     "kat_qk_norm_rope_bwd_workspace_bytes",
     "kat_qk_norm_rope_bwd",
+    "kat_distance_bias_fwd",
+    "kat_distance_bias_bwd_workspace_bytes",
+    "kat_distance_bias_bwd",
+    "kat_index_bias_fwd",
+    "kat_index_bias_bwd_workspace_bytes",
+    "kat_index_bias_bwd",
 )
 
 KAT_SHARED_NUMERATOR = 0x100
@@ -217,6 +224,21 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.kat_qk_norm_rope_bwd_workspace_bytes.restype = ctypes.c_size_t
     lib.kat_qk_norm_rope_bwd.argtypes = [vp, vp, c32, vp, ctypes.c_size_t, vp]
     lib.kat_qk_norm_rope_bwd.restype = i32
+    lib.kat_distance_bias_fwd.argtypes = [vp, c32, c32, c32, vp, c32, i64, i64, i64, c32, vp,
+                                          c32, vp]
+    lib.kat_distance_bias_fwd.restype = i32
+    lib.kat_distance_bias_bwd_workspace_bytes.argtypes = [c32, i64, i64]
+    lib.kat_distance_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.kat_distance_bias_bwd.argtypes = [vp, c32, vp, c32, c32, vp, vp, i64, i64, i64, c32, vp,
+                                          c32, vp, ctypes.c_size_t, vp]
+    lib.kat_distance_bias_bwd.restype = i32
+    lib.kat_index_bias_fwd.argtypes = [vp, c32, c32, c32, vp, i64, i64, vp, c32, vp]
+    lib.kat_index_bias_fwd.restype = i32
+    lib.kat_index_bias_bwd_workspace_bytes.argtypes = [c32, i64]
+    lib.kat_index_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.kat_index_bias_bwd.argtypes = [vp, c32, vp, c32, c32, i64, i64, vp, vp, i64, vp, i64, c32,
+                                       vp, vp, vp, c32, vp, ctypes.c_size_t, vp]
+    lib.kat_index_bias_bwd.restype = i32
     lib.kat_rational_exchange_destroy.argtypes = [vp]
     lib.kat_rational_exchange_destroy.restype = i32
 
