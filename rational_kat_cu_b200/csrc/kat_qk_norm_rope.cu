@@ -5,8 +5,13 @@
 // kernels a group of LANES lanes holds a head, 16 values to a lane in two chunks of 8 chosen so
 // that both values of a pair lie in the same lane (chunks rot/2 apart for pairs (i, i + rot/2)),
 // so the rotation needs no exchange and every access is a 16-byte one.  The sums over a head are
-// shuffles inside the group.  Blocks walk the heads of all tokens with a grid stride, heads
-// fastest, so that the heads of a token read the same table row at the same time.
+// shuffles inside the group.  A group takes runs of up to four consecutive heads (heads are numbered
+// through all tokens, a token's heads next to each other), so that a token's angles are mostly
+// loaded once a run, and walks the runs with a grid stride.
+// What bounds it is HBM; what it takes is enough bytes in flight.  Loads into registers alone kept
+// too few (x[128,197,12+12,64] bf16: forward 37 us, backward 76 us, 64 and 62 % of the copy rate):
+// each thread copies the values of its next heads with cp.async into slots of its own in
+// shared memory, three heads ahead, which needs no barrier, only its own wait.
 // Any other size, stride or alignment takes the general kernels, one warp to a head.
 
 #include <cuda_runtime.h>
@@ -28,7 +33,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxHeadDim = 1024;
 constexpr int kVecMaxHeadDim = 256;
 constexpr int kChunk = 8;
-constexpr int kBwdBlocksPerSm = 4;   // partial rows of the weights' gradients per SM
+constexpr int kFwdBlocksPerSm = 3;
+constexpr int kBwdBlocksPerSm = 2;   // also the partial rows of the weights' gradients per SM
+constexpr int kMaxRun = 4;           // heads a group takes in a row
 
 // Division of n < 2^31 by an invariant d >= 1: with l = ceil(log2 d) and
 // m = floor(2^(31 + l) / d) + 1 (below 2^32), n / d = (n m) >> (31 + l).
@@ -45,6 +52,7 @@ struct Stream {
   int64_t xs[3], ds[3], os[3];
   Divider heads;
   uint32_t rows;       // heads of all tokens
+  uint32_t run;        // consecutive heads of a group's turn
 };
 
 struct Params {
@@ -67,20 +75,25 @@ __device__ __forceinline__ void divide(uint32_t n, const Divider& v, uint32_t& q
 
 // One head of one token: its place and its table row.
 struct Where {
-  uint32_t b, t, h;
-  int64_t pos;
-  bool in_table;
+  uint32_t b, t, h, token;
 };
 __device__ __forceinline__ Where locate(const Params& p, const Stream& s, uint32_t row) {
   Where w;
-  uint32_t token;
-  divide(row, s.heads, token, w.h);
-  divide(token, p.tokens, w.b, w.t);
-  w.pos = p.positions != nullptr
+  divide(row, s.heads, w.token, w.h);
+  divide(w.token, p.tokens, w.b, w.t);
+  return w;
+}
+struct Row {
+  int64_t pos;
+  bool in_table;
+};
+__device__ __forceinline__ Row table_row(const Params& p, const Where& w) {
+  Row r;
+  r.pos = p.positions != nullptr
               ? __ldg(p.positions + int64_t(w.b) * p.ps[0] + int64_t(w.t) * p.ps[1])
               : int64_t(w.t);
-  w.in_table = p.rot_dim == 0 || (w.pos >= 0 && w.pos < p.table_rows);
-  return w;
+  r.in_table = p.rot_dim == 0 || (r.pos >= 0 && r.pos < p.table_rows);
+  return r;
 }
 __device__ __forceinline__ int64_t offset(const int64_t (&st)[3], const Where& w) {
   return int64_t(w.b) * st[0] + int64_t(w.t) * st[1] + int64_t(w.h) * st[2];
@@ -190,7 +203,7 @@ __device__ __forceinline__ void load4(const float* p, float* f) {
   const float4 v = __ldg(reinterpret_cast<const float4*>(p));
   f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
 }
-__device__ __forceinline__ Angles load_angles(const Params& p, const Part& part, const Where& w) {
+__device__ __forceinline__ Angles load_angles(const Params& p, const Part& part, const Row& w) {
   Angles g;
 #pragma unroll
   for (int i = 0; i < 8; ++i) { g.c[i] = 1.0f; g.s[i] = 0.0f; }
@@ -209,7 +222,7 @@ __device__ __forceinline__ Angles load_angles(const Params& p, const Part& part,
 }
 // Turns the pairs by the angles, or back by them.
 template <bool INTER, bool BACK>
-__device__ __forceinline__ void turn(float (&a)[8], float (&b)[8], const Angles& g) {
+__device__ __forceinline__ void turn_pairs(float (&a)[8], float (&b)[8], const Angles& g) {
   if constexpr (INTER) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -236,9 +249,9 @@ template <int LANES> __device__ __forceinline__ float group_sum(float v) {
   for (int k = LANES / 2; k > 0; k >>= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
   return v;
 }
-__device__ __forceinline__ float norm_of(const Params& p, const Where& w, float sum) {
+__device__ __forceinline__ float norm_of(const Params& p, bool in_table, float sum) {
   const float r = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
-  return w.in_table ? r : __int_as_float(0x7fc00000);
+  return in_table ? r : __int_as_float(0x7fc00000);
 }
 __device__ __forceinline__ void load_weights(const Params& p, const Stream& s, const Part& part,
                                              float (&wa)[8], float (&wb)[8]) {
@@ -250,67 +263,177 @@ __device__ __forceinline__ void load_weights(const Params& p, const Stream& s, c
   }
 }
 
+// A thread's ring of slots in shared memory: kChunks pieces of 8 values to a stage, three stages
+// ahead (two of fp32, whose stages are twice as large).
+template <typename T, int kChunks> struct Ring {
+  static constexpr int kStages = sizeof(T) == 4 ? 3 : 4;
+  static constexpr int kWords = Raw<T>::kWords;
+  static constexpr uint32_t kBytes = uint32_t(kStages) * kChunks * kWords * kThreads * 16;
+  uint32_t base;   // shared address of this thread's first slot
+  __device__ __forceinline__ explicit Ring(const void* smem)
+      : base(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16u) {}
+  __device__ __forceinline__ uint32_t slot(int stage, int chunk, int word) const {
+    return base + uint32_t(((stage * kChunks + chunk) * kWords + word) * kThreads * 16);
+  }
+  __device__ __forceinline__ void copy(int stage, int chunk, const T* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(
+                       slot(stage, chunk, i)), "l"(p + i * (16 / int(sizeof(T)))) : "memory");
+  }
+  __device__ __forceinline__ Raw<T> read(int stage, int chunk) const {
+    Raw<T> r;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w)
+                   : "r"(slot(stage, chunk, i)) : "memory");
+    return r;
+  }
+  __device__ __forceinline__ static void commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // all but the newest kStages - 2 groups of copies of this thread have landed
+  __device__ __forceinline__ static void wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+  }
+};
+
+// The heads of a group of lanes, one after the other: turn k takes head k % run of the group's
+// run k / run.  Every lane of a warp makes the same number of turns (the shuffles need them
+// all); turns behind the last head are idle.
+template <int LANES> struct Walk {
+  uint32_t group, stride, run, rows, turns;
+  uint32_t at, k;     // the run and the place in it of the next turn
+  __device__ __forceinline__ Walk(const Stream& s) {
+    constexpr uint32_t kPerWarp = 32 / LANES;
+    const uint32_t warp = (blockIdx.x * kThreads + threadIdx.x) / 32;
+    run = s.run;
+    rows = s.rows;
+    group = warp * kPerWarp + (threadIdx.x & 31) / LANES;
+    stride = gridDim.x * (kThreads / LANES);
+    const uint32_t runs = (rows + run - 1) / run, first = warp * kPerWarp;
+    turns = first < runs ? ((runs - first + stride - 1) / stride) * run : 0;
+    at = group;
+    k = 0;
+  }
+  // the next turn's head (past the end: >= rows)
+  __device__ __forceinline__ uint32_t next() {
+    const uint64_t row = uint64_t(at) * run + k;
+    if (++k == run) {
+      k = 0;
+      at += stride;
+    }
+    return row < rows ? uint32_t(row) : 0xffffffffu;
+  }
+};
+
 template <typename T, int LANES, bool INTER>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kFwdBlocksPerSm)
 kat_head_fwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kGroups = kThreads / LANES;  // heads per block
+  using R = Ring<T, 2>;
+  extern __shared__ uint4 ring_smem[];
+  const R ring(ring_smem);
   const Stream& s = p.s[blockIdx.y];
-  const int l = threadIdx.x % LANES;
-  const Part part = part_of<INTER>(l, p.head_dim, p.rot_dim);
+  const Part part = part_of<INTER>(threadIdx.x % LANES, p.head_dim, p.rot_dim);
   const T* x = static_cast<const T*>(s.x);
   T* out = static_cast<T*>(s.out);
   float wa[8], wb[8];
   load_weights(p, s, part, wa, wb);
-  // the trip count is the same for all lanes of a warp: the shuffles need them all
-  for (uint64_t base = uint64_t(blockIdx.x) * kGroups; base < s.rows;
-       base += uint64_t(gridDim.x) * kGroups) {
-    const uint64_t row = base + threadIdx.x / LANES;
-    const bool live = row < s.rows && part.active;
-    const Where w = locate(p, s, row < s.rows ? uint32_t(row) : 0u);
-    const int64_t at = offset(s.xs, w);
-    const Raw<T> ra = live ? load8(x + at + part.a) : zero8<T>();
-    const Raw<T> rb = live ? load8(x + at + part.b) : zero8<T>();
-    const Angles g = load_angles(p, part, w);
+  Walk<LANES> ahead(s), now(s);
+  auto fetch = [&](int stage) {
+    const uint32_t row = ahead.next();
+    if (row != 0xffffffffu && part.active) {
+      const T* from = x + offset(s.xs, locate(p, s, row));
+      ring.copy(stage, 0, from + part.a);
+      ring.copy(stage, 1, from + part.b);
+    }
+    R::commit();
+  };
+#pragma unroll
+  for (int i = 0; i < R::kStages - 1; ++i) fetch(i);
+  uint32_t token = 0xffffffffu;
+  bool in_table = true;
+  Angles g;
+  int stage = 0;
+  for (uint32_t turn = 0; turn < now.turns; ++turn) {
+    const uint32_t row = now.next();
+    const bool live = row != 0xffffffffu && part.active;
+    const Where w = locate(p, s, row != 0xffffffffu ? row : 0u);
+    if (w.token != token) {
+      const Row tr = table_row(p, w);
+      g = load_angles(p, part, tr);
+      in_table = tr.in_table;
+      token = w.token;
+    }
+    R::wait();
+    const Raw<T> ra = live ? ring.read(stage, 0) : zero8<T>();
+    const Raw<T> rb = live ? ring.read(stage, 1) : zero8<T>();
+    fetch(stage == 0 ? R::kStages - 1 : stage - 1);
+    if (++stage == R::kStages) stage = 0;
     float a[8], b[8];
     to_float<T>(ra, a);
     to_float<T>(rb, b);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
-    const float r = norm_of(p, w, group_sum<LANES>(sum));
+    const float r = norm_of(p, in_table, group_sum<LANES>(sum));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       a[i] = a[i] * r * wa[i];
       b[i] = b[i] * r * wb[i];
     }
-    turn<INTER, false>(a, b, g);
+    turn_pairs<INTER, false>(a, b, g);
     if (live) {
-      const int64_t to = offset(s.os, w);
-      store8(out + to + part.a, from_float<T>(a));
-      store8(out + to + part.b, from_float<T>(b));
+      T* to = out + offset(s.os, w);
+      store8(to + part.a, from_float<T>(a));
+      store8(to + part.b, from_float<T>(b));
     }
   }
 }
 
 template <typename T, int LANES, bool INTER>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kBwdBlocksPerSm)
 kat_head_bwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kGroups = kThreads / LANES;
+  using R = Ring<T, 4>;
+  extern __shared__ uint4 ring_smem[];
+  const R ring(ring_smem);
   const Stream& s = p.s[blockIdx.y];
-  const int l = threadIdx.x % LANES;
-  const Part part = part_of<INTER>(l, p.head_dim, p.rot_dim);
+  const Part part = part_of<INTER>(threadIdx.x % LANES, p.head_dim, p.rot_dim);
   const T* x = static_cast<const T*>(s.x);
   const T* dy = static_cast<const T*>(s.dy);
   T* out = static_cast<T*>(s.out);
-  if (x == nullptr) {  // values that passed by: their gradient is copied
-    for (uint64_t row = uint64_t(blockIdx.x) * kGroups + threadIdx.x / LANES; row < s.rows;
-         row += uint64_t(gridDim.x) * kGroups) {
-      if (!part.active) continue;
-      const Where w = locate(p, s, uint32_t(row));
-      const int64_t from = offset(s.ds, w), to = offset(s.os, w);
-      const Raw<T> ra = load8(dy + from + part.a), rb = load8(dy + from + part.b);
-      store8(out + to + part.a, ra);
-      store8(out + to + part.b, rb);
+  const bool copy = x == nullptr;  // values that passed by: their gradient is copied
+  Walk<LANES> ahead(s), now(s);
+  auto fetch = [&](int stage) {
+    const uint32_t row = ahead.next();
+    if (row != 0xffffffffu && part.active) {
+      const Where w = locate(p, s, row);
+      if (!copy) {
+        const T* from = x + offset(s.xs, w);
+        ring.copy(stage, 0, from + part.a);
+        ring.copy(stage, 1, from + part.b);
+      }
+      const T* from = dy + offset(s.ds, w);
+      ring.copy(stage, 2, from + part.a);
+      ring.copy(stage, 3, from + part.b);
+    }
+    R::commit();
+  };
+#pragma unroll
+  for (int i = 0; i < R::kStages - 1; ++i) fetch(i);
+  int stage = 0;
+  if (copy) {
+    for (uint32_t turn = 0; turn < now.turns; ++turn) {
+      const uint32_t row = now.next();
+      R::wait();
+      if (row != 0xffffffffu && part.active) {
+        T* to = out + offset(s.os, locate(p, s, row));
+        store8(to + part.a, ring.read(stage, 2));
+        store8(to + part.b, ring.read(stage, 3));
+      }
+      fetch(stage == 0 ? R::kStages - 1 : stage - 1);
+      if (++stage == R::kStages) stage = 0;
     }
     return;
   }
@@ -318,23 +441,32 @@ kat_head_bwd_kernel(const __grid_constant__ Params p) {
   load_weights(p, s, part, wa, wb);
 #pragma unroll
   for (int i = 0; i < 8; ++i) da[i] = db[i] = 0.0f;
-  for (uint64_t base = uint64_t(blockIdx.x) * kGroups; base < s.rows;
-       base += uint64_t(gridDim.x) * kGroups) {
-    const uint64_t row = base + threadIdx.x / LANES;
-    const bool live = row < s.rows && part.active;
-    const Where w = locate(p, s, row < s.rows ? uint32_t(row) : 0u);
-    const int64_t at = offset(s.xs, w), from = offset(s.ds, w);
-    const Raw<T> ra = live ? load8(x + at + part.a) : zero8<T>();
-    const Raw<T> rb = live ? load8(x + at + part.b) : zero8<T>();
-    const Raw<T> rga = live ? load8(dy + from + part.a) : zero8<T>();
-    const Raw<T> rgb = live ? load8(dy + from + part.b) : zero8<T>();
-    const Angles g = load_angles(p, part, w);
+  uint32_t token = 0xffffffffu;
+  bool in_table = true;
+  Angles g;
+  for (uint32_t turn = 0; turn < now.turns; ++turn) {
+    const uint32_t row = now.next();
+    const bool live = row != 0xffffffffu && part.active;
+    const Where w = locate(p, s, row != 0xffffffffu ? row : 0u);
+    if (w.token != token) {
+      const Row tr = table_row(p, w);
+      g = load_angles(p, part, tr);
+      in_table = tr.in_table;
+      token = w.token;
+    }
+    R::wait();
+    const Raw<T> ra = live ? ring.read(stage, 0) : zero8<T>();
+    const Raw<T> rb = live ? ring.read(stage, 1) : zero8<T>();
+    const Raw<T> rga = live ? ring.read(stage, 2) : zero8<T>();
+    const Raw<T> rgb = live ? ring.read(stage, 3) : zero8<T>();
+    fetch(stage == 0 ? R::kStages - 1 : stage - 1);
+    if (++stage == R::kStages) stage = 0;
     float a[8], b[8], ga[8], gb[8];
     to_float<T>(ra, a);
     to_float<T>(rb, b);
     to_float<T>(rga, ga);
     to_float<T>(rgb, gb);
-    turn<INTER, true>(ga, gb, g);
+    turn_pairs<INTER, true>(ga, gb, g);
     float sum = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -343,23 +475,22 @@ kat_head_bwd_kernel(const __grid_constant__ Params p) {
     }
     sum = group_sum<LANES>(sum);
     dot = group_sum<LANES>(dot);
-    const float r = norm_of(p, w, sum);
+    const float r = norm_of(p, in_table, sum);
     const float mean = dot * r * p.inv_dim;   // mean(dn w x r)
-    float oa[8], ob[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float ha = a[i] * r, hb = b[i] * r;
-      oa[i] = r * (ga[i] * wa[i] - ha * mean);
-      ob[i] = r * (gb[i] * wb[i] - hb * mean);
+      a[i] = r * (ga[i] * wa[i] - ha * mean);
+      b[i] = r * (gb[i] * wb[i] - hb * mean);
       if (live) {
         da[i] = fmaf(ga[i], ha, da[i]);
         db[i] = fmaf(gb[i], hb, db[i]);
       }
     }
     if (live) {
-      const int64_t to = offset(s.os, w);
-      store8(out + to + part.a, from_float<T>(oa));
-      store8(out + to + part.b, from_float<T>(ob));
+      T* to = out + offset(s.os, w);
+      store8(to + part.a, from_float<T>(a));
+      store8(to + part.b, from_float<T>(b));
     }
   }
   if (s.dweight == nullptr) return;
@@ -440,6 +571,7 @@ kat_head_fwd_any_kernel(const __grid_constant__ Params p) {
   for (uint64_t row = uint64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); row < s.rows;
        row += uint64_t(gridDim.x) * kWarps) {
     const Where w = locate(p, s, uint32_t(row));
+    const Row tr = table_row(p, w);
     const T* x = static_cast<const T*>(s.x) + offset(s.xs, w);
     T* out = static_cast<T*>(s.out) + offset(s.os, w);
     float sum = 0.0f;
@@ -447,11 +579,11 @@ kat_head_fwd_any_kernel(const __grid_constant__ Params p) {
       const float v = value_of(x + i);
       sum = fmaf(v, v, sum);
     }
-    const float r = norm_of(p, w, warp_sum(sum));
-    const int64_t angles = w.pos * (p.rot_dim / 2);
+    const float r = norm_of(p, tr.in_table, warp_sum(sum));
+    const int64_t angles = tr.pos * (p.rot_dim / 2);
     for (int i = lane; i < p.head_dim; i += 32) {
       float y = value_of(x + i) * r * weight_of(p, s, i);
-      if (i < p.rot_dim && w.in_table) {
+      if (i < p.rot_dim && tr.in_table) {
         const Pair q = pair_of<INTER>(i, p.rot_dim);
         const float z = value_of(x + q.other) * r * weight_of(p, s, q.other);
         const float c = __ldg(p.cos_table + angles + q.angle);
@@ -480,11 +612,12 @@ kat_head_bwd_any_kernel(const __grid_constant__ Params p) {
       for (int i = lane; i < p.head_dim; i += 32) out[i] = dy[i];
       continue;
     }
+    const Row tr = table_row(p, w);
     const T* x = static_cast<const T*>(s.x) + offset(s.xs, w);
-    const int64_t angles = w.pos * (p.rot_dim / 2);
+    const int64_t angles = tr.pos * (p.rot_dim / 2);
     auto back = [&](int i) {
       float g = value_of(dy + i);
-      if (i < p.rot_dim && w.in_table) {
+      if (i < p.rot_dim && tr.in_table) {
         const Pair q = pair_of<INTER>(i, p.rot_dim);
         const float z = value_of(dy + q.other);
         const float c = __ldg(p.cos_table + angles + q.angle);
@@ -501,7 +634,7 @@ kat_head_bwd_any_kernel(const __grid_constant__ Params p) {
     }
     sum = warp_sum(sum);
     dot = warp_sum(dot);
-    const float r = norm_of(p, w, sum);
+    const float r = norm_of(p, tr.in_table, sum);
     const float mean = dot * r * p.inv_dim;
     for (int i = lane; i < p.head_dim; i += 32) {
       const float g = back(i), h = value_of(x + i) * r;
@@ -518,25 +651,29 @@ kat_head_bwd_any_kernel(const __grid_constant__ Params p) {
   }
 }
 
-// dweight = the blocks' partial rows added up in fp64: 32 columns to a block, 8 runs of rows.
-__global__ void __launch_bounds__(256)
+// dweight = the blocks' partial rows added up in fp64: 32 columns to a block, 32 runs of rows (8 runs
+// of 74 rows each took 9 us, as long as the loads one after the other).
+__global__ void __launch_bounds__(1024)
 kat_head_dweight_kernel(const __grid_constant__ Params p, int blocks) {
   const Stream& s = p.s[blockIdx.y];
   if (s.dweight == nullptr || s.x == nullptr) return;
-  __shared__ double acc[8][32];
+  __shared__ double acc[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + tx;
   double sum = 0.0;
   if (col < p.head_dim) {
     const float* src = p.partial + int64_t(blockIdx.y) * blocks * p.head_dim + col;
-    for (int b = ty; b < blocks; b += 8) sum += double(src[int64_t(b) * p.head_dim]);
+#pragma unroll 4
+    for (int b = ty; b < blocks; b += 32) sum += double(src[int64_t(b) * p.head_dim]);
   }
   acc[ty][tx] = sum;
   __syncthreads();
-  if (ty == 0 && col < p.head_dim) {
-    for (int k = 1; k < 8; ++k) sum += acc[k][tx];
-    s.dweight[col] = float(sum);
-  }
+  // a warp to a column, its runs in a fixed tree
+  sum = acc[tx][ty];
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+  const int mine = blockIdx.x * 32 + ty;
+  if (tx == 0 && mine < p.head_dim) s.dweight[mine] = float(sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -640,22 +777,29 @@ int make_params(const kat_head_problem* q, const kat_head_stream* streams, int32
 
 int lanes_of(int head_dim) { return head_dim <= 32 ? 2 : head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16; }
 
+template <typename K>
+int launch_ring(K kernel, uint32_t smem, const Params& p, dim3 grid, cudaStream_t st) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) !=
+          cudaSuccess)
+    return KAT_ERR_CUDA;
+  kernel<<<grid, kThreads, smem, st>>>(p);
+  return KAT_OK;
+}
 template <typename T, int LANES, bool INTER>
-void launch_vec(const Params& p, bool backward, dim3 grid, cudaStream_t st) {
-  if (backward)
-    kat_head_bwd_kernel<T, LANES, INTER><<<grid, kThreads, 0, st>>>(p);
-  else
-    kat_head_fwd_kernel<T, LANES, INTER><<<grid, kThreads, 0, st>>>(p);
+int launch_vec(const Params& p, bool backward, dim3 grid, cudaStream_t st) {
+  return backward ? launch_ring(kat_head_bwd_kernel<T, LANES, INTER>, Ring<T, 4>::kBytes, p, grid, st)
+                  : launch_ring(kat_head_fwd_kernel<T, LANES, INTER>, Ring<T, 2>::kBytes, p, grid, st);
 }
 template <typename T, bool INTER>
-void launch_t(const Params& p, bool vec, bool backward, dim3 grid, cudaStream_t st) {
+int launch_t(const Params& p, bool vec, bool backward, dim3 grid, cudaStream_t st) {
   if (!vec) {
     if (backward)
       kat_head_bwd_any_kernel<T, INTER>
           <<<grid, kThreads, size_t(kWarps) * p.head_dim * sizeof(float), st>>>(p);
     else
       kat_head_fwd_any_kernel<T, INTER><<<grid, kThreads, 0, st>>>(p);
-    return;
+    return KAT_OK;
   }
   switch (lanes_of(p.head_dim)) {
     case 2: return launch_vec<T, 2, INTER>(p, backward, grid, st);
@@ -665,18 +809,19 @@ void launch_t(const Params& p, bool vec, bool backward, dim3 grid, cudaStream_t 
   }
 }
 template <typename T>
-void launch_i(const Params& p, bool inter, bool vec, bool backward, dim3 grid, cudaStream_t st) {
-  if (inter) launch_t<T, true>(p, vec, backward, grid, st);
-  else launch_t<T, false>(p, vec, backward, grid, st);
+int launch_i(const Params& p, bool inter, bool vec, bool backward, dim3 grid, cudaStream_t st) {
+  return inter ? launch_t<T, true>(p, vec, backward, grid, st)
+               : launch_t<T, false>(p, vec, backward, grid, st);
 }
 int launch(const Params& p, int dtype, bool inter, bool vec, bool backward, dim3 grid,
            cudaStream_t st) {
+  int rc = KAT_OK;
   switch (dtype) {
-    case KAT_DTYPE_F32: launch_i<float>(p, inter, vec, backward, grid, st); break;
-    case KAT_DTYPE_F16: launch_i<__half>(p, inter, vec, backward, grid, st); break;
-    default: launch_i<__nv_bfloat16>(p, inter, vec, backward, grid, st); break;
+    case KAT_DTYPE_F32: rc = launch_i<float>(p, inter, vec, backward, grid, st); break;
+    case KAT_DTYPE_F16: rc = launch_i<__half>(p, inter, vec, backward, grid, st); break;
+    default: rc = launch_i<__nv_bfloat16>(p, inter, vec, backward, grid, st); break;
   }
-  return cudaGetLastError() == cudaSuccess ? KAT_OK : KAT_ERR_CUDA;
+  return cudaGetLastError() == cudaSuccess ? rc : KAT_ERR_CUDA;
 }
 
 int current_sms(int* sms) {
@@ -686,11 +831,17 @@ int current_sms(int* sms) {
   return *sms > 0 ? KAT_OK : KAT_ERR_CUDA;
 }
 
-// Blocks that hold every head of the longest stream at once, but no more than `most`.
-uint32_t blocks_for(uint32_t rows, int head_dim, bool vec, uint32_t most) {
-  const uint32_t per = vec ? kThreads / lanes_of(head_dim) : kWarps;
+// Blocks that hold every head of the longest stream at once, but no more than `most`; and each
+// stream's run: as long as it leaves every group a turn.
+uint32_t blocks_for(Params* p, int count, uint32_t rows, bool vec, uint32_t most) {
+  const uint32_t per = vec ? kThreads / lanes_of(p->head_dim) : kWarps;
   const uint32_t want = (rows + per - 1) / per;
-  return want < most ? want : most;
+  const uint32_t blocks = want < most ? want : most;
+  for (int i = 0; i < count; ++i) {
+    p->s[i].run = kMaxRun;
+    while (p->s[i].run > 1 && p->s[i].rows / p->s[i].run < blocks * per) p->s[i].run /= 2;
+  }
+  return blocks;
 }
 
 }  // namespace
@@ -706,7 +857,8 @@ int kat_qk_norm_rope_fwd(const kat_head_problem* problem, const kat_head_stream*
   if (rows == 0) return KAT_OK;
   int sms = 0;
   if (int st = current_sms(&sms)) return st;
-  const dim3 grid(blocks_for(rows, p.head_dim, vec, uint32_t(sms) * 8), uint32_t(count));
+  const dim3 grid(blocks_for(&p, count, rows, vec, uint32_t(sms) * kFwdBlocksPerSm),
+                  uint32_t(count));
   return launch(p, problem->dtype, problem->interleaved != 0, vec, false, grid,
                 static_cast<cudaStream_t>(stream));
 }
@@ -737,7 +889,7 @@ int kat_qk_norm_rope_bwd(const kat_head_problem* problem, const kat_head_stream*
   }
   int sms = 0;
   if (int rc = current_sms(&sms)) return rc;
-  const dim3 grid(blocks_for(rows, p.head_dim, vec, uint32_t(sms) * kBwdBlocksPerSm),
+  const dim3 grid(blocks_for(&p, count, rows, vec, uint32_t(sms) * kBwdBlocksPerSm),
                   uint32_t(count));
   if (sums && (workspace == nullptr || !aligned16(workspace) ||
                workspace_bytes < size_t(count) * grid.x * p.head_dim * sizeof(float)))
@@ -746,7 +898,7 @@ int kat_qk_norm_rope_bwd(const kat_head_problem* problem, const kat_head_stream*
   if (int rc = launch(p, problem->dtype, problem->interleaved != 0, vec, true, grid, st))
     return rc;
   if (sums) {
-    kat_head_dweight_kernel<<<dim3((p.head_dim + 31) / 32, uint32_t(count)), 256, 0, st>>>(
+    kat_head_dweight_kernel<<<dim3((p.head_dim + 31) / 32, uint32_t(count)), 1024, 0, st>>>(
         p, int(grid.x));
     if (cudaGetLastError() != cudaSuccess) return KAT_ERR_CUDA;
   }

@@ -18,6 +18,8 @@ There is no CPU implementation: CPU tensors raise, and a missing library raises 
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -85,35 +87,35 @@ class _Problem(ctypes.Structure):
                 ("position_stride", ctypes.c_int64 * 2)]
 
 
+# The same as `_Stream` and `_Problem`, packed at once: filling ctypes fields one by one costs several
+# microseconds a call, as much as a small launch.
+_PACK_STREAM = struct.Struct("=5Q9qi4x")
+_PACK_PROBLEM = struct.Struct("=2q5if2QqQ2q")
+assert _PACK_STREAM.size == ctypes.sizeof(_Stream)
+assert _PACK_PROBLEM.size == ctypes.sizeof(_Problem)
 _NO_STRIDE = (0, 0, 0)
 
 
-def _stream_of(x: Optional[Tensor], dy: Optional[Tensor], out: Tensor, weight: Optional[Tensor],
-               dweight: Optional[Tensor]) -> _Stream:
-    return _Stream(x.data_ptr() if x is not None else None,
-                   dy.data_ptr() if dy is not None else None, out.data_ptr(),
-                   weight.data_ptr() if weight is not None else None,
-                   dweight.data_ptr() if dweight is not None else None,
-                   x.stride()[:3] if x is not None else _NO_STRIDE,
-                   dy.stride()[:3] if dy is not None else _NO_STRIDE, out.stride()[:3],
-                   out.shape[2])
+def _pack(x: int, dy: int, out: int, weight: Optional[Tensor], dweight: Optional[Tensor], xs, ds,
+          os, heads: int) -> bytes:
+    """A stream from addresses (0: none) and strides."""
+    return _PACK_STREAM.pack(x, dy, out, 0 if weight is None else weight.data_ptr(),
+                             0 if dweight is None else dweight.data_ptr(), *xs, *ds, *os, heads)
 
 
-def _problem_of(x: Tensor, weight: Optional[Tensor], cos: Optional[Tensor],
-                sin: Optional[Tensor], positions: Optional[Tensor], eps: float,
-                interleaved: bool) -> _Problem:
-    B, L, _, D = x.shape
-    rot = 0 if cos is None else 2 * cos.shape[1]
-    return _Problem(B, L, D, rot, int(interleaved), DTYPES[x.dtype],
-                    DTYPES[weight.dtype] if weight is not None else 0, eps,
-                    cos.data_ptr() if rot else None, sin.data_ptr() if rot else None,
-                    cos.shape[0] if rot else 0,
-                    positions.data_ptr() if positions is not None else None,
-                    positions.stride() if positions is not None else (0, 0))
-
-
-def _cuda_stream(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _pack_problem(batch: int, tokens: int, head_dim: int, dtype: torch.dtype,
+                  q_weight: Optional[Tensor], k_weight: Optional[Tensor], cos: Optional[Tensor],
+                  sin: Optional[Tensor], positions: Optional[Tensor], eps: float,
+                  interleaved: bool) -> bytes:
+    weight = q_weight if q_weight is not None else k_weight
+    wdtype = 0 if weight is None else DTYPES[weight.dtype]
+    pos, ps = (0, (0, 0)) if positions is None else (positions.data_ptr(), positions.stride())
+    if cos is None:
+        return _PACK_PROBLEM.pack(batch, tokens, head_dim, 0, 0, DTYPES[dtype], wdtype, eps, 0, 0,
+                                  0, 0, 0, 0)
+    rows, pairs = cos.shape
+    return _PACK_PROBLEM.pack(batch, tokens, head_dim, 2 * pairs, int(interleaved), DTYPES[dtype],
+                              wdtype, eps, cos.data_ptr(), sin.data_ptr(), rows, pos, *ps)
 
 
 def _heads(t: Tensor) -> Tensor:
@@ -121,26 +123,34 @@ def _heads(t: Tensor) -> Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
-def _forward(streams, problem: _Problem, device: torch.device) -> None:
+def _launch(device: torch.device, call, *args) -> int:
+    """`call` with the device's current stream as its last argument, on that device."""
+    if device.index == torch.cuda.current_device():
+        return call(*args, torch.cuda.current_stream(device).cuda_stream)
     with torch.cuda.device(device):
-        st = _native.lib().kat_qk_norm_rope_fwd(
-            ctypes.byref(problem), (_Stream * len(streams))(*streams), len(streams),
-            _cuda_stream(device))
-    _native.check("kat_qk_norm_rope_fwd", st)
+        return call(*args, torch.cuda.current_stream(device).cuda_stream)
 
 
-def _backward(streams, problem: _Problem, device: torch.device) -> None:
-    lib = _native.lib()
-    ws_bytes = lib.kat_qk_norm_rope_bwd_workspace_bytes(problem.head_dim, len(streams),
-                                                        device.index or 0)
-    if ws_bytes == 0:
+def _forward(problem: bytes, streams: bytes, count: int, device: torch.device) -> None:
+    _native.check("kat_qk_norm_rope_fwd",
+                  _launch(device, _native.lib().kat_qk_norm_rope_fwd, problem, streams, count))
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(head_dim: int, count: int, device_index: int) -> int:
+    n = _native.lib().kat_qk_norm_rope_bwd_workspace_bytes(head_dim, count, device_index)
+    if n == 0:
         raise RuntimeError("kat_qk_norm_rope_bwd_workspace_bytes returned 0")
-    ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8)
-    with torch.cuda.device(device):
-        st = lib.kat_qk_norm_rope_bwd(ctypes.byref(problem), (_Stream * len(streams))(*streams),
-                                      len(streams), ws.data_ptr(), ws_bytes,
-                                      _cuda_stream(device))
-    _native.check("kat_qk_norm_rope_bwd", st)
+    return n
+
+
+def _backward(problem: bytes, streams: bytes, count: int, head_dim: int,
+              device: torch.device) -> None:
+    n = _workspace_bytes(head_dim, count, device.index)
+    ws = torch.empty(n, device=device, dtype=torch.uint8)
+    _native.check("kat_qk_norm_rope_bwd",
+                  _launch(device, _native.lib().kat_qk_norm_rope_bwd, problem, streams, count,
+                          ws.data_ptr(), n))
 
 
 def _dweight(weight: Optional[Tensor], wanted: bool) -> Optional[Tensor]:
@@ -150,7 +160,25 @@ def _dweight(weight: Optional[Tensor], wanted: bool) -> Optional[Tensor]:
 
 
 def _as(grad: Optional[Tensor], like: Optional[Tensor]) -> Optional[Tensor]:
-    return grad if grad is None else grad.to(like.dtype)
+    return grad if grad is None or grad.dtype == like.dtype else grad.to(like.dtype)
+
+
+def _qk_forward(q: Tensor, k: Tensor, q_weight, k_weight, cos, sin, positions, eps: float,
+                interleaved: bool):
+    """(q', k') and the queries and keys as the kernels read them."""
+    q, k = _heads(q), _heads(k)
+    B, L, Hq, D = q.shape
+    Hk = k.shape[2]
+    device, dtype = q.device, q.dtype
+    out_q = torch.empty((B, L, Hq, D), device=device, dtype=dtype)
+    out_k = torch.empty((B, L, Hk, D), device=device, dtype=dtype)
+    _forward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, eps,
+                           interleaved),
+             _pack(q.data_ptr(), 0, out_q.data_ptr(), q_weight, None, q.stride()[:3], _NO_STRIDE,
+                   (L * Hq * D, Hq * D, D), Hq)
+             + _pack(k.data_ptr(), 0, out_k.data_ptr(), k_weight, None, k.stride()[:3],
+                     _NO_STRIDE, (L * Hk * D, Hk * D, D), Hk), 2, device)
+    return out_q, out_k, q, k
 
 
 class QKNormRopeFunction(torch.autograd.Function):
@@ -160,13 +188,8 @@ class QKNormRopeFunction(torch.autograd.Function):
     def forward(ctx, q: Tensor, k: Tensor, q_weight: Optional[Tensor],
                 k_weight: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor],
                 positions: Optional[Tensor], eps: float, interleaved: bool):
-        q, k = _heads(q), _heads(k)
-        out_q = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        out_k = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        weight = q_weight if q_weight is not None else k_weight
-        _forward((_stream_of(q, None, out_q, q_weight, None),
-                  _stream_of(k, None, out_k, k_weight, None)),
-                 _problem_of(q, weight, cos, sin, positions, eps, interleaved), q.device)
+        out_q, out_k, q, k = _qk_forward(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                         interleaved)
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.eps, ctx.interleaved = eps, interleaved
         return out_q, out_k
@@ -176,15 +199,43 @@ class QKNormRopeFunction(torch.autograd.Function):
     def backward(ctx, gq: Tensor, gk: Tensor):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype)
+        gq, gk = _heads(gq), _heads(gk)
+        B, L, Hq, D = q.shape
+        Hk = k.shape[2]
+        device, dtype = q.device, q.dtype
+        dq = torch.empty((B, L, Hq, D), device=device, dtype=dtype)
+        dk = torch.empty((B, L, Hk, D), device=device, dtype=dtype)
         dwq, dwk = _dweight(q_weight, need[2]), _dweight(k_weight, need[3])
-        weight = q_weight if q_weight is not None else k_weight
-        _backward((_stream_of(q, _heads(gq), dq, q_weight, dwq),
-                   _stream_of(k, _heads(gk), dk, k_weight, dwk)),
-                  _problem_of(q, weight, cos, sin, positions, ctx.eps, ctx.interleaved),
-                  q.device)
+        _backward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, ctx.eps,
+                                ctx.interleaved),
+                  _pack(q.data_ptr(), gq.data_ptr(), dq.data_ptr(), q_weight, dwq,
+                        q.stride()[:3], gq.stride()[:3], (L * Hq * D, Hq * D, D), Hq)
+                  + _pack(k.data_ptr(), gk.data_ptr(), dk.data_ptr(), k_weight, dwk,
+                          k.stride()[:3], gk.stride()[:3], (L * Hk * D, Hk * D, D), Hk), 2, D,
+                  device)
         return (dq, dk, _as(dwq, q_weight), _as(dwk, k_weight), None, None, None, None, None)
+
+
+def _qkv_forward(qkv: Tensor, Hq: int, Hk: int, q_weight, k_weight, cos, sin, positions,
+                 eps: float, interleaved: bool):
+    """(q', k', v) and the projection's output as the kernels read it."""
+    if qkv.stride(2) != 1 and qkv.shape[2] != 1:
+        qkv = qkv.contiguous()
+    B, L, width = qkv.shape
+    D = width // (Hq + 2 * Hk)
+    device, dtype, size = qkv.device, qkv.dtype, qkv.element_size()
+    sb, sl = qkv.stride()[:2]
+    at, xs = qkv.data_ptr(), (sb, sl, D)
+    out_q = torch.empty((B, L, Hq, D), device=device, dtype=dtype)
+    out_k = torch.empty((B, L, Hk, D), device=device, dtype=dtype)
+    v = qkv.as_strided((B, L, Hk, D), (sb, sl, D, 1), qkv.storage_offset() + (Hq + Hk) * D)
+    _forward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, eps,
+                           interleaved),
+             _pack(at, 0, out_q.data_ptr(), q_weight, None, xs, _NO_STRIDE,
+                   (L * Hq * D, Hq * D, D), Hq)
+             + _pack(at and at + Hq * D * size, 0, out_k.data_ptr(), k_weight, None, xs,
+                     _NO_STRIDE, (L * Hk * D, Hk * D, D), Hk), 2, device)
+    return out_q, out_k, v, qkv
 
 
 class QKVNormRopeFunction(torch.autograd.Function):
@@ -195,16 +246,8 @@ class QKVNormRopeFunction(torch.autograd.Function):
     def forward(ctx, qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Tensor],
                 k_weight: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor],
                 positions: Optional[Tensor], eps: float, interleaved: bool):
-        B, L, width = qkv.shape
-        D = width // (q_heads + 2 * k_heads)
-        x = _heads(qkv.unflatten(2, (q_heads + 2 * k_heads, D)))
-        q, k, v = x.split((q_heads, k_heads, k_heads), 2)
-        out_q = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        out_k = torch.empty(k.shape, device=k.device, dtype=k.dtype)
-        weight = q_weight if q_weight is not None else k_weight
-        _forward((_stream_of(q, None, out_q, q_weight, None),
-                  _stream_of(k, None, out_k, k_weight, None)),
-                 _problem_of(q, weight, cos, sin, positions, eps, interleaved), q.device)
+        out_q, out_k, v, x = _qkv_forward(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
+                                          positions, eps, interleaved)
         ctx.save_for_backward(x, q_weight, k_weight, cos, sin, positions)
         ctx.heads, ctx.eps, ctx.interleaved = (q_heads, k_heads), eps, interleaved
         return out_q, out_k, v
@@ -213,20 +256,31 @@ class QKVNormRopeFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gq: Tensor, gk: Tensor, gv: Tensor):
         x, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        q_heads, k_heads = ctx.heads
+        Hq, Hk = ctx.heads
         need = ctx.needs_input_grad
-        q, k, _ = x.split((q_heads, k_heads, k_heads), 2)
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        dq, dk, dv = dx.split((q_heads, k_heads, k_heads), 2)
+        gq, gk, gv = _heads(gq), _heads(gk), _heads(gv)
+        B, L, width = x.shape
+        D = width // (Hq + 2 * Hk)
+        device, dtype, size = x.device, x.dtype, x.element_size()
+        dx = torch.empty((B, L, width), device=device, dtype=dtype)
         dwq, dwk = _dweight(q_weight, need[3]), _dweight(k_weight, need[4])
-        weight = q_weight if q_weight is not None else k_weight
-        _backward((_stream_of(q, _heads(gq), dq, q_weight, dwq),
-                   _stream_of(k, _heads(gk), dk, k_weight, dwk),
-                   _stream_of(None, _heads(gv), dv, None, None)),
-                  _problem_of(q, weight, cos, sin, positions, ctx.eps, ctx.interleaved),
-                  q.device)
-        return (dx.flatten(2), None, None, _as(dwq, q_weight), _as(dwk, k_weight), None, None,
-                None, None, None)
+        sb, sl = x.stride()[:2]
+        at, xs = x.data_ptr(), (sb, sl, D)
+        to, os = dx.data_ptr(), (L * width, width, D)
+        k_off, v_off = Hq * D * size, (Hq + Hk) * D * size
+        _backward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, ctx.eps,
+                                ctx.interleaved),
+                  _pack(at, gq.data_ptr(), to, q_weight, dwq, xs, gq.stride()[:3], os, Hq)
+                  + _pack(at and at + k_off, gk.data_ptr(), to and to + k_off, k_weight, dwk, xs,
+                          gk.stride()[:3], os, Hk)
+                  + _pack(0, gv.data_ptr(), to and to + v_off, None, None, _NO_STRIDE,
+                          gv.stride()[:3], os, Hk), 3, D, device)
+        return (dx, None, None, _as(dwq, q_weight), _as(dwk, k_weight), None, None, None, None,
+                None)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _check_rest(name: str, x: Tensor, head_dim: int, q_weight, k_weight, cos, sin, positions):
@@ -275,6 +329,8 @@ def _check_rest(name: str, x: Tensor, head_dim: int, q_weight, k_weight, cos, si
         raise TypeError(f"{name}: positions must be int64 or int32, got {positions.dtype}")
     if positions.device != x.device:
         raise ValueError(f"{name}: positions must be on {x.device}, got {positions.device}")
+    if positions.shape == (B, L) and positions.dtype == torch.int64:
+        return positions
     try:
         return positions.long().expand(B, L)
     except RuntimeError:
@@ -306,6 +362,8 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None,
         raise TypeError(f"qk_norm_rope: q is {q.dtype} on {q.device}, k {k.dtype} on {k.device}")
     positions = _check_rest("qk_norm_rope", q, q.shape[3], q_weight, k_weight, cos, sin,
                             positions)
+    if not _wants_grad(q, k, q_weight, k_weight):
+        return _qk_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)[:2]
     return QKNormRopeFunction.apply(q, k, q_weight, k_weight, cos, sin, positions, eps,
                                     interleaved)
 
@@ -327,6 +385,9 @@ def qkv_norm_rope(qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Te
                          f"{k_heads} heads, got {tuple(qkv.shape)}")
     positions = _check_rest("qkv_norm_rope", qkv, qkv.shape[2] // (q_heads + 2 * k_heads),
                             q_weight, k_weight, cos, sin, positions)
+    if not _wants_grad(qkv, q_weight, k_weight):
+        return _qkv_forward(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin, positions, eps,
+                            interleaved)[:3]
     return QKVNormRopeFunction.apply(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
                                      positions, eps, interleaved)
 

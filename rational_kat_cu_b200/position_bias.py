@@ -36,10 +36,6 @@ MAX_REACH = 1 << 24
 INT32_MIN, INT32_MAX = -(1 << 31), (1 << 31) - 1
 
 
-def _cuda_stream(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
 def _round8(n: int) -> int:
     return (n + 7) // 8 * 8
 
@@ -232,74 +228,89 @@ def _stride(t: Tensor):
     return (ctypes.c_int64 * 3)(*t.stride())
 
 
+def _launch(device: torch.device, call, *args) -> int:
+    """`call` with the device's current stream as its last argument, on that device."""
+    if device.index == torch.cuda.current_device():
+        return call(*args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return call(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _output(heads: int, lq: int, lk: int, device: torch.device,
+            dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    """The padded rows and the view of them that is returned."""
+    out = torch.empty((heads, lq, _round8(lk)), device=device, dtype=dtype)
+    return out, (out if lk % 8 == 0 else out[:, :, :lk])
+
+
+def _distance_forward(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int,
+                      causal: bool, dtype: torch.dtype) -> Tensor:
+    device, heads = table.device, table.shape[1]
+    table = table.contiguous()
+    out, view = _output(heads, lq, lk, device, dtype)
+    _native.check("kat_distance_bias_fwd", _launch(
+        device, _native.lib().kat_distance_bias_fwd, table.data_ptr(), DTYPES[table.dtype],
+        buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), buckets.reach, lq, lk,
+        offset, causal, out.data_ptr(), DTYPES[dtype]))
+    return view
+
+
 class DistanceBiasFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int,
                 causal: bool, dtype: torch.dtype) -> Tensor:
-        heads = table.shape[1]
-        of, begin, end = buckets.on(table.device)
-        t = table.contiguous()
-        out = torch.empty(heads, lq, _round8(lk), device=table.device, dtype=dtype)
-        with torch.cuda.device(table.device):
-            st = _native.lib().kat_distance_bias_fwd(
-                t.data_ptr(), DTYPES[t.dtype], buckets.num_buckets, heads, of.data_ptr(),
-                buckets.reach, lq, lk, offset, int(causal), out.data_ptr(), DTYPES[dtype],
-                _cuda_stream(table.device))
-        _native.check("kat_distance_bias_fwd", st)
-        ctx.runs = (begin, end)
-        ctx.args = (buckets.num_buckets, heads, lq, lk, offset, int(causal), table.dtype)
-        return out[:, :, :lk]
+        ctx.args = (buckets, table.shape[1], lq, lk, offset, causal, table.dtype)
+        return _distance_forward(table, buckets, lq, lk, offset, causal, dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad: Tensor):
-        nb, heads, lq, lk, offset, causal, dtype = ctx.args
-        lib = _native.lib()
-        d = torch.empty(nb, heads, device=grad.device, dtype=dtype)
+        buckets, heads, lq, lk, offset, causal, dtype = ctx.args
+        lib, device = _native.lib(), grad.device
+        _, begin, end = buckets.on(device)
+        nb = buckets.num_buckets
+        d = torch.empty((nb, heads), device=device, dtype=dtype)
         size = lib.kat_distance_bias_bwd_workspace_bytes(heads, lq, lk)
-        ws = torch.empty(size, device=grad.device, dtype=torch.uint8)
-        with torch.cuda.device(grad.device):
-            st = lib.kat_distance_bias_bwd(
-                grad.data_ptr(), DTYPES[grad.dtype], _stride(grad), nb, heads,
-                ctx.runs[0].data_ptr(), ctx.runs[1].data_ptr(), lq, lk, offset, causal,
-                d.data_ptr(), DTYPES[dtype], ws.data_ptr(), size, _cuda_stream(grad.device))
-        _native.check("kat_distance_bias_bwd", st)
+        ws = torch.empty(size, device=device, dtype=torch.uint8)
+        _native.check("kat_distance_bias_bwd", _launch(
+            device, lib.kat_distance_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
+            nb, heads, begin.data_ptr(), end.data_ptr(), lq, lk, offset, causal, d.data_ptr(),
+            DTYPES[dtype], ws.data_ptr(), size))
         return d, None, None, None, None, None, None
+
+
+def _index_forward(table: Tensor, buckets: IndexBuckets, dtype: torch.dtype) -> Tensor:
+    device, heads = table.device, table.shape[1]
+    lq, lk = buckets.shape
+    table = table.contiguous()
+    out, view = _output(heads, lq, lk, device, dtype)
+    _native.check("kat_index_bias_fwd", _launch(
+        device, _native.lib().kat_index_bias_fwd, table.data_ptr(), DTYPES[table.dtype],
+        buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), lq, lk, out.data_ptr(),
+        DTYPES[dtype]))
+    return view
 
 
 class IndexBiasFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table: Tensor, buckets: IndexBuckets, dtype: torch.dtype) -> Tensor:
-        heads = table.shape[1]
-        lq, lk = buckets.shape
-        t = table.contiguous()
-        out = torch.empty(heads, lq, _round8(lk), device=table.device, dtype=dtype)
-        with torch.cuda.device(table.device):
-            st = _native.lib().kat_index_bias_fwd(
-                t.data_ptr(), DTYPES[t.dtype], buckets.num_buckets, heads,
-                buckets.on(table.device)[0].data_ptr(), lq, lk, out.data_ptr(), DTYPES[dtype],
-                _cuda_stream(table.device))
-        _native.check("kat_index_bias_fwd", st)
-        ctx.buckets, ctx.heads, ctx.dtype = buckets, heads, table.dtype
-        return out[:, :, :lk]
+        ctx.args = (buckets, table.shape[1], table.dtype)
+        return _index_forward(table, buckets, dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad: Tensor):
-        b, heads = ctx.buckets, ctx.heads
-        lib = _native.lib()
-        _, cells, seg_begin, slab_begin, by_bucket, bucket_begin = b.on(grad.device)
-        d = torch.empty(b.num_buckets, heads, device=grad.device, dtype=ctx.dtype)
+        b, heads, dtype = ctx.args
+        lib, device = _native.lib(), grad.device
+        _, cells, seg_begin, slab_begin, by_bucket, bucket_begin = b.on(device)
+        d = torch.empty((b.num_buckets, heads), device=device, dtype=dtype)
         size = lib.kat_index_bias_bwd_workspace_bytes(heads, b.segments)
-        ws = torch.empty(size, device=grad.device, dtype=torch.uint8)
-        with torch.cuda.device(grad.device):
-            st = lib.kat_index_bias_bwd(
-                grad.data_ptr(), DTYPES[grad.dtype], _stride(grad), b.num_buckets, heads,
-                b.shape[0], b.shape[1], cells.data_ptr(), seg_begin.data_ptr(), b.segments,
-                slab_begin.data_ptr(), b.slabs, b.slab_rows, by_bucket.data_ptr(),
-                bucket_begin.data_ptr(), d.data_ptr(), DTYPES[ctx.dtype], ws.data_ptr(), size,
-                _cuda_stream(grad.device))
-        _native.check("kat_index_bias_bwd", st)
+        ws = torch.empty(size, device=device, dtype=torch.uint8)
+        _native.check("kat_index_bias_bwd", _launch(
+            device, lib.kat_index_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
+            b.num_buckets, heads, b.shape[0], b.shape[1], cells.data_ptr(), seg_begin.data_ptr(),
+            b.segments, slab_begin.data_ptr(), b.slabs, b.slab_rows, by_bucket.data_ptr(),
+            bucket_begin.data_ptr(), d.data_ptr(), DTYPES[dtype], ws.data_ptr(), size))
         return d, None, None
 
 
@@ -314,6 +325,8 @@ def distance_bias(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, off
     if not (0 <= lq <= MAX_LENGTH and 0 <= lk <= MAX_LENGTH and abs(offset) <= MAX_LENGTH):
         raise ValueError(f"distance_bias: lq, lk and |offset| must be 0..{MAX_LENGTH}, got "
                          f"{lq}, {lk} and {offset}")
+    if not (table.requires_grad and torch.is_grad_enabled()):
+        return _distance_forward(table, buckets, lq, lk, offset, causal, dtype)
     return DistanceBiasFunction.apply(table, buckets, lq, lk, offset, causal, dtype)
 
 
@@ -323,6 +336,8 @@ def index_bias(table: Tensor, buckets: IndexBuckets,
     table's)."""
     dtype = dtype or table.dtype
     _check_table("index_bias", table, buckets.num_buckets, dtype)
+    if not (table.requires_grad and torch.is_grad_enabled()):
+        return _index_forward(table, buckets, dtype)
     return IndexBiasFunction.apply(table, buckets, dtype)
 
 
