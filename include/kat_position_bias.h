@@ -24,7 +24,8 @@
  * segments of one bucket each and at most KAT_BIAS_SEGMENT cells.
  *   cells       uint16 place in the slab (row in the slab * ld + column), segment by segment
  *   seg_begin   [segments + 1] first cell of each segment; slab_begin [slabs + 1] first segment
- *   by_bucket   [segments] segments sorted by bucket; bucket_begin [num_buckets + 1]
+ *   seg_place   [segments] each segment's place in the order of buckets; bucket_begin
+ *               [num_buckets + 1] first place of each bucket
  *
  * The same rules as in kat_rational.h: nothing is allocated, work is enqueued on `stream` of the
  * current device, argument errors are reported before anything is enqueued.
@@ -66,7 +67,7 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
                        int32_t num_buckets, int32_t heads, int64_t lq, int64_t lk,
                        const uint16_t* cells, const int32_t* seg_begin, int64_t segments,
                        const int32_t* slab_begin, int64_t slabs, int32_t slab_rows,
-                       const int32_t* by_bucket, const int32_t* bucket_begin, void* d_table,
+                       const int32_t* seg_place, const int32_t* bucket_begin, void* d_table,
                        int32_t table_dtype, void* workspace, size_t workspace_bytes,
                        void* stream);
 

@@ -5,11 +5,14 @@
 // values up once into shared memory; a thread owns 8 columns and walks down the rows, where its
 // window of 8 values moves by one: one shared-memory read and a shift for every 16-byte
 // store.  Backward: a thread owns 15 neighbouring diagonals and keeps their sums in registers: it
-// reads 8 x 8 cells at a time, stepping 8 rows down and 8 columns right, so that every cell is
-// read once, in 16-byte accesses, and no two threads add to one sum.
+// takes 8 x 8 cells at a time, stepping 8 rows down and 8 columns right, so that every cell is
+// read once, in 16-byte accesses, and no two threads add to one sum.  The cells come by cp.async
+// into slots of the thread's own, two steps ahead: loads into registers left too few bytes in
+// flight (dout[16,4096,4096] bf16: 132 us, 62 % of the copy rate).  Where rows do not start on 16
+// bytes, a thread owns one diagonal and a warp reads 32 neighbouring cells of a row.
 //
-// Index form.  Forward: the table's column of a head in shared memory, 8 cells of the index read
-// once for several heads.  Backward: a slab of whole rows goes to shared memory in 16-byte
+// Index form.  Forward: the table's columns of a few heads in shared memory, 8 cells of the index
+// read once for all of them.  Backward: a slab of whole rows goes to shared memory in 16-byte
 // accesses; then one thread sums each segment (cells of one bucket, listed by the caller) there.
 //
 // Both backwards write partial sums that small kernels add in a fixed order: no atomics.
@@ -143,95 +146,112 @@ kat_distance_bias_fwd_kernel(const __grid_constant__ DistanceFwd a) {
 
 constexpr int kBwdThreads = 128;
 constexpr int kWin = 16;   // 15 diagonals of a thread, padded
+constexpr int kBwdStages = 3;
 
 struct DistanceBwd {
   const void* dout;
   int64_t sh, si, sj;
   int64_t lq, lk, offset;
   int32_t causal, groups;    // groups of 8 rows in a split
-  int64_t splits, chunks;    // splits of the rows; threads (windows) of a split
-  float* part;               // [head][split][chunk][16]
+  int64_t splits, chunks;    // splits of the rows; threads (windows, or diagonals) of a split
+  float* part;               // [head][split][chunk][16], or [head][split][diagonal]
   double* diag;              // [head][lq + lk - 1]
 };
 
 template <typename T> __device__ __forceinline__ float load_one(const T* p);
-template <> __device__ __forceinline__ float load_one<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float load_one<float>(const float* p) { return __ldg(p); }
 template <> __device__ __forceinline__ float load_one<__half>(const __half* p) {
-  return __half2float(*p);
+  return __half2float(__ldg(p));
 }
 template <> __device__ __forceinline__ float load_one<__nv_bfloat16>(const __nv_bfloat16* p) {
-  return __bfloat162float(*p);
+  return __bfloat162float(__ldg(p));
 }
 
-// Up to 8 x 8 cells one by one; the loads of one row at a time, so that their addresses do not
-// fill the registers.
+template <typename T> constexpr uint32_t distance_ring_bytes() {
+  return uint32_t(kBwdStages) * kBwdThreads * 64 * uint32_t(sizeof(T));
+}
+
+// Rows start on 16 bytes: a thread owns the diagonals 8c - 7 .. 8c + 7.
 template <typename T>
-__device__ __forceinline__ void add_cells(const T* p, int64_t si, int64_t sj, int rows, int cols,
-                                          float (&acc)[15]) {
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    if (r < rows) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < cols) acc[e - r + 7] += load_one(p + e * sj);
-    }
-    p += si;
-    asm volatile("" ::: "memory");
-  }
-}
-
-// Where the rows of a gradient start on 16 bytes, `kVec`.
-template <typename T, bool kVec>
 __global__ void __launch_bounds__(kBwdThreads)
 kat_distance_bias_bwd_kernel(const __grid_constant__ DistanceBwd a) {
+  constexpr int kWords = int(sizeof(T)) / 2;   // 16-byte words of 8 cells
+  extern __shared__ uint4 cell_smem[];
   const int64_t k = int64_t(blockIdx.x) * kBwdThreads + threadIdx.x;
   if (k >= a.chunks) return;
   const int64_t split = blockIdx.y, h = blockIdx.z;
   const int64_t g0 = split * a.groups;
   const int64_t rows8 = (a.lq + 7) / 8, cols8 = (a.lk + 7) / 8;
   const int64_t g1 = g0 + a.groups < rows8 ? g0 + a.groups : rows8;
-  const int64_t c = k - (g0 + a.groups - 1);        // window: diagonals 8c - 7 .. 8c + 7
+  const int64_t c = k - (g0 + a.groups - 1);
   if (a.causal && 8 * c - 7 > a.offset) return;     // masked, and never read
   float acc[15];
 #pragma unroll
   for (int i = 0; i < 15; ++i) acc[i] = 0.0f;
   const T* base = static_cast<const T*>(a.dout) + h * a.sh;
   const int64_t gb = g0 > -c ? g0 : -c, ge = g1 < cols8 - c ? g1 : cols8 - c;
-  for (int64_t g = gb; g < ge; ++g) {
-    const int64_t i = 8 * g, j = 8 * (c + g);
-    const T* p = base + i * a.si + j * a.sj;
-    bool whole = false;
-    if constexpr (kVec) {
-      whole = i + 8 <= a.lq && j + 8 <= a.lk;
-      if (whole) {
-        constexpr int kPer = 16 / int(sizeof(T));
-        uint4 raw[8][8 / kPer];
+  // of the steps gb .. ge - 1 only the last may reach over the last row or column
+  int64_t whole = a.lq / 8 < a.lk / 8 - c ? a.lq / 8 : a.lk / 8 - c;
+  if (whole > ge) whole = ge;
+  const int steps = whole > gb ? int(whole - gb) : 0;
+  const uint32_t slot0 =
+      static_cast<uint32_t>(__cvta_generic_to_shared(cell_smem)) + threadIdx.x * 16u;
+  auto slot = [&](int stage, int r, int q) {
+    return slot0 + uint32_t(((stage * 8 + r) * kWords + q) * kBwdThreads * 16);
+  };
+  const T* next = base + gb * 8 * a.si + (c + gb) * 8;
+  int left = steps;
+  auto fetch = [&](int stage) {
+    if (left > 0) {
+      --left;
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+      for (int r = 0; r < 8; ++r)
 #pragma unroll
-          for (int q = 0; q < 8 / kPer; ++q) raw[r][q] = load_raw<T, kPer>(p + r * a.si + q * kPer);
+        for (int q = 0; q < kWords; ++q)
+          asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(slot(stage, r, q)),
+                       "l"(next + r * a.si + q * (16 / int(sizeof(T)))) : "memory");
+      next += 8 * a.si + 8;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+  for (int i = 0; i < kBwdStages - 1; ++i) fetch(i);
+  int stage = 0;
+  for (int t = 0; t < steps; ++t) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kBwdStages - 2) : "memory");
 #pragma unroll
-          for (int q = 0; q < 8 / kPer; ++q) {
-            const uint32_t w[4] = {raw[r][q].x, raw[r][q].y, raw[r][q].z, raw[r][q].w};
+    for (int r = 0; r < 8; ++r) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (sizeof(T) == 4) {
-                acc[4 * q + e - r + 7] += __uint_as_float(w[e]);
-              } else {
-                const float2 v = Codec<T>::unpack_word(w[e]);
-                acc[2 * e - r + 7] += v.x;
-                acc[2 * e + 1 - r + 7] += v.y;
-              }
-            }
+      for (int q = 0; q < kWords; ++q) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(slot(stage, r, q))
+                     : "memory");
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            acc[4 * q + e - r + 7] += __uint_as_float(w[e]);
+          } else {
+            const float2 v = Codec<T>::unpack_word(w[e]);
+            acc[2 * e - r + 7] += v.x;
+            acc[2 * e + 1 - r + 7] += v.y;
           }
         }
       }
     }
-    if (!whole) {
-      const int64_t rows = a.lq - i, cols = a.lk - j;
-      add_cells<T>(p, a.si, a.sj, int(rows < 8 ? rows : 8), int(cols < 8 ? cols : 8), acc);
+    fetch(stage == 0 ? kBwdStages - 1 : stage - 1);
+    if (++stage == kBwdStages) stage = 0;
+  }
+  for (int64_t g = gb + steps; g < ge; ++g) {
+    const T* p = base + 8 * g * a.si + 8 * (c + g);
+    const int64_t rows = a.lq - 8 * g, cols = a.lk - 8 * (c + g);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (r < rows && e < cols) acc[e - r + 7] += load_one(p + e);
+      p += a.si;
+      asm volatile("" ::: "memory");   // one row's loads at a time: 64 would fill the registers
     }
   }
   float4* to = reinterpret_cast<float4*>(a.part + ((h * a.splits + split) * a.chunks + k) * kWin);
@@ -241,7 +261,29 @@ kat_distance_bias_bwd_kernel(const __grid_constant__ DistanceBwd a) {
   to[3] = make_float4(acc[12], acc[13], acc[14], 0.0f);
 }
 
-// One sum for each diagonal: two windows hold it in every split.
+// Any strides: a thread owns one diagonal.
+template <typename T>
+__global__ void __launch_bounds__(kBwdThreads)
+kat_distance_bias_bwd_any_kernel(const __grid_constant__ DistanceBwd a) {
+  const int64_t k = int64_t(blockIdx.x) * kBwdThreads + threadIdx.x;
+  if (k >= a.chunks) return;
+  const int64_t split = blockIdx.y, h = blockIdx.z;
+  const int64_t d = k - (a.lq - 1);
+  if (a.causal && d > a.offset) return;
+  int64_t i0 = split * a.groups * 8, i1 = i0 + int64_t(a.groups) * 8;
+  if (i0 < -d) i0 = -d;
+  if (i1 > a.lq) i1 = a.lq;
+  if (i1 > a.lk - d) i1 = a.lk - d;
+  const int64_t step = a.si + a.sj;
+  const T* p = static_cast<const T*>(a.dout) + h * a.sh + i0 * a.si + (i0 + d) * a.sj;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int64_t i = i0; i < i1; ++i, p += step) sum += load_one(p);
+  a.part[(h * a.splits + split) * a.chunks + k] = sum;
+}
+
+// One sum for each diagonal: its splits, in each of which two windows hold it (kVec) or one thread.
+template <bool kVec>
 __global__ void __launch_bounds__(256)
 kat_distance_bias_diag_kernel(const __grid_constant__ DistanceBwd a) {
   const int64_t count = a.lq + a.lk - 1;
@@ -251,13 +293,21 @@ kat_distance_bias_diag_kernel(const __grid_constant__ DistanceBwd a) {
   const int64_t d = k - (a.lq - 1);
   double sum = 0.0;
   if (!a.causal || d <= a.offset) {
-    const int64_t c = d >= 0 ? d / 8 : -((7 - d) / 8);
-    const int o = int(d - 8 * c);
-    for (int64_t s = 0; s < a.splits; ++s) {
-      const int64_t at = c + s * a.groups + a.groups - 1;
-      const float* part = a.part + ((h * a.splits + s) * a.chunks + at) * kWin;
-      if (at >= 0 && at < a.chunks) sum += double(part[o + 7]);
-      if (o > 0 && at + 1 >= 0 && at + 1 < a.chunks) sum += double(part[kWin + o - 1]);
+    if constexpr (kVec) {
+      const int64_t c = d >= 0 ? d / 8 : -((7 - d) / 8);
+      const int o = int(d - 8 * c);
+#pragma unroll 4
+      for (int64_t s = 0; s < a.splits; ++s) {
+        const int64_t at = c + s * a.groups + a.groups - 1;
+        const float* part = a.part + ((h * a.splits + s) * a.chunks + at) * kWin;
+        const float one = at >= 0 && at < a.chunks ? part[o + 7] : 0.0f;
+        const float two = o > 0 && at + 1 >= 0 && at + 1 < a.chunks ? part[kWin + o - 1] : 0.0f;
+        sum += double(one) + double(two);
+      }
+    } else {
+#pragma unroll 4
+      for (int64_t s = 0; s < a.splits; ++s)
+        sum += double(a.part[(h * a.splits + s) * a.chunks + k]);
     }
   }
   a.diag[h * count + k] = sum;
@@ -321,13 +371,13 @@ kat_index_bias_fwd_kernel(const __grid_constant__ IndexFwd a) {
   const int heads = a.heads - h0 < a.group ? a.heads - h0 : a.group;
   const int pitch = spread(a.num_buckets) + 1;   // the last one is the zero of cells without bias
   if constexpr (kSmem) {
-    for (int64_t k = threadIdx.x; k < int64_t(a.num_buckets + 1) * heads; k += kIdxThreads) {
-      const int b = int(k / heads), h = int(k % heads);
-      f[h * pitch + spread(b)] =
-          b == a.num_buckets ? U(0)
-                             : bits_of<T>(load_any(a.table, a.table_dtype,
-                                                   int64_t(b) * a.heads + h0 + h));
-    }
+#pragma unroll 4
+    for (int b = threadIdx.x; b < a.num_buckets; b += kIdxThreads)
+      for (int h = 0; h < heads; ++h)
+        f[h * pitch + spread(b)] =
+            bits_of<T>(load_any(a.table, a.table_dtype, int64_t(b) * a.heads + h0 + h));
+    for (int h = threadIdx.x; h < heads; h += kIdxThreads)
+      f[h * pitch + spread(a.num_buckets)] = U(0);
     __syncthreads();
   }
   for (int64_t k = int64_t(blockIdx.x) * kIdxThreads + threadIdx.x; k < a.chunks;
@@ -371,38 +421,66 @@ struct IndexBwd {
   const uint16_t* cells;
   const int32_t* seg_begin;
   const int32_t* slab_begin;
+  const int32_t* seg_place;
   int64_t segments;
   int32_t slab_rows;
-  float* part;             // [head][segment]
+  float* part;             // [head][place of the segment]
 };
 
-template <typename T, bool kVec>
+// kRows: the cells of a row follow each other (any start); each 16 bytes of a row that lie on a
+// 16-byte boundary are loaded at once, four of them in flight, and spread over shared memory.
+template <typename T, bool kRows>
 __global__ void __launch_bounds__(kIdxThreads)
 kat_index_bias_bwd_kernel(const __grid_constant__ IndexBwd a) {
+  using U = typename Bits<T>::U;
   extern __shared__ uint4 slab_smem[];
-  T* s = reinterpret_cast<T*>(slab_smem);
+  U* s = reinterpret_cast<U*>(slab_smem);
   const int64_t h = blockIdx.y;
   const int64_t i0 = int64_t(blockIdx.x) * a.slab_rows;
-  const int rows = int(a.lq - i0 < a.slab_rows ? a.lq - i0 : a.slab_rows);
-  const T* base = static_cast<const T*>(a.dout) + h * a.sh + i0 * a.si;
-  const uint32_t ld = uint32_t(a.ld);
-  if constexpr (kVec) {
-    constexpr int kPer = 16 / int(sizeof(T));
-    const uint32_t per_row = ld / kPer, full = uint32_t(a.lk) / kPer;
-    for (uint32_t k = threadIdx.x; k < uint32_t(rows) * per_row; k += kIdxThreads) {
-      const uint32_t r = k / per_row, q = k % per_row;
-      const T* p = base + int64_t(r) * a.si + q * kPer;
-      if (q < full) {
-        slab_smem[k] = load_raw<T, kPer>(p);
-      } else {
-        for (uint32_t e = 0; e < kPer && q * kPer + e < uint32_t(a.lk); ++e)
-          s[k * kPer + e] = p[e];
+  const uint32_t rows = uint32_t(a.lq - i0 < a.slab_rows ? a.lq - i0 : a.slab_rows);
+  const U* base = static_cast<const U*>(a.dout) + h * a.sh + i0 * a.si;
+  const uint32_t ld = uint32_t(a.ld), lk = uint32_t(a.lk);
+  if constexpr (kRows) {
+    constexpr uint32_t kPer = 16 / sizeof(T);
+    constexpr int kFlight = 4;
+    const uint32_t per_row = lk / kPer + 2;   // pieces a row may touch
+    const uint32_t pieces = rows * per_row;
+    for (uint32_t k0 = threadIdx.x; k0 < pieces; k0 += kFlight * kIdxThreads) {
+      uint4 raw[kFlight];
+      int32_t col[kFlight];
+      uint32_t row[kFlight];
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        const uint32_t k = k0 + f * kIdxThreads;
+        row[f] = k / per_row;
+        const U* p = base + int64_t(row[f]) * a.si;
+        const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T);
+        col[f] = int32_t((k % per_row) * kPer) - int32_t(skew);
+        if (k < pieces && col[f] >= 0 && col[f] + int32_t(kPer) <= int32_t(lk))
+          raw[f] = load_raw<T, int(kPer)>(reinterpret_cast<const T*>(p + col[f]));
+        else if (k >= pieces)
+          col[f] = int32_t(lk);               // nothing
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        U* to = s + row[f] * ld;
+        if (col[f] >= 0 && col[f] + int32_t(kPer) <= int32_t(lk)) {
+          const uint32_t w[4] = {raw[f].x, raw[f].y, raw[f].z, raw[f].w};
+#pragma unroll
+          for (uint32_t e = 0; e < kPer; ++e)
+            to[col[f] + e] = U(sizeof(T) == 4 ? w[e % 4] : w[(e / 2) % 4] >> (16 * (e & 1)));
+        } else {
+          const U* p = base + int64_t(row[f]) * a.si;
+          for (int32_t j = col[f] < 0 ? 0 : col[f];
+               j < col[f] + int32_t(kPer) && j < int32_t(lk); ++j)
+            to[j] = __ldg(p + j);
+        }
       }
     }
   } else {
-    for (uint32_t k = threadIdx.x; k < uint32_t(rows) * ld; k += kIdxThreads) {
-      const uint32_t r = k / ld, j = k % ld;
-      if (j < uint32_t(a.lk)) s[k] = base[int64_t(r) * a.si + int64_t(j) * a.sj];
+    for (uint32_t k = threadIdx.x; k < rows * lk; k += kIdxThreads) {
+      const uint32_t r = k / lk, j = k % lk;
+      s[r * ld + j] = __ldg(base + int64_t(r) * a.si + int64_t(j) * a.sj);
     }
   }
   __syncthreads();
@@ -410,18 +488,16 @@ kat_index_bias_bwd_kernel(const __grid_constant__ IndexBwd a) {
   for (int32_t g = __ldg(a.slab_begin + blockIdx.x) + int(threadIdx.x); g < end; g += kIdxThreads) {
     float sum = 0.0f;
     const int32_t last = __ldg(a.seg_begin + g + 1);
-    for (int32_t k = __ldg(a.seg_begin + g); k < last; ++k) {
-      if constexpr (sizeof(T) == 4) sum += s[__ldg(a.cells + k)];
-      else sum += Codec<T>::unpack1(reinterpret_cast<const uint16_t*>(s)[__ldg(a.cells + k)]);
-    }
-    a.part[h * a.segments + g] = sum;
+#pragma unroll 4
+    for (int32_t k = __ldg(a.seg_begin + g); k < last; ++k)
+      sum += Codec<T>::unpack1(s[__ldg(a.cells + k)]);
+    a.part[h * a.segments + __ldg(a.seg_place + g)] = sum;
   }
 }
 
 // The segments of a bucket for one head, by 8 lanes.
 __global__ void __launch_bounds__(256)
 kat_index_bias_bucket_kernel(const float* __restrict__ part, int64_t segments,
-                             const int32_t* __restrict__ by_bucket,
                              const int32_t* __restrict__ bucket_begin, int num_buckets, int heads,
                              void* d_table, int table_dtype) {
   const int64_t k = int64_t(blockIdx.x) * 32 + (threadIdx.x >> 3);
@@ -431,8 +507,9 @@ kat_index_bias_bucket_kernel(const float* __restrict__ part, int64_t segments,
   double sum = 0.0;
   if (live) {
     const int32_t end = bucket_begin[b + 1];
+#pragma unroll 4
     for (int32_t g = bucket_begin[b] + lane; g < end; g += 8)
-      sum += double(part[int64_t(h) * segments + by_bucket[g]]);
+      sum += double(part[int64_t(h) * segments + g]);
   }
 #pragma unroll
   for (int m = 4; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
@@ -470,19 +547,22 @@ struct DistancePlan {
   int64_t splits, chunks;
   size_t part, total;
 };
-// Rows of a split: as many as leave enough windows for the whole device (148 SMs x 1024 threads),
-// since every window of a split costs 64 bytes of partial sums for 128 bytes a group.
-DistancePlan distance_plan(int32_t heads, int64_t lq, int64_t lk) {
+// Groups of 8 rows in a split: as many as leave enough threads for the whole device.  A window's
+// 15 sums of a split cost 64 bytes (a diagonal's 4) next to the cells that it reads there.
+DistancePlan distance_plan(int32_t heads, int64_t lq, int64_t lk, bool vec) {
   const int64_t rows8 = (lq + 7) / 8, cols8 = (lk + 7) / 8;
-  int64_t g = 32;
+  const int64_t most = 32, threads = 148 * (vec ? 512 : 2048);
+  int64_t g = most;
   auto splits = [&](int64_t n) { return (rows8 + n - 1) / n; };
-  while (g > 1 && heads * splits(g) * (cols8 + g - 1) < 148 * 1024) g /= 2;
+  auto chunks = [&](int64_t n) { return vec ? cols8 + n - 1 : lq + lk - 1; };
+  while (g > 1 && heads * splits(g) * chunks(g) < threads) g /= 2;
   while (splits(g) > 65535) g *= 2;
   DistancePlan p;
   p.groups = int32_t(g);
   p.splits = splits(g);
-  p.chunks = cols8 + g - 1;
-  p.part = size_t(heads) * size_t(p.splits) * size_t(p.chunks) * kWin * sizeof(float);
+  p.chunks = chunks(g);
+  p.part = size_t(heads) * size_t(p.splits) * size_t(p.chunks) * (vec ? kWin : 1) * sizeof(float);
+  p.part = (p.part + 15) / 16 * 16;
   p.total = p.part + size_t(heads) * size_t(lq + lk - 1) * sizeof(double);
   return p;
 }
@@ -503,9 +583,15 @@ void launch_distance_fwd(const DistanceFwd& a, dim3 grid, size_t smem, cudaStrea
 }
 
 template <typename T>
-void launch_distance_bwd(const DistanceBwd& a, bool vec, dim3 grid, cudaStream_t st) {
-  if (vec) kat_distance_bias_bwd_kernel<T, true><<<grid, kBwdThreads, 0, st>>>(a);
-  else kat_distance_bias_bwd_kernel<T, false><<<grid, kBwdThreads, 0, st>>>(a);
+int launch_distance_bwd(const DistanceBwd& a, bool vec, dim3 grid, cudaStream_t st) {
+  if (!vec) {
+    kat_distance_bias_bwd_any_kernel<T><<<grid, kBwdThreads, 0, st>>>(a);
+    return launched();
+  }
+  constexpr uint32_t bytes = distance_ring_bytes<T>();
+  if (int rc = set_smem(kat_distance_bias_bwd_kernel<T>, bytes)) return rc;
+  kat_distance_bias_bwd_kernel<T><<<grid, kBwdThreads, bytes, st>>>(a);
+  return launched();
 }
 
 template <typename T>
@@ -520,8 +606,10 @@ int launch_index_fwd(IndexFwd a, cudaStream_t st) {
   while (group > 1 && blocks * ((a.heads + group - 1) / group) < 148 * 2) group = (group + 1) / 2;
   a.group = group;
   const int head_blocks = (a.heads + group - 1) / group;
-  // large ones: a block takes several runs of cells, so that it loads its table columns once
-  const int64_t most = (148 * 6 + head_blocks - 1) / head_blocks;
+  // large ones: a block loads its table columns once and takes several runs of cells, as many as
+  // make one wave of blocks (index[1025,1025], 16 heads fp32: six waves spent 69 us, most of it on
+  // the columns)
+  const int64_t most = (148 * (smem ? 3 : 8) + head_blocks - 1) / head_blocks;
   if (blocks > most) blocks = most;
   const dim3 grid{uint32_t(blocks), uint32_t(head_blocks)};
   if (smem) {
@@ -534,16 +622,17 @@ int launch_index_fwd(IndexFwd a, cudaStream_t st) {
   return launched();
 }
 
-template <typename T, bool kVec>
+template <typename T, bool kRows>
 int launch_index_bwd_v(const IndexBwd& a, dim3 grid, cudaStream_t st) {
   const size_t bytes = size_t(a.slab_rows) * size_t(a.ld) * sizeof(T);
-  if (int rc = set_smem(kat_index_bias_bwd_kernel<T, kVec>, bytes)) return rc;
-  kat_index_bias_bwd_kernel<T, kVec><<<grid, kIdxThreads, bytes, st>>>(a);
+  if (int rc = set_smem(kat_index_bias_bwd_kernel<T, kRows>, bytes)) return rc;
+  kat_index_bias_bwd_kernel<T, kRows><<<grid, kIdxThreads, bytes, st>>>(a);
   return launched();
 }
 template <typename T>
-int launch_index_bwd(const IndexBwd& a, bool vec, dim3 grid, cudaStream_t st) {
-  return vec ? launch_index_bwd_v<T, true>(a, grid, st) : launch_index_bwd_v<T, false>(a, grid, st);
+int launch_index_bwd(const IndexBwd& a, dim3 grid, cudaStream_t st) {
+  return a.sj == 1 ? launch_index_bwd_v<T, true>(a, grid, st)
+                   : launch_index_bwd_v<T, false>(a, grid, st);
 }
 
 }  // namespace
@@ -601,7 +690,9 @@ size_t kat_distance_bias_bwd_workspace_bytes(int32_t heads, int64_t lq, int64_t 
   if (check_common(KAT_DTYPE_F32, KAT_DTYPE_F32, 1, heads, lq, lk) != KAT_OK || heads == 0 ||
       lq == 0 || lk == 0)
     return 0;
-  return distance_plan(heads, lq, lk).total;
+  const size_t vec = distance_plan(heads, lq, lk, true).total;
+  const size_t any = distance_plan(heads, lq, lk, false).total;
+  return vec > any ? vec : any;
 }
 
 int kat_distance_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout_stride,
@@ -621,7 +712,8 @@ int kat_distance_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* d
                : KAT_ERR_CUDA;
   if (dout == nullptr || dout_stride == nullptr || run_begin == nullptr || run_end == nullptr)
     return KAT_ERR_NULL_POINTER;
-  const DistancePlan plan = distance_plan(heads, lq, lk);
+  const bool vec = vector_rows(dout, dout_dtype, dout_stride);
+  const DistancePlan plan = distance_plan(heads, lq, lk, vec);
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < plan.total)
     return KAT_ERR_WORKSPACE;
   DistanceBwd a{};
@@ -640,15 +732,16 @@ int kat_distance_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* d
   a.diag = reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + plan.part);
   const dim3 grid{uint32_t((plan.chunks + kBwdThreads - 1) / kBwdThreads), uint32_t(plan.splits),
                   uint32_t(heads)};
-  const bool vec = vector_rows(dout, dout_dtype, dout_stride);
+  int rc = KAT_OK;
   switch (dout_dtype) {
-    case KAT_DTYPE_F32: launch_distance_bwd<float>(a, vec, grid, st); break;
-    case KAT_DTYPE_F16: launch_distance_bwd<__half>(a, vec, grid, st); break;
-    default: launch_distance_bwd<__nv_bfloat16>(a, vec, grid, st); break;
+    case KAT_DTYPE_F32: rc = launch_distance_bwd<float>(a, vec, grid, st); break;
+    case KAT_DTYPE_F16: rc = launch_distance_bwd<__half>(a, vec, grid, st); break;
+    default: rc = launch_distance_bwd<__nv_bfloat16>(a, vec, grid, st); break;
   }
-  if (int rc = launched()) return rc;
-  kat_distance_bias_diag_kernel<<<dim3(uint32_t((lq + lk - 1 + 255) / 256), uint32_t(heads)), 256,
-                                  0, st>>>(a);
+  if (rc) return rc;
+  const dim3 diag_grid{uint32_t((lq + lk - 1 + 255) / 256), uint32_t(heads)};
+  if (vec) kat_distance_bias_diag_kernel<true><<<diag_grid, 256, 0, st>>>(a);
+  else kat_distance_bias_diag_kernel<false><<<diag_grid, 256, 0, st>>>(a);
   kat_distance_bias_run_kernel<<<dim3(uint32_t(num_buckets), uint32_t(heads)), 256, 0, st>>>(
       a, run_begin, run_end, heads, d_table, table_dtype);
   return launched();
@@ -686,7 +779,7 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
                        int32_t num_buckets, int32_t heads, int64_t lq, int64_t lk,
                        const uint16_t* cells, const int32_t* seg_begin, int64_t segments,
                        const int32_t* slab_begin, int64_t slabs, int32_t slab_rows,
-                       const int32_t* by_bucket, const int32_t* bucket_begin, void* d_table,
+                       const int32_t* seg_place, const int32_t* bucket_begin, void* d_table,
                        int32_t table_dtype, void* workspace, size_t workspace_bytes,
                        void* stream) {
   if (int rc = check_common(table_dtype, dout_dtype, num_buckets, heads, lq, lk)) return rc;
@@ -699,7 +792,7 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
                ? KAT_OK
                : KAT_ERR_CUDA;
   if (dout == nullptr || dout_stride == nullptr || cells == nullptr || seg_begin == nullptr ||
-      slab_begin == nullptr || by_bucket == nullptr || bucket_begin == nullptr)
+      slab_begin == nullptr || seg_place == nullptr || bucket_begin == nullptr)
     return KAT_ERR_NULL_POINTER;
   const int64_t ld = round8(lk);
   if (segments < 0 || segments >= (int64_t(1) << 31) || slab_rows < 1 ||
@@ -720,21 +813,21 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
   a.cells = cells;
   a.seg_begin = seg_begin;
   a.slab_begin = slab_begin;
+  a.seg_place = seg_place;
   a.segments = segments;
   a.slab_rows = slab_rows;
   a.part = static_cast<float*>(workspace);
   const dim3 grid{uint32_t(slabs), uint32_t(heads)};
-  const bool vec = vector_rows(dout, dout_dtype, dout_stride);
   int rc = KAT_OK;
   switch (dout_dtype) {
-    case KAT_DTYPE_F32: rc = launch_index_bwd<float>(a, vec, grid, st); break;
-    case KAT_DTYPE_F16: rc = launch_index_bwd<__half>(a, vec, grid, st); break;
-    default: rc = launch_index_bwd<__nv_bfloat16>(a, vec, grid, st); break;
+    case KAT_DTYPE_F32: rc = launch_index_bwd<float>(a, grid, st); break;
+    case KAT_DTYPE_F16: rc = launch_index_bwd<__half>(a, grid, st); break;
+    default: rc = launch_index_bwd<__nv_bfloat16>(a, grid, st); break;
   }
   if (rc) return rc;
   const int64_t sums = int64_t(num_buckets) * heads;
   kat_index_bias_bucket_kernel<<<uint32_t((sums + 31) / 32), 256, 0, st>>>(
-      a.part, segments, by_bucket, bucket_begin, num_buckets, heads, d_table, table_dtype);
+      a.part, segments, bucket_begin, num_buckets, heads, d_table, table_dtype);
   return launched();
 }
 

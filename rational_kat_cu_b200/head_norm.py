@@ -123,17 +123,9 @@ def _heads(t: Tensor) -> Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
-def _launch(device: torch.device, call, *args) -> int:
-    """`call` with the device's current stream as its last argument, on that device."""
-    if device.index == torch.cuda.current_device():
-        return call(*args, torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        return call(*args, torch.cuda.current_stream(device).cuda_stream)
-
-
 def _forward(problem: bytes, streams: bytes, count: int, device: torch.device) -> None:
     _native.check("kat_qk_norm_rope_fwd",
-                  _launch(device, _native.lib().kat_qk_norm_rope_fwd, problem, streams, count))
+                  _native.on_stream(device, _native.lib().kat_qk_norm_rope_fwd, problem, streams, count))
 
 
 @functools.lru_cache(maxsize=None)
@@ -149,7 +141,7 @@ def _backward(problem: bytes, streams: bytes, count: int, head_dim: int,
     n = _workspace_bytes(head_dim, count, device.index)
     ws = torch.empty(n, device=device, dtype=torch.uint8)
     _native.check("kat_qk_norm_rope_bwd",
-                  _launch(device, _native.lib().kat_qk_norm_rope_bwd, problem, streams, count,
+                  _native.on_stream(device, _native.lib().kat_qk_norm_rope_bwd, problem, streams, count,
                           ws.data_ptr(), n))
 
 

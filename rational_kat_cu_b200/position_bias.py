@@ -153,7 +153,9 @@ class IndexBuckets:
         dev = index.device
         padded = torch.full((lq, ld), num_buckets, dtype=torch.int32, device=dev)
         padded[:, :lk] = torch.where(index < 0, num_buckets, index)
-        self.slab_rows = max(1, SLAB_CELLS // max(ld, 1))
+        # rows of a slab: at most what its shared memory holds, and at least 16 slabs' worth of
+        # blocks for each head
+        self.slab_rows = max(1, min(SLAB_CELLS // max(ld, 1), -(-lq // 16)))
         self.slabs = -(-lq // self.slab_rows)
 
         flat = padded.flatten()
@@ -171,18 +173,20 @@ class IndexBuckets:
         self.segments = begin.numel()
         seg_slab, seg_bucket = key[begin] // num_buckets, key[begin] % num_buckets
         sorted_bucket, by_bucket = seg_bucket.sort(stable=True)
+        seg_place = torch.empty_like(by_bucket)
+        seg_place[by_bucket] = torch.arange(self.segments, device=dev)
         self._tensors = (
             padded,
             cells.to(torch.uint16),
             torch.cat([begin, torch.tensor([n], device=dev)]).to(torch.int32),
             torch.searchsorted(seg_slab, torch.arange(self.slabs + 1, device=dev)).to(torch.int32),
-            by_bucket.to(torch.int32),
+            seg_place.to(torch.int32),
             torch.searchsorted(sorted_bucket,
                                torch.arange(num_buckets + 1, device=dev)).to(torch.int32))
         self._on: Dict[torch.device, Tuple[Tensor, ...]] = {dev: self._tensors}
 
     def on(self, device: torch.device) -> Tuple[Tensor, ...]:
-        """(index, cells, seg_begin, slab_begin, by_bucket, bucket_begin) on `device`, kept there
+        """(index, cells, seg_begin, slab_begin, seg_place, bucket_begin) on `device`, kept there
         (the first use on a device copies them: not inside a graph capture)."""
         if device not in self._on:
             self._on[device] = tuple(t.to(device) for t in self._tensors)
@@ -228,14 +232,6 @@ def _stride(t: Tensor):
     return (ctypes.c_int64 * 3)(*t.stride())
 
 
-def _launch(device: torch.device, call, *args) -> int:
-    """`call` with the device's current stream as its last argument, on that device."""
-    if device.index == torch.cuda.current_device():
-        return call(*args, torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        return call(*args, torch.cuda.current_stream(device).cuda_stream)
-
-
 def _output(heads: int, lq: int, lk: int, device: torch.device,
             dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
     """The padded rows and the view of them that is returned."""
@@ -248,7 +244,7 @@ def _distance_forward(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int,
     device, heads = table.device, table.shape[1]
     table = table.contiguous()
     out, view = _output(heads, lq, lk, device, dtype)
-    _native.check("kat_distance_bias_fwd", _launch(
+    _native.check("kat_distance_bias_fwd", _native.on_stream(
         device, _native.lib().kat_distance_bias_fwd, table.data_ptr(), DTYPES[table.dtype],
         buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), buckets.reach, lq, lk,
         offset, causal, out.data_ptr(), DTYPES[dtype]))
@@ -272,7 +268,7 @@ class DistanceBiasFunction(torch.autograd.Function):
         d = torch.empty((nb, heads), device=device, dtype=dtype)
         size = lib.kat_distance_bias_bwd_workspace_bytes(heads, lq, lk)
         ws = torch.empty(size, device=device, dtype=torch.uint8)
-        _native.check("kat_distance_bias_bwd", _launch(
+        _native.check("kat_distance_bias_bwd", _native.on_stream(
             device, lib.kat_distance_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
             nb, heads, begin.data_ptr(), end.data_ptr(), lq, lk, offset, causal, d.data_ptr(),
             DTYPES[dtype], ws.data_ptr(), size))
@@ -284,7 +280,7 @@ def _index_forward(table: Tensor, buckets: IndexBuckets, dtype: torch.dtype) -> 
     lq, lk = buckets.shape
     table = table.contiguous()
     out, view = _output(heads, lq, lk, device, dtype)
-    _native.check("kat_index_bias_fwd", _launch(
+    _native.check("kat_index_bias_fwd", _native.on_stream(
         device, _native.lib().kat_index_bias_fwd, table.data_ptr(), DTYPES[table.dtype],
         buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), lq, lk, out.data_ptr(),
         DTYPES[dtype]))
@@ -302,14 +298,14 @@ class IndexBiasFunction(torch.autograd.Function):
     def backward(ctx, grad: Tensor):
         b, heads, dtype = ctx.args
         lib, device = _native.lib(), grad.device
-        _, cells, seg_begin, slab_begin, by_bucket, bucket_begin = b.on(device)
+        _, cells, seg_begin, slab_begin, seg_place, bucket_begin = b.on(device)
         d = torch.empty((b.num_buckets, heads), device=device, dtype=dtype)
         size = lib.kat_index_bias_bwd_workspace_bytes(heads, b.segments)
         ws = torch.empty(size, device=device, dtype=torch.uint8)
-        _native.check("kat_index_bias_bwd", _launch(
+        _native.check("kat_index_bias_bwd", _native.on_stream(
             device, lib.kat_index_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
             b.num_buckets, heads, b.shape[0], b.shape[1], cells.data_ptr(), seg_begin.data_ptr(),
-            b.segments, slab_begin.data_ptr(), b.slabs, b.slab_rows, by_bucket.data_ptr(),
+            b.segments, slab_begin.data_ptr(), b.slabs, b.slab_rows, seg_place.data_ptr(),
             bucket_begin.data_ptr(), d.data_ptr(), DTYPES[dtype], ws.data_ptr(), size))
         return d, None, None
 
