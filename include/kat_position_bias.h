@@ -22,7 +22,8 @@
  * The index gradient goes by segments: the rows are cut into slabs of whole rows of at most
  * KAT_BIAS_SLAB_CELLS padded cells; within a slab the cells are sorted by bucket and cut into
  * segments of one bucket each and at most KAT_BIAS_SEGMENT cells.
- *   cells       uint16 place in the slab (row in the slab * ld + column), segment by segment
+ *   cells       uint16 place in the slab (row in the slab * lk + column), segment by segment;
+ *               padded_cells the same with rows of ld (the kernel takes what dout's rows are)
  *   seg_begin   [segments + 1] first cell of each segment; slab_begin [slabs + 1] first segment
  *   seg_place   [segments] each segment's place in the order of buckets; bucket_begin
  *               [num_buckets + 1] first place of each bucket
@@ -65,8 +66,9 @@ size_t kat_index_bias_bwd_workspace_bytes(int32_t heads, int64_t segments);
 
 int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout_stride,
                        int32_t num_buckets, int32_t heads, int64_t lq, int64_t lk,
-                       const uint16_t* cells, const int32_t* seg_begin, int64_t segments,
-                       const int32_t* slab_begin, int64_t slabs, int32_t slab_rows,
+                       const uint16_t* cells, const uint16_t* padded_cells,
+                       const int32_t* seg_begin, int64_t segments, const int32_t* slab_begin,
+                       int64_t slabs, int32_t slab_rows,
                        const int32_t* seg_place, const int32_t* bucket_begin, void* d_table,
                        int32_t table_dtype, void* workspace, size_t workspace_bytes,
                        void* stream);

@@ -236,7 +236,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.kat_index_bias_fwd.restype = i32
     lib.kat_index_bias_bwd_workspace_bytes.argtypes = [c32, i64]
     lib.kat_index_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
-    lib.kat_index_bias_bwd.argtypes = [vp, c32, vp, c32, c32, i64, i64, vp, vp, i64, vp, i64, c32,
+    lib.kat_index_bias_bwd.argtypes = [vp, c32, vp, c32, c32, i64, i64, vp, vp, vp, i64, vp, i64, c32,
                                        vp, vp, vp, c32, vp, ctypes.c_size_t, vp]
     lib.kat_index_bias_bwd.restype = i32
     lib.kat_rational_exchange_destroy.argtypes = [vp]

@@ -154,6 +154,7 @@ struct DistanceBwd {
   int64_t lq, lk, offset;
   int32_t causal, groups;    // groups of 8 rows in a split
   int64_t splits, chunks;    // splits of the rows; threads (windows, or diagonals) of a split
+  int64_t threads;           // of all heads and splits
   float* part;               // [head][split][chunk][16], or [head][split][diagonal]
   double* diag;              // [head][lq + lk - 1]
 };
@@ -177,17 +178,17 @@ __global__ void __launch_bounds__(kBwdThreads)
 kat_distance_bias_bwd_kernel(const __grid_constant__ DistanceBwd a) {
   constexpr int kWords = int(sizeof(T)) / 2;   // 16-byte words of 8 cells
   extern __shared__ uint4 cell_smem[];
-  const int64_t k = int64_t(blockIdx.x) * kBwdThreads + threadIdx.x;
-  if (k >= a.chunks) return;
-  const int64_t split = blockIdx.y, h = blockIdx.z;
+  const int64_t id = int64_t(blockIdx.x) * kBwdThreads + threadIdx.x;
+  if (id >= a.threads) return;
+  const int64_t k = id % a.chunks, split = id / a.chunks % a.splits, h = id / a.chunks / a.splits;
   const int64_t g0 = split * a.groups;
   const int64_t rows8 = (a.lq + 7) / 8, cols8 = (a.lk + 7) / 8;
   const int64_t g1 = g0 + a.groups < rows8 ? g0 + a.groups : rows8;
   const int64_t c = k - (g0 + a.groups - 1);
   if (a.causal && 8 * c - 7 > a.offset) return;     // masked, and never read
-  float acc[15];
+  float acc[15], tot[15];   // 256 terms at most go one after the other into a sum
 #pragma unroll
-  for (int i = 0; i < 15; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < 15; ++i) acc[i] = tot[i] = 0.0f;
   const T* base = static_cast<const T*>(a.dout) + h * a.sh;
   const int64_t gb = g0 > -c ? g0 : -c, ge = g1 < cols8 - c ? g1 : cols8 - c;
   // of the steps gb .. ge - 1 only the last may reach over the last row or column
@@ -241,6 +242,13 @@ kat_distance_bias_bwd_kernel(const __grid_constant__ DistanceBwd a) {
     }
     fetch(stage == 0 ? kBwdStages - 1 : stage - 1);
     if (++stage == kBwdStages) stage = 0;
+    if ((t & 31) == 31) {
+#pragma unroll
+      for (int i = 0; i < 15; ++i) {
+        tot[i] += acc[i];
+        acc[i] = 0.0f;
+      }
+    }
   }
   for (int64_t g = gb + steps; g < ge; ++g) {
     const T* p = base + 8 * g * a.si + 8 * (c + g);
@@ -254,7 +262,9 @@ kat_distance_bias_bwd_kernel(const __grid_constant__ DistanceBwd a) {
       asm volatile("" ::: "memory");   // one row's loads at a time: 64 would fill the registers
     }
   }
-  float4* to = reinterpret_cast<float4*>(a.part + ((h * a.splits + split) * a.chunks + k) * kWin);
+#pragma unroll
+  for (int i = 0; i < 15; ++i) acc[i] += tot[i];
+  float4* to = reinterpret_cast<float4*>(a.part + id * kWin);
   to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
   to[2] = make_float4(acc[8], acc[9], acc[10], acc[11]);
@@ -265,9 +275,9 @@ kat_distance_bias_bwd_kernel(const __grid_constant__ DistanceBwd a) {
 template <typename T>
 __global__ void __launch_bounds__(kBwdThreads)
 kat_distance_bias_bwd_any_kernel(const __grid_constant__ DistanceBwd a) {
-  const int64_t k = int64_t(blockIdx.x) * kBwdThreads + threadIdx.x;
-  if (k >= a.chunks) return;
-  const int64_t split = blockIdx.y, h = blockIdx.z;
+  const int64_t id = int64_t(blockIdx.x) * kBwdThreads + threadIdx.x;
+  if (id >= a.threads) return;
+  const int64_t k = id % a.chunks, split = id / a.chunks % a.splits, h = id / a.chunks / a.splits;
   const int64_t d = k - (a.lq - 1);
   if (a.causal && d > a.offset) return;
   int64_t i0 = split * a.groups * 8, i1 = i0 + int64_t(a.groups) * 8;
@@ -276,41 +286,58 @@ kat_distance_bias_bwd_any_kernel(const __grid_constant__ DistanceBwd a) {
   if (i1 > a.lk - d) i1 = a.lk - d;
   const int64_t step = a.si + a.sj;
   const T* p = static_cast<const T*>(a.dout) + h * a.sh + i0 * a.si + (i0 + d) * a.sj;
-  float sum = 0.0f;
+  float total = 0.0f;
+  while (i0 < i1) {
+    const int64_t end = i0 + 256 < i1 ? i0 + 256 : i1;
+    float sum = 0.0f;
 #pragma unroll 8
-  for (int64_t i = i0; i < i1; ++i, p += step) sum += load_one(p);
-  a.part[(h * a.splits + split) * a.chunks + k] = sum;
+    for (; i0 < end; ++i0, p += step) sum += load_one(p);
+    total += sum;
+  }
+  a.part[id] = total;
 }
 
 // One sum for each diagonal: its splits, in each of which two windows hold it (kVec) or one thread.
+// 32 diagonals to a block, their splits in 8 runs added in order.
 template <bool kVec>
 __global__ void __launch_bounds__(256)
 kat_distance_bias_diag_kernel(const __grid_constant__ DistanceBwd a) {
   const int64_t count = a.lq + a.lk - 1;
-  const int64_t k = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (k >= count) return;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t k = int64_t(blockIdx.x) * 32 + tx;
   const int64_t h = blockIdx.y;
   const int64_t d = k - (a.lq - 1);
   double sum = 0.0;
-  if (!a.causal || d <= a.offset) {
+  if (k < count && (!a.causal || d <= a.offset)) {
+    // from split to split: the next part, and there the window that lies `groups` further
+    const float* part = a.part + (h * a.splits + ty) * a.chunks * (kVec ? kWin : 1);
+    const int splits = int(a.splits);
     if constexpr (kVec) {
-      const int64_t c = d >= 0 ? d / 8 : -((7 - d) / 8);
-      const int o = int(d - 8 * c);
-#pragma unroll 4
-      for (int64_t s = 0; s < a.splits; ++s) {
-        const int64_t at = c + s * a.groups + a.groups - 1;
-        const float* part = a.part + ((h * a.splits + s) * a.chunks + at) * kWin;
-        const float one = at >= 0 && at < a.chunks ? part[o + 7] : 0.0f;
-        const float two = o > 0 && at + 1 >= 0 && at + 1 < a.chunks ? part[kWin + o - 1] : 0.0f;
+      const int c = int(d >= 0 ? d / 8 : -((7 - d) / 8)), o = int(d - 8 * int64_t(c));
+      const int chunks = int(a.chunks);
+      int at = c + ty * a.groups + a.groups - 1;
+      const float* p = part + int64_t(at) * kWin + o;
+      const int64_t step = 8 * (a.chunks + a.groups) * kWin;
+#pragma unroll 2
+      for (int s = ty; s < splits; s += 8, at += 8 * a.groups, p += step) {
+        const float one = unsigned(at) < unsigned(chunks) ? p[7] : 0.0f;
+        const float two = o > 0 && unsigned(at + 1) < unsigned(chunks) ? p[kWin - 1] : 0.0f;
         sum += double(one) + double(two);
       }
     } else {
+      const float* p = part + k;
 #pragma unroll 4
-      for (int64_t s = 0; s < a.splits; ++s)
-        sum += double(a.part[(h * a.splits + s) * a.chunks + k]);
+      for (int s = ty; s < splits; s += 8, p += 8 * a.chunks) sum += double(*p);
     }
   }
-  a.diag[h * count + k] = sum;
+  __shared__ double acc[8][32];
+  acc[ty][tx] = sum;
+  __syncthreads();
+  if (ty == 0 && k < count) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) sum += acc[r][tx];
+    a.diag[h * count + k] = sum;
+  }
 }
 
 // A bucket's run of diagonals, one block.
@@ -345,6 +372,7 @@ kat_distance_bias_run_kernel(const __grid_constant__ DistanceBwd a,
 // ---------------------------------------------------------------------------
 
 constexpr int kIdxThreads = 256;
+constexpr int kIdxBwdThreads = 512;
 constexpr int kIdxSmem = 64 * 1024;       // table columns of a block
 constexpr int kIdxSmemMost = 200 * 1024;  // above this even one column stays in global memory
 
@@ -417,7 +445,7 @@ kat_index_bias_fwd_kernel(const __grid_constant__ IndexFwd a) {
 struct IndexBwd {
   const void* dout;
   int64_t sh, si, sj;
-  int64_t lq, lk, ld;
+  int64_t lq, lk, pitch;   // pitch: cells from row to row in `cells`
   const uint16_t* cells;
   const int32_t* seg_begin;
   const int32_t* slab_begin;
@@ -427,65 +455,50 @@ struct IndexBwd {
   float* part;             // [head][place of the segment]
 };
 
-// kRows: the cells of a row follow each other (any start); each 16 bytes of a row that lie on a
-// 16-byte boundary are loaded at once, four of them in flight, and spread over shared memory.
-template <typename T, bool kRows>
-__global__ void __launch_bounds__(kIdxThreads)
+// kFlat: the slab's rows are one run of memory of the cells' own pitch, which goes to shared memory
+// as it lies there: every 16 bytes on a 16-byte boundary by cp.async, all of them in flight at
+// once, and the cells are read `skew` places further.  (Spreading pieces from registers over padded
+// rows instead cost four times the shared-memory wavefronts: dout[16,1025,1025] fp32 61 us.)
+// Otherwise cell by cell, into rows of the cells' pitch.
+template <typename T, bool kFlat>
+__global__ void __launch_bounds__(kIdxBwdThreads)
 kat_index_bias_bwd_kernel(const __grid_constant__ IndexBwd a) {
   using U = typename Bits<T>::U;
   extern __shared__ uint4 slab_smem[];
-  U* s = reinterpret_cast<U*>(slab_smem);
+  const U* s = reinterpret_cast<const U*>(slab_smem);
   const int64_t h = blockIdx.y;
   const int64_t i0 = int64_t(blockIdx.x) * a.slab_rows;
   const uint32_t rows = uint32_t(a.lq - i0 < a.slab_rows ? a.lq - i0 : a.slab_rows);
   const U* base = static_cast<const U*>(a.dout) + h * a.sh + i0 * a.si;
-  const uint32_t ld = uint32_t(a.ld), lk = uint32_t(a.lk);
-  if constexpr (kRows) {
+  const uint32_t pitch = uint32_t(a.pitch), lk = uint32_t(a.lk);
+  if constexpr (kFlat) {
     constexpr uint32_t kPer = 16 / sizeof(T);
-    constexpr int kFlight = 4;
-    const uint32_t per_row = lk / kPer + 2;   // pieces a row may touch
-    const uint32_t pieces = rows * per_row;
-    for (uint32_t k0 = threadIdx.x; k0 < pieces; k0 += kFlight * kIdxThreads) {
-      uint4 raw[kFlight];
-      int32_t col[kFlight];
-      uint32_t row[kFlight];
-#pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
-        const uint32_t k = k0 + f * kIdxThreads;
-        row[f] = k / per_row;
-        const U* p = base + int64_t(row[f]) * a.si;
-        const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T);
-        col[f] = int32_t((k % per_row) * kPer) - int32_t(skew);
-        if (k < pieces && col[f] >= 0 && col[f] + int32_t(kPer) <= int32_t(lk))
-          raw[f] = load_raw<T, int(kPer)>(reinterpret_cast<const T*>(p + col[f]));
-        else if (k >= pieces)
-          col[f] = int32_t(lk);               // nothing
-      }
-#pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
-        U* to = s + row[f] * ld;
-        if (col[f] >= 0 && col[f] + int32_t(kPer) <= int32_t(lk)) {
-          const uint32_t w[4] = {raw[f].x, raw[f].y, raw[f].z, raw[f].w};
-#pragma unroll
-          for (uint32_t e = 0; e < kPer; ++e)
-            to[col[f] + e] = U(sizeof(T) == 4 ? w[e % 4] : w[(e / 2) % 4] >> (16 * (e & 1)));
-        } else {
-          const U* p = base + int64_t(row[f]) * a.si;
-          for (int32_t j = col[f] < 0 ? 0 : col[f];
-               j < col[f] + int32_t(kPer) && j < int32_t(lk); ++j)
-            to[j] = __ldg(p + j);
-        }
+    const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T);
+    const uint32_t cells = (rows - 1) * pitch + lk;      // up to the last row's last cell
+    U* to = reinterpret_cast<U*>(slab_smem);
+    const uint32_t to0 = static_cast<uint32_t>(__cvta_generic_to_shared(slab_smem));
+    for (uint32_t k = threadIdx.x; k * kPer < cells + skew; k += kIdxBwdThreads) {
+      const int32_t first = int32_t(k * kPer) - int32_t(skew);   // the piece's first cell
+      if (first >= 0 && first + kPer <= cells) {
+        asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(to0 + k * 16u),
+                     "l"(base + first) : "memory");
+      } else {   // the run's ends
+        for (uint32_t e = 0; e < kPer; ++e)
+          if (first + int32_t(e) >= 0 && first + e < cells) to[k * kPer + e] = __ldg(base + first + e);
       }
     }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    s += skew;
   } else {
-    for (uint32_t k = threadIdx.x; k < rows * lk; k += kIdxThreads) {
+    U* to = reinterpret_cast<U*>(slab_smem);
+    for (uint32_t k = threadIdx.x; k < rows * lk; k += kIdxBwdThreads) {
       const uint32_t r = k / lk, j = k % lk;
-      s[r * ld + j] = __ldg(base + int64_t(r) * a.si + int64_t(j) * a.sj);
+      to[r * pitch + j] = __ldg(base + int64_t(r) * a.si + int64_t(j) * a.sj);
     }
   }
   __syncthreads();
   const int32_t end = __ldg(a.slab_begin + blockIdx.x + 1);
-  for (int32_t g = __ldg(a.slab_begin + blockIdx.x) + int(threadIdx.x); g < end; g += kIdxThreads) {
+  for (int32_t g = __ldg(a.slab_begin + blockIdx.x) + int(threadIdx.x); g < end; g += kIdxBwdThreads) {
     float sum = 0.0f;
     const int32_t last = __ldg(a.seg_begin + g + 1);
 #pragma unroll 4
@@ -547,16 +560,17 @@ struct DistancePlan {
   int64_t splits, chunks;
   size_t part, total;
 };
-// Groups of 8 rows in a split: as many as leave enough threads for the whole device.  A window's
-// 15 sums of a split cost 64 bytes (a diagonal's 4) next to the cells that it reads there.
+// Groups of 8 rows in a split: the most that leave the device about two waves of blocks (4 of
+// windows or 16 of diagonals to an SM).  dout[16,4096,4096] bf16, kernel and sum over the splits:
+// 8 groups 99 + 37 us, 16: 101 + 19, 32: 103 + 11, 64 (one wave, its blocks of unequal length):
+// 125 + 6; the sum over the splits has since become quicker.
 DistancePlan distance_plan(int32_t heads, int64_t lq, int64_t lk, bool vec) {
   const int64_t rows8 = (lq + 7) / 8, cols8 = (lk + 7) / 8;
-  const int64_t most = 32, threads = 148 * (vec ? 512 : 2048);
-  int64_t g = most;
+  const double resident = 148.0 * kBwdThreads * (vec ? 4 : 16);
   auto splits = [&](int64_t n) { return (rows8 + n - 1) / n; };
   auto chunks = [&](int64_t n) { return vec ? cols8 + n - 1 : lq + lk - 1; };
-  while (g > 1 && heads * splits(g) * chunks(g) < threads) g /= 2;
-  while (splits(g) > 65535) g *= 2;
+  int64_t g = 1024;
+  while (g > 1 && double(heads) * double(splits(g)) * double(chunks(g)) < 1.75 * resident) g /= 2;
   DistancePlan p;
   p.groups = int32_t(g);
   p.splits = splits(g);
@@ -622,17 +636,17 @@ int launch_index_fwd(IndexFwd a, cudaStream_t st) {
   return launched();
 }
 
-template <typename T, bool kRows>
+template <typename T, bool kFlat>
 int launch_index_bwd_v(const IndexBwd& a, dim3 grid, cudaStream_t st) {
-  const size_t bytes = size_t(a.slab_rows) * size_t(a.ld) * sizeof(T);
-  if (int rc = set_smem(kat_index_bias_bwd_kernel<T, kRows>, bytes)) return rc;
-  kat_index_bias_bwd_kernel<T, kRows><<<grid, kIdxThreads, bytes, st>>>(a);
+  const size_t bytes = size_t(a.slab_rows) * size_t(a.pitch) * sizeof(T) + 16;
+  if (int rc = set_smem(kat_index_bias_bwd_kernel<T, kFlat>, bytes)) return rc;
+  kat_index_bias_bwd_kernel<T, kFlat><<<grid, kIdxBwdThreads, bytes, st>>>(a);
   return launched();
 }
 template <typename T>
 int launch_index_bwd(const IndexBwd& a, dim3 grid, cudaStream_t st) {
-  return a.sj == 1 ? launch_index_bwd_v<T, true>(a, grid, st)
-                   : launch_index_bwd_v<T, false>(a, grid, st);
+  return a.sj == 1 && a.si == a.pitch ? launch_index_bwd_v<T, true>(a, grid, st)
+                                      : launch_index_bwd_v<T, false>(a, grid, st);
 }
 
 }  // namespace
@@ -728,10 +742,12 @@ int kat_distance_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* d
   a.groups = plan.groups;
   a.splits = plan.splits;
   a.chunks = plan.chunks;
+  a.threads = int64_t(heads) * plan.splits * plan.chunks;
   a.part = static_cast<float*>(workspace);
   a.diag = reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + plan.part);
-  const dim3 grid{uint32_t((plan.chunks + kBwdThreads - 1) / kBwdThreads), uint32_t(plan.splits),
-                  uint32_t(heads)};
+  const int64_t blocks = (a.threads + kBwdThreads - 1) / kBwdThreads;
+  if (blocks >= (int64_t(1) << 31)) return KAT_ERR_BAD_SHAPE;
+  const dim3 grid{uint32_t(blocks)};
   int rc = KAT_OK;
   switch (dout_dtype) {
     case KAT_DTYPE_F32: rc = launch_distance_bwd<float>(a, vec, grid, st); break;
@@ -739,7 +755,7 @@ int kat_distance_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* d
     default: rc = launch_distance_bwd<__nv_bfloat16>(a, vec, grid, st); break;
   }
   if (rc) return rc;
-  const dim3 diag_grid{uint32_t((lq + lk - 1 + 255) / 256), uint32_t(heads)};
+  const dim3 diag_grid{uint32_t((lq + lk - 1 + 31) / 32), uint32_t(heads)};
   if (vec) kat_distance_bias_diag_kernel<true><<<diag_grid, 256, 0, st>>>(a);
   else kat_distance_bias_diag_kernel<false><<<diag_grid, 256, 0, st>>>(a);
   kat_distance_bias_run_kernel<<<dim3(uint32_t(num_buckets), uint32_t(heads)), 256, 0, st>>>(
@@ -777,8 +793,9 @@ size_t kat_index_bias_bwd_workspace_bytes(int32_t heads, int64_t segments) {
 
 int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout_stride,
                        int32_t num_buckets, int32_t heads, int64_t lq, int64_t lk,
-                       const uint16_t* cells, const int32_t* seg_begin, int64_t segments,
-                       const int32_t* slab_begin, int64_t slabs, int32_t slab_rows,
+                       const uint16_t* cells, const uint16_t* padded_cells,
+                       const int32_t* seg_begin, int64_t segments, const int32_t* slab_begin,
+                       int64_t slabs, int32_t slab_rows,
                        const int32_t* seg_place, const int32_t* bucket_begin, void* d_table,
                        int32_t table_dtype, void* workspace, size_t workspace_bytes,
                        void* stream) {
@@ -791,7 +808,8 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
                    cudaSuccess
                ? KAT_OK
                : KAT_ERR_CUDA;
-  if (dout == nullptr || dout_stride == nullptr || cells == nullptr || seg_begin == nullptr ||
+  if (dout == nullptr || dout_stride == nullptr || cells == nullptr || padded_cells == nullptr ||
+      seg_begin == nullptr ||
       slab_begin == nullptr || seg_place == nullptr || bucket_begin == nullptr)
     return KAT_ERR_NULL_POINTER;
   const int64_t ld = round8(lk);
@@ -809,8 +827,8 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
   a.sj = dout_stride[2];
   a.lq = lq;
   a.lk = lk;
-  a.ld = ld;
-  a.cells = cells;
+  a.pitch = dout_stride[1] == ld ? ld : lk;
+  a.cells = a.pitch == ld ? padded_cells : cells;
   a.seg_begin = seg_begin;
   a.slab_begin = slab_begin;
   a.seg_place = seg_place;

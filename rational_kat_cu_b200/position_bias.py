@@ -163,7 +163,9 @@ class IndexBuckets:
         row, col = at // max(ld, 1), at % max(ld, 1)
         key = row // self.slab_rows * num_buckets + flat[at]
         key, order = key.sort(stable=True)
-        cells = ((row % self.slab_rows) * ld + col)[order]
+        in_slab = row % self.slab_rows
+        cells, padded_cells = ((in_slab * pitch + col)[order].to(torch.uint16)
+                               for pitch in (lk, ld))
         n = key.numel()
         place = torch.arange(n, device=dev)
         new = torch.ones(n, dtype=torch.bool, device=dev)
@@ -177,7 +179,8 @@ class IndexBuckets:
         seg_place[by_bucket] = torch.arange(self.segments, device=dev)
         self._tensors = (
             padded,
-            cells.to(torch.uint16),
+            cells,
+            padded_cells if ld != lk else cells,
             torch.cat([begin, torch.tensor([n], device=dev)]).to(torch.int32),
             torch.searchsorted(seg_slab, torch.arange(self.slabs + 1, device=dev)).to(torch.int32),
             seg_place.to(torch.int32),
@@ -186,7 +189,7 @@ class IndexBuckets:
         self._on: Dict[torch.device, Tuple[Tensor, ...]] = {dev: self._tensors}
 
     def on(self, device: torch.device) -> Tuple[Tensor, ...]:
-        """(index, cells, seg_begin, slab_begin, seg_place, bucket_begin) on `device`, kept there
+        """(index, cells, padded_cells, seg_begin, slab_begin, seg_place, bucket_begin) on `device`, kept there
         (the first use on a device copies them: not inside a graph capture)."""
         if device not in self._on:
             self._on[device] = tuple(t.to(device) for t in self._tensors)
@@ -298,15 +301,16 @@ class IndexBiasFunction(torch.autograd.Function):
     def backward(ctx, grad: Tensor):
         b, heads, dtype = ctx.args
         lib, device = _native.lib(), grad.device
-        _, cells, seg_begin, slab_begin, seg_place, bucket_begin = b.on(device)
+        _, cells, padded, seg_begin, slab_begin, seg_place, bucket_begin = b.on(device)
         d = torch.empty((b.num_buckets, heads), device=device, dtype=dtype)
         size = lib.kat_index_bias_bwd_workspace_bytes(heads, b.segments)
         ws = torch.empty(size, device=device, dtype=torch.uint8)
         _native.check("kat_index_bias_bwd", _native.on_stream(
             device, lib.kat_index_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
-            b.num_buckets, heads, b.shape[0], b.shape[1], cells.data_ptr(), seg_begin.data_ptr(),
-            b.segments, slab_begin.data_ptr(), b.slabs, b.slab_rows, seg_place.data_ptr(),
-            bucket_begin.data_ptr(), d.data_ptr(), DTYPES[dtype], ws.data_ptr(), size))
+            b.num_buckets, heads, b.shape[0], b.shape[1], cells.data_ptr(),
+            padded.data_ptr(), seg_begin.data_ptr(), b.segments, slab_begin.data_ptr(), b.slabs,
+            b.slab_rows, seg_place.data_ptr(), bucket_begin.data_ptr(), d.data_ptr(),
+            DTYPES[dtype], ws.data_ptr(), size))
         return d, None, None
 
 

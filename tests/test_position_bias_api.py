@@ -56,7 +56,7 @@ def test_index_buckets_list_every_cell_once(lq, lk, nb):
     g = torch.Generator().manual_seed(lq)
     index = torch.randint(-1, nb, (lq, lk), generator=g)
     b = kat.IndexBuckets(index, nb)
-    padded, cells, seg_begin, slab_begin, seg_place, bucket_begin = b.on(index.device)
+    padded, plain, cells, seg_begin, slab_begin, seg_place, bucket_begin = b.on(index.device)
     ld = (lk + 7) // 8 * 8
     assert padded.shape == (lq, ld) and (padded[:, lk:] == nb).all()
     assert b.slab_rows * ld <= position_bias.SLAB_CELLS or b.slab_rows == 1
@@ -69,6 +69,7 @@ def test_index_buckets_list_every_cell_once(lq, lk, nb):
             assert 0 < end - begin <= position_bias.SEGMENT
             at = cells[begin:end].long()
             row, col = s * b.slab_rows + at // ld, at % ld
+            assert torch.equal(plain[begin:end].long(), at // ld * lk + col)
             assert (row < lq).all() and (col < lk).all()
             seen[row, col] += 1
             values = index[row, col]
@@ -124,9 +125,9 @@ def test_entry_points_refuse():
     def ifwd(table=P, tdt=0, nb=4, heads=2, index=P, lq=5, lk=6, out=P, odt=0):
         return lib.kat_index_bias_fwd(table, tdt, nb, heads, index, lq, lk, out, odt, None)
 
-    def ibwd(dout=P, ddt=0, st=stride, nb=4, heads=2, lq=5, lk=6, cells=P, sb=P, segs=9, slb=P,
+    def ibwd(dout=P, ddt=0, st=stride, nb=4, heads=2, lq=5, lk=6, cells=P, pc=P, sb=P, segs=9, slb=P,
              slabs=1, rows=5, bb=P, bkb=P, dt=P, tdt=0, ws=P, size=1 << 20):
-        return lib.kat_index_bias_bwd(dout, ddt, st, nb, heads, lq, lk, cells, sb, segs, slb,
+        return lib.kat_index_bias_bwd(dout, ddt, st, nb, heads, lq, lk, cells, pc, sb, segs, slb,
                                       slabs, rows, bb, bkb, dt, tdt, ws, size, None)
 
     for f in (dfwd, dbwd, ifwd, ibwd):
@@ -137,7 +138,7 @@ def test_entry_points_refuse():
         assert f(heads=0) == E.KAT_OK
     for f, names in ((dfwd, ("table", "of", "out")), (dbwd, ("dout", "st", "rb", "re", "dt")),
                      (ifwd, ("table", "index", "out")),
-                     (ibwd, ("dout", "st", "cells", "sb", "slb", "bb", "bkb", "dt"))):
+                     (ibwd, ("dout", "st", "cells", "pc", "sb", "slb", "bb", "bkb", "dt"))):
         for name in names:
             assert f(**{name: None}) == E.KAT_ERR_NULL_POINTER
     for f in (dfwd, ifwd):
