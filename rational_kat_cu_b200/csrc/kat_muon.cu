@@ -1,14 +1,28 @@
 // kat_muon.cu — Newton-Schulz orthogonalisation of matrix updates (C ABI: include/kat_muon.h).
 //
-// A call takes up to 64 matrices of one shape.  Two elementwise kernels bring the update into
+// A call takes up to 64 matrices of one shape, m <= n.  Two elementwise kernels bring the update into
 // the working form (the momentum update with the sums of squares, then scaling and splitting into
-// planes), then every step is three batched products on the tensor cores:
-//   gram    A  = X X^T          both operands rows of X
-//   poly    B  = b A + c A A    both operands rows of A (A is symmetric)
-//   apply   X' = a X + B X      rows of B against X itself, read with its columns contiguous
-//                               (an MN-major shared-memory operand), so X is never transposed
-// gram and poly are symmetric: only the tiles on and below the diagonal are computed, and each
-// is written twice, once transposed.  The last apply writes the output or updates the weights.
+// planes); all else is batched products on the tensor cores.  One step of the iteration is
+//   gram    A  = X X^T                  both operands rows of X
+//   poly    P  = a I + b A + c A A      both operands rows of A (A is symmetric)
+//   apply   X' = P X                    rows of P against X itself, read with its columns contiguous
+//                                       (an MN-major shared-memory operand): X is never transposed
+// gram, poly and all other m x m products are symmetric: only the tiles on and below the diagonal
+// are computed, and each is written twice, once transposed.  The last apply writes the output or
+// updates the weights.
+//
+// Wide matrices take up to three steps at once on the Gram matrix: the next step's is
+// A' = P A P (all of these commute), and X is multiplied once by the product of the P's:
+// 6 m^2 n + 14 m^3 operations for five steps in blocks of 3 and 2, instead of 15 m^2 n + 5 m^3
+// (products of two factors counted by halves).  Taking all five steps at once would cost
+// 3 m^2 n + 17 m^3 but loses digits where the singular values spread (relative error 2.7e-4 against
+// 1.4e-5 of fp32 products for singular values 1 / k; blocks of 3 and 2: 1.3e-5).
+//
+// Each product of two split matrices takes three MMAs (hi hi, hi lo, lo hi) on four operand planes.
+// With one CTA to a 128 x 128 tile the planes' way from L2 is what bounds it (64 KB a k-block for
+// 768 cycles of MMA); a CTA pair (cta_group::2) on a 256 x 256 tile loads the same bytes for twice
+// the MMAs.  Launches overlap by programmatic dependent launch: a kernel sets up its barriers and
+// tensor memory while the one before it ends.
 
 #include <cuda.h>  // CUtensorMap and its enums (types only: the encoder is fetched at run time)
 #include <cuda_runtime.h>
@@ -31,8 +45,7 @@ constexpr int kMaxMats = KAT_MUON_MAX_MATRICES;
 constexpr int64_t kMaxDim = 65536;
 constexpr int kMaxSteps = 32;
 
-constexpr int kTM = 128;   // output tile rows (MMA M, TMEM lanes)
-constexpr int kTN = 128;   // output tile columns (MMA N, TMEM columns of one accumulator)
+constexpr int kTM = 128;   // operand rows of a CTA: its tile rows, and its share of the columns
 constexpr int kTK = 64;    // k-block: 64 fp16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
 constexpr int kStages = 3;
@@ -40,21 +53,19 @@ constexpr uint32_t kPlaneBytes = kTM * kTK * 2;        // one operand plane of a
 constexpr uint32_t kStageBytes = 4 * kPlaneBytes;      // P hi, P lo, Q hi, Q lo
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
-constexpr uint32_t kTmemCols = 2 * kTN;
 constexpr uint32_t kSmemBytes = 1024 + kStages * kStageBytes + 256;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
-static_assert(kTM == kTN, "symmetric tiles are square");
 constexpr long long kWaitCycles = 4000000000LL;
 
-// Planes hold value x 2^14: the iterates' entries stay below 1.25, those of A below 1.5 and those
-// of bA + cA^2 below 2.9, so 2^14 keeps the largest under fp16's 65504 and leaves the most bits
-// above its subnormals.
+// Planes of X, A and P hold value x 2^14: the iterates' entries stay below 1.25, those of A below 1.5
+// and those of P below 3.45, so 2^14 keeps the largest under fp16's 65504 and leaves the most bits
+// above its subnormals.  A product of k P's reaches 3.45^k and holds value x 2^(16 - 2k).
 constexpr float kScale = 16384.0f;
-constexpr float kInvScale = 1.0f / 16384.0f;
+constexpr int kMaxBlock = 3;   // steps taken on the Gram matrix at once
 
 __device__ int g_muon_status;
 
-enum Mode { kGram = 0, kPoly = 1, kApply = 2, kFinal = 3 };
+enum Mode { kSym = 0, kPoly = 1, kApply = 2, kFinal = 3 };
 
 struct PtrTable {
   const void* p[kMaxMats];
@@ -132,28 +143,94 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
+template <int kPair>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(slot)), "r"(cols) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if constexpr (kPair == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
 }
+template <int kPair>
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols)
-               : "memory");
+  if constexpr (kPair == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols)
+                 : "memory");
+  } else {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols)
+                 : "memory");
+  }
 }
 // D[tmem] (+)= P[smem] Q[smem]^T for one K = 16 slice, fp16 operands.
+template <int kPair>
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t p_desc, uint64_t q_desc,
                                          uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kPair == 1) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+// Arrive on the mbarrier at shared::cluster address `bar` when every MMA this thread issued so far
+// has completed.
+template <int kPair>
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+  if constexpr (kPair == 1) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                     bar) : "memory");
+  } else {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                     bar) : "memory");
+  }
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" :::
+                   "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+// Load into this CTA's shared memory whose completion is counted on the pair's rank-0 barrier.
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar,
+                                                 int32_t x, int32_t y, int32_t z) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate)
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar)) : "memory");
+// Programmatic dependent launch: let the next kernel's blocks start; wait until the kernel before
+// has completed and its writes are visible.
+__device__ __forceinline__ void pdl_launch_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 // 16 consecutive fp32 columns of this thread's TMEM lane, complete on return.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
@@ -184,10 +261,10 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
          (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 // Instruction descriptor: fp32 accumulator (bits 4-5 = 1), fp16 operands (7-9, 10-12 = 0), B's
-// major-ness in bit 16, N >> 3 in 17-22, M >> 4 in 24-28.
-__host__ __device__ constexpr uint32_t idesc_of(bool mn_major_q) {
-  return (1u << 4) | (mn_major_q ? (1u << 16) : 0u) | (uint32_t(kTN >> 3) << 17) |
-         (uint32_t(kTM >> 4) << 24);
+// major-ness in bit 16, N >> 3 in 17-22, M >> 4 in 24-28; tiles are 128 or (a CTA pair) 256 square.
+__host__ __device__ constexpr uint32_t idesc_of(bool mn_major_q, int pair) {
+  return (1u << 4) | (mn_major_q ? (1u << 16) : 0u) | (uint32_t((kTM * pair) >> 3) << 17) |
+         (uint32_t((kTM * pair) >> 4) << 24);
 }
 
 // ---------------------------------------------------------------------------
@@ -204,9 +281,7 @@ __device__ __forceinline__ uint32_t pack2(__half a, __half b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 // 8 values of both planes added up.
-__device__ __forceinline__ void join8(const __half* hi, const __half* lo, float (&v)[8]) {
-  const uint4 h = *reinterpret_cast<const uint4*>(hi);
-  const uint4 l = *reinterpret_cast<const uint4*>(lo);
+__device__ __forceinline__ void join8(const uint4& h, const uint4& l, float (&v)[8]) {
   const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -250,23 +325,75 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 constexpr int kNormThreads = 256;
 constexpr int kNormBlocks = 64;  // partial sums of one matrix
 
+// V neighbouring values as fp32: 8 at once where the matrices start on 16 bytes, else one.
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* p, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = load1(p);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const float4 v = reinterpret_cast<const float4*>(p)[q];
+      f[4 * q] = v.x; f[4 * q + 1] = v.y; f[4 * q + 2] = v.z; f[4 * q + 3] = v.w;
+    }
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 h = Codec<T>::unpack_word(w[q]);
+      f[2 * q] = h.x;
+      f[2 * q + 1] = h.y;
+    }
+  }
+}
+
+// The update at element i, momentum already renewed.
+template <typename T, int V>
+__device__ __forceinline__ void load_update(const Update& u, const T* x, const float* m, int64_t i,
+                                            float (&f)[V]) {
+  load_values<T, V>(x + i, f);
+  if (u.has_momentum) {
+    float mom[V];
+    load_values<float, V>(m + i, mom);
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = u.nesterov ? fmaf(u.mu, mom[k], f[k]) : mom[k];
+  }
+}
+
 // m <- mu m + g, and each block's sum of the squared update in fp64 (a gradient's square may
 // leave fp32's range, and its norm is what all else is divided by).
-template <typename T>
+template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads)
 kat_muon_norm_kernel(const __grid_constant__ Update u, double* __restrict__ partial) {
+  pdl_launch_next();
   const T* x = static_cast<const T*>(u.x.p[blockIdx.y]);
   float* m = static_cast<float*>(const_cast<void*>(u.m.p[blockIdx.y]));
   double sum = 0.0;
-  for (int64_t i = int64_t(blockIdx.x) * kNormThreads + threadIdx.x; i < u.size;
-       i += int64_t(gridDim.x) * kNormThreads) {
-    float v = load1(x + i);
+#pragma unroll 2
+  for (int64_t i = (int64_t(blockIdx.x) * kNormThreads + threadIdx.x) * V; i < u.size;
+       i += int64_t(gridDim.x) * kNormThreads * V) {
+    float f[V];
+    load_values<T, V>(x + i, f);
     if (u.has_momentum) {
-      const float mom = fmaf(u.mu, m[i], v);
-      m[i] = mom;
-      v = u.nesterov ? fmaf(u.mu, mom, v) : mom;
+      float mom[V];
+      load_values<float, V>(m + i, mom);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        mom[k] = fmaf(u.mu, mom[k], f[k]);
+        f[k] = u.nesterov ? fmaf(u.mu, mom[k], f[k]) : mom[k];
+      }
+      if constexpr (V == 1) {
+        m[i] = mom[0];
+      } else {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q)
+          reinterpret_cast<float4*>(m + i)[q] =
+              make_float4(mom[4 * q], mom[4 * q + 1], mom[4 * q + 2], mom[4 * q + 3]);
+      }
     }
-    sum += double(v) * double(v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum += double(f[k]) * double(f[k]);
   }
   __shared__ double s[kNormThreads / 32];
 #pragma unroll
@@ -279,65 +406,76 @@ kat_muon_norm_kernel(const __grid_constant__ Update u, double* __restrict__ part
   }
 }
 
-constexpr int kSplitTile = 32;
+// 2^14 / |u|_F of a matrix, by one warp: 0 for a zero update, NaN where the sum is.
+__device__ __forceinline__ double scale_of(const double* partial, int blocks) {
+  const int lane = threadIdx.x & 31;
+  double sum = (lane < blocks ? partial[lane] : 0.0) + (lane + 32 < blocks ? partial[lane + 32] : 0.0);
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+  return sum > 0.0 ? double(kScale) / sqrt(sum) : (sum == 0.0 ? 0.0 : sum);
+}
+static_assert(kNormBlocks == 64, "scale_of adds two partial sums a lane");
+
+constexpr int kSplitTile = 64;
+constexpr int kSplitThreads = 256;
 
 // The scaled update in planes: X[i][j] = u / |u|_F x 2^14, rows i < m, leading dimension ld; where
-// `transposed`, X = u^T.  Tiles go through shared memory so that both sides are read and written
-// along their rows.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// `transposed`, X = u^T.  64 x 64 tiles go through shared memory, so that both sides are read and
+// written along their rows, 8 values a thread.
+template <typename T, int V>
+__global__ void __launch_bounds__(kSplitThreads)
 kat_muon_split_kernel(const __grid_constant__ Update u, const double* __restrict__ partial,
                       int norm_blocks, __half* __restrict__ planes, int64_t rows, int64_t cols,
                       int64_t ld, int64_t plane, int transposed, int col_tiles) {
+  pdl_launch_next();
+  pdl_wait_previous();
   const int mat = blockIdx.y;
   __shared__ double s_scale;
   __shared__ float tile[kSplitTile][kSplitTile + 1];
-  if (threadIdx.x == 0) {
-    double sum = 0.0;
-    for (int b = 0; b < norm_blocks; ++b) sum += partial[int64_t(mat) * kNormBlocks + b];
-    s_scale = sum > 0.0 ? double(kScale) / sqrt(sum) : (sum == 0.0 ? 0.0 : sum);
+  if (threadIdx.x < 32) {
+    const double v = scale_of(partial + int64_t(mat) * kNormBlocks, norm_blocks);
+    if (threadIdx.x == 0) s_scale = v;
   }
-  __syncthreads();
-  const double scale = s_scale;
   const T* x = static_cast<const T*>(u.x.p[mat]);
   const float* m = static_cast<const float*>(u.m.p[mat]);
   const int64_t r0 = int64_t(blockIdx.x / col_tiles) * kSplitTile;
   const int64_t c0 = int64_t(blockIdx.x % col_tiles) * kSplitTile;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  constexpr int kAcross = kSplitTile / V;                 // pieces of a tile's row
+  constexpr int kPasses = kSplitTile * kAcross / kSplitThreads;
+  const int px = threadIdx.x % kAcross, py = threadIdx.x / kAcross;
 #pragma unroll
-  for (int k = 0; k < kSplitTile; k += 8) {
-    const int64_t r = r0 + ty + k, c = c0 + tx;
-    float v = 0.0f;
-    if (r < rows && c < cols) {
-      const int64_t i = r * cols + c;
-      v = load1(x + i);
-      if (u.has_momentum) v = u.nesterov ? fmaf(u.mu, m[i], v) : m[i];
-      v = float(double(v) * scale);  // the norm may lie outside fp32's range
-    }
-    tile[ty + k][tx] = v;
+  for (int k = 0; k < kPasses; ++k) {
+    const int tr = py + k * (kSplitThreads / kAcross);
+    const int64_t r = r0 + tr, c = c0 + px * V;
+    float f[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = 0.0f;
+    if (r < rows && c < cols) load_update<T, V>(u, x, m, r * cols + c, f);  // cols % V == 0
+#pragma unroll
+    for (int e = 0; e < V; ++e) tile[tr][px * V + e] = f[e];
   }
   __syncthreads();
+  const double scale = s_scale;
   __half* hi = planes + int64_t(mat) * 2 * plane;
   __half* lo = hi + plane;
+  const int64_t i0 = transposed ? c0 : r0, j0 = transposed ? r0 : c0;
+  const int64_t height = transposed ? cols : rows;
 #pragma unroll
-  for (int k = 0; k < kSplitTile; k += 8) {
-    int64_t i, j;
-    float v;
-    if (transposed) {
-      i = c0 + ty + k;
-      j = r0 + tx;
-      v = tile[tx][ty + k];
-      if (i >= cols || j >= rows) continue;
-    } else {
-      i = r0 + ty + k;
-      j = c0 + tx;
-      v = tile[ty + k][tx];
-      if (i >= rows || j >= cols) continue;
+  for (int k = 0; k < kSplitTile * kSplitTile / 8 / kSplitThreads; ++k) {
+    const int piece = threadIdx.x + k * kSplitThreads;
+    const int ti = piece / 8, tj = piece % 8 * 8;
+    const int64_t i = i0 + ti, j = j0 + tj;
+    if (i >= height || j >= ld) continue;                // ld is a multiple of 8
+    __half h[8], l[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = transposed ? tile[tj + e][ti] : tile[ti][tj + e];
+      split(float(double(f) * scale), h[e], l[e]);       // the norm may lie outside fp32's range
     }
-    __half h, l;
-    split(v, h, l);
-    hi[i * ld + j] = h;
-    lo[i * ld + j] = l;
+    *reinterpret_cast<uint4*>(hi + i * ld + j) =
+        make_uint4(pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
+    *reinterpret_cast<uint4*>(lo + i * ld + j) =
+        make_uint4(pack2(l[0], l[1]), pack2(l[2], l[3]), pack2(l[4], l[5]), pack2(l[6], l[7]));
   }
 }
 
@@ -347,12 +485,15 @@ kat_muon_split_kernel(const __grid_constant__ Update u, const double* __restrict
 
 struct GemmArgs {
   int32_t m, n;            // output rows and columns of a matrix
-  int32_t row_tiles, col_tiles, tiles;  // of one matrix; `tiles` counts the computed ones
-  int32_t total_tiles;     // over all matrices
+  int32_t row_tiles;
+  int32_t tiles;           // computed tiles of one matrix
+  int32_t set_tiles;       // of all matrices of one set of operands
+  int32_t total_tiles;     // of both sets
   int32_t k_blocks;
-  const __half* in;        // planes the epilogue adds (poly: A, apply: X), leading dimension ld
-  __half* out;             // planes written
-  int64_t ld, plane;       // of both
+  float mult[2];           // accumulator -> plane (or, last, output) value, by set
+  const __half* in;        // poly: planes of A, leading dimension and plane as the output's
+  __half* out[2];          // planes written, by set
+  int64_t ld, plane;
   // final step
   int32_t transposed;
   int64_t out_ld;          // columns of the caller's matrices
@@ -362,63 +503,91 @@ struct GemmArgs {
   const float* lr_device;
 };
 
+constexpr int kPiece = 32;   // columns a warp takes from the accumulator at once
+
+// A thread's kPiece output values of one row (col .. col + 31): the weights they are added to,
+// loaded before the accumulator is waited for ...
 template <typename T>
-__device__ __forceinline__ void final_store(const GemmArgs& args, const PtrTable& outs, int mat,
-                                            int row, int col, const float (&o)[8], float lr) {
-  T* base = static_cast<T*>(const_cast<void*>(outs.p[mat]));
-  const float keep = 1.0f - lr * args.weight_decay, step = lr * args.scale;
+__device__ __forceinline__ void load_weights(const GemmArgs& args, const PtrTable& outs, int mat,
+                                             int row, int col, float (&w)[kPiece]) {
+  const T* base = static_cast<const T*>(outs.p[mat]);
+  if (row >= args.m) return;
   if (args.transposed) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (col + k >= args.n) break;
-      T* p = base + int64_t(col + k) * args.out_ld + row;
-      *p = from_float<T>(args.has_momentum ? fmaf(keep, load1(p), -step * o[k]) : o[k]);
-    }
-  } else if (args.vec && col + 8 <= args.n) {
-    T* p = base + int64_t(row) * args.out_ld + col;
-    union { uint4 q[sizeof(T) / 2]; T e[8]; } w;
-    if (args.has_momentum) {
+    for (int k = 0; k < kPiece; ++k)
+      if (col + k < args.n) w[k] = load1(base + int64_t(col + k) * args.out_ld + row);
+  } else {
+    const T* p = base + int64_t(row) * args.out_ld + col;
+    if (args.vec) {
 #pragma unroll
-      for (int q = 0; q < int(sizeof(T) / 2); ++q) w.q[q] = reinterpret_cast<const uint4*>(p)[q];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        w.e[k] = from_float<T>(fmaf(keep, load1(&w.e[k]), -step * o[k]));
+      for (int g = 0; g < kPiece / 8; ++g)
+        if (col + g * 8 < args.n)
+          load_values<T, 8>(p + g * 8, *reinterpret_cast<float(*)[8]>(&w[g * 8]));
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w.e[k] = from_float<T>(o[k]);
+      for (int k = 0; k < kPiece; ++k)
+        if (col + k < args.n) w[k] = load1(p + k);
     }
+  }
+}
+// ... and the results written.
+template <typename T>
+__device__ __forceinline__ void store_result(const GemmArgs& args, const PtrTable& outs, int mat,
+                                             int row, int col, const float (&o)[kPiece]) {
+  T* base = static_cast<T*>(const_cast<void*>(outs.p[mat]));
+  if (row >= args.m) return;
+  if (args.transposed) {
 #pragma unroll
-    for (int q = 0; q < int(sizeof(T) / 2); ++q) reinterpret_cast<uint4*>(p)[q] = w.q[q];
+    for (int k = 0; k < kPiece; ++k)
+      if (col + k < args.n) base[int64_t(col + k) * args.out_ld + row] = from_float<T>(o[k]);
   } else {
+    T* p = base + int64_t(row) * args.out_ld + col;
+    if (args.vec) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (col + k >= args.n) break;
-      T* p = base + int64_t(row) * args.out_ld + col + k;
-      *p = from_float<T>(args.has_momentum ? fmaf(keep, load1(p), -step * o[k]) : o[k]);
+      for (int g = 0; g < kPiece / 8; ++g) {
+        if (col + g * 8 < args.n) {
+          union { uint4 q[sizeof(T) / 2]; T e[8]; } v;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v.e[k] = from_float<T>(o[g * 8 + k]);
+#pragma unroll
+          for (int q = 0; q < int(sizeof(T) / 2); ++q)
+            reinterpret_cast<uint4*>(p + g * 8)[q] = v.q[q];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k)
+        if (col + k < args.n) p[k] = from_float<T>(o[k]);
     }
   }
 }
 
-template <int kMode, typename T>
+template <int kMode, typename T, int kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
-                     const __grid_constant__ CUtensorMap tm_q,
+                     const __grid_constant__ CUtensorMap tm_q0,
+                     const __grid_constant__ CUtensorMap tm_q1,
                      const __grid_constant__ GemmArgs args,
                      const __grid_constant__ PtrTable outs) {
-  constexpr bool kSym = kMode == kGram || kMode == kPoly;
+  constexpr bool kMirror = kMode == kSym || kMode == kPoly;
+  constexpr int kTile = kTM * kPair;                  // output tile, square
+  constexpr uint32_t kTmemCols = 2 * kTile;           // two accumulators
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* tfull = empty + kStages;
-  uint64_t* tempty = tfull + 2;
+  uint64_t* empty = full + kStages;   // in each CTA
+  uint64_t* tfull = empty + kStages;  // in each CTA
+  uint64_t* tempty = tfull + 2;       // rank 0's counts the epilogue warps of both CTAs
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  pdl_launch_next();
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const uint32_t rank = kPair == 2 ? cluster_rank() : 0u;
+  const int slot0 = int(blockIdx.x) / kPair, slots = int(gridDim.x) / kPair;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -427,25 +596,29 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     }
     for (int j = 0; j < 2; ++j) {
       mbar_init(tfull + j, 1);
-      mbar_init(tempty + j, kEpiWarps);
+      mbar_init(tempty + j, kPair * kEpiWarps);
     }
     mbar_init(drain, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&tm_p);
-    prefetch_map(&tm_q);
+    prefetch_map(&tm_q0);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == 1) tmem_alloc<kPair>(tmem_slot, kTmemCols);
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair == 2) cluster_sync();  // the peer's barriers exist before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait_previous();
 
-  // Tile -> matrix, row tile, column tile (row >= column where the product is symmetric).
-  auto locate = [&](int tile, int& mat, int& tr, int& tc) {
+  // Tile -> set, matrix, row tile, column tile (row >= column where the product is symmetric).
+  auto locate = [&](int tile, int& set, int& mat, int& tr, int& tc) {
+    set = kMode == kSym && tile >= args.set_tiles ? 1 : 0;
+    if (set) tile -= args.set_tiles;
     mat = tile / args.tiles;
     const int t = tile - mat * args.tiles;
-    if (kSym) {
+    if (kMirror) {
       tr = int((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);
       while ((tr + 1) * (tr + 2) / 2 <= t) ++tr;
       while (tr * (tr + 1) / 2 > t) --tr;
@@ -457,76 +630,87 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   };
 
   if (warp == 0) {
-    // ---------------- TMA producer ----------------
+    // ---------------- TMA producer: this CTA's 128 rows of P, its 128 rows or columns of Q ------
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true, wrapped = false;
-      for (int tile = blockIdx.x; tile < args.total_tiles && ok; tile += gridDim.x) {
-        int mat, tr, tc;
-        locate(tile, mat, tr, tc);
+      for (int tile = slot0; tile < args.total_tiles && ok; tile += slots) {
+        int set, mat, tr, tc;
+        locate(tile, set, mat, tr, tc);
+        const CUtensorMap* tm_q = set ? &tm_q1 : &tm_q0;
+        const int p0 = tr * kTile + int(rank) * kTM, q0 = tc * kTile + int(rank) * kTM;
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!wait_phase(empty + stage, phase ^ 1u, abort)) { ok = false; break; }
           uint8_t* s = smem + stage * kStageBytes;
-          mbar_expect_tx(full + stage, kStageBytes);
+          uint32_t bar = smem_u32(full + stage);
+          if constexpr (kPair == 2) bar = cluster_addr(full + stage, 0);
+          if (rank == 0) mbar_expect_tx(full + stage, kPair * kStageBytes);
+          auto load = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
+            if constexpr (kPair == 1) tma_load_3d(dst, map, full + stage, x, y, z);
+            else tma_load_3d_pair(dst, map, bar, x, y, z);
+          };
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
-            tma_load_3d(s + h * kPlaneBytes, &tm_p, full + stage, kb * kTK, tr * kTM,
-                        2 * mat + h);
+            load(s + h * kPlaneBytes, &tm_p, kb * kTK, p0, 2 * mat + h);
             uint8_t* q = s + (2 + h) * kPlaneBytes;
-            if (kSym) {
-              tma_load_3d(q, &tm_q, full + stage, kb * kTK, tc * kTN, 2 * mat + h);
+            if (kMirror) {
+              load(q, tm_q, kb * kTK, q0, 2 * mat + h);
             } else {
-              tma_load_3d(q, &tm_q, full + stage, tc * kTN, kb * kTK, 2 * mat + h);
-              tma_load_3d(q + kBoxBytes, &tm_q, full + stage, tc * kTN + 64, kb * kTK,
-                          2 * mat + h);
+              load(q, tm_q, q0, kb * kTK, 2 * mat + h);
+              load(q + kBoxBytes, tm_q, q0 + 64, kb * kTK, 2 * mat + h);
             }
           }
           if (++stage == kStages) { stage = 0; phase ^= 1u; wrapped = true; }
         }
       }
-      if (!ok) {
-        // given up: the copies in flight land before the block ends
+      if (!ok && rank == 0) {
+        // given up: the copies in flight land before the block (or the pair) ends
         for (int s = 0; s < kStages; ++s)
           if (s < stage || wrapped) drain_phase(full + s, s < stage ? phase : phase ^ 1u);
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    // ---------------- MMA issuer (rank 0 of a pair issues for both CTAs) ----------------
+    if (lane == 0 && rank == 0) {
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool issued = false, ok = true;
-      for (int tile = blockIdx.x; tile < args.total_tiles && ok; tile += gridDim.x, ++local) {
+      auto commit_all = [&](uint64_t* bar) {
+        umma_commit<kPair>(kPair == 1 ? smem_u32(bar) : cluster_addr(bar, 0));
+        if constexpr (kPair == 2) umma_commit<kPair>(cluster_addr(bar, 1));
+      };
+      for (int tile = slot0; tile < args.total_tiles && ok; tile += slots, ++local) {
         const int acc = local & 1;
         if (!wait_phase(tempty + acc, ((local >> 1) & 1) ^ 1u, abort)) break;
         tc_fence_after();
-        const uint32_t d = tmem_base + uint32_t(acc * kTN);
+        const uint32_t d = tmem_base + uint32_t(acc * kTile);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!wait_phase(full + stage, phase, abort)) { ok = false; break; }
           tc_fence_after();
           const uint32_t s = smem_u32(smem + stage * kStageBytes);
           const uint64_t p_hi = desc_k(s), p_lo = desc_k(s + kPlaneBytes);
-          const uint64_t q_hi = kSym ? desc_k(s + 2 * kPlaneBytes) : desc_mn(s + 2 * kPlaneBytes);
-          const uint64_t q_lo = kSym ? desc_k(s + 3 * kPlaneBytes) : desc_mn(s + 3 * kPlaneBytes);
+          const uint64_t q_hi = kMirror ? desc_k(s + 2 * kPlaneBytes) : desc_mn(s + 2 * kPlaneBytes);
+          const uint64_t q_lo = kMirror ? desc_k(s + 3 * kPlaneBytes) : desc_mn(s + 3 * kPlaneBytes);
           // a K = 16 slice further: 32 bytes inside the swizzled rows (K-major), two 8-k groups
           // (MN-major)
-          constexpr uint64_t kStepP = 32 >> 4, kStepQ = kSym ? (32 >> 4) : (2048 >> 4);
-          constexpr uint32_t idesc = idesc_of(!kSym);
+          constexpr uint64_t kStepP = 32 >> 4, kStepQ = kMirror ? (32 >> 4) : (2048 >> 4);
+          constexpr uint32_t idesc = idesc_of(!kMirror, kPair);
 #pragma unroll
           for (int k = 0; k < kTK / kUmmaK; ++k) {
-            umma_f16(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, (kb | k) != 0 ? 1u : 0u);
-            umma_f16(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u);
-            umma_f16(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u);
+            umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u);
+            umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u);
           }
           issued = true;
-          umma_commit(empty + stage);
+          commit_all(empty + stage);
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
-        if (ok) umma_commit(tfull + acc);
+        if (ok) commit_all(tfull + acc);
       }
       if (issued) {
         // Every MMA has completed before the tensor memory is freed.
-        umma_commit(drain);
+        umma_commit<kPair>(kPair == 1 ? smem_u32(drain) : cluster_addr(drain, 0));
         drain_phase(drain, 0);
       }
     }
@@ -536,52 +720,97 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     const int quad = warp & 3;
     const int half = ew >> 2;
     const uint32_t lane_addr = tmem_base + (uint32_t(quad * 32) << 16);
-    const float lr = kMode == kFinal && args.has_momentum && args.lr_device != nullptr
-                         ? *args.lr_device : args.lr;
+    constexpr int kPieces = kTile / 2 / kPiece;   // of this warp's half of the columns
+    float keep = 0.0f, step = 0.0f;
+    if (kMode == kFinal && args.has_momentum) {
+      const float lr = args.lr_device != nullptr ? *args.lr_device : args.lr;
+      keep = 1.0f - lr * args.weight_decay;
+      step = lr * args.scale;
+    }
     int local = 0;
-    for (int tile = blockIdx.x; tile < args.total_tiles; tile += gridDim.x, ++local) {
+    for (int tile = slot0; tile < args.total_tiles; tile += slots, ++local) {
       const int acc = local & 1;
-      int mat, tr, tc;
-      locate(tile, mat, tr, tc);
+      int set, mat, tr, tc;
+      locate(tile, set, mat, tr, tc);
+      const int row = tr * kTile + int(rank) * kTM + quad * 32 + lane;
+      const int col_base = tc * kTile + half * (kTile / 2);
+      // what the epilogue reads is loaded a piece ahead, the first one while the MMAs run
+      uint4 in_h[kPiece / 8], in_l[kPiece / 8];
+      float w[kPiece];
+      auto prefetch = [&](int piece) {
+        const int col = col_base + piece * kPiece;
+        if constexpr (kMode == kPoly) {
+          const __half* hi = args.in + int64_t(mat) * 2 * args.plane + int64_t(row) * args.ld + col;
+#pragma unroll
+          for (int g = 0; g < kPiece / 8; ++g) {
+            in_h[g] = in_l[g] = make_uint4(0u, 0u, 0u, 0u);
+            if (row < args.m && col + g * 8 < int(args.ld)) {   // ld is a multiple of 8
+              in_h[g] = *reinterpret_cast<const uint4*>(hi + g * 8);
+              in_l[g] = *reinterpret_cast<const uint4*>(hi + args.plane + g * 8);
+            }
+          }
+        } else if constexpr (kMode == kFinal) {
+          if (args.has_momentum) load_weights<T>(args, outs, mat, row, col, w);
+        }
+      };
+      prefetch(0);
       int ok = 1;
       if (lane == 0) ok = wait_phase(tfull + acc, (local >> 1) & 1, abort) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       (void)mbar_try(tfull + acc, (local >> 1) & 1);  // completed: acquire for every lane
       tc_fence_after();
-      const int row = tr * kTM + quad * 32 + lane;
-      const __half* in_hi = args.in + int64_t(mat) * 2 * args.plane;
-      __half* out_hi = args.out + int64_t(mat) * 2 * args.plane;
-      for (int c = 0; c < 4; ++c) {
-        const int col0 = tc * kTN + half * 64 + c * 16;
-        uint32_t v[16];
-        tmem_ld16(lane_addr + uint32_t(acc * kTN + half * 64 + c * 16), v);
+      __half* out_hi = args.out[set] + int64_t(mat) * 2 * args.plane;
+      const float mult = args.mult[set];
+#pragma unroll 1
+      for (int c = 0; c < kPieces; ++c) {
+        const int col0 = col_base + c * kPiece;
+        float y[kPiece];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const int col = col0 + g * 8;
-          float y[8];
+          uint32_t v[16];
+          tmem_ld16(lane_addr + uint32_t(acc * kTile + half * (kTile / 2) + c * kPiece + g * 16), v);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(v[g * 8 + k]) * kInvScale;
-          const bool inside = row < args.m && col < int(args.ld);  // ld is a multiple of 8
-          if (kMode != kGram && inside) {
-            float x[8];
-            const int64_t at = int64_t(row) * args.ld + col;
-            join8(in_hi + at, in_hi + args.plane + at, x);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              y[k] = kMode == kPoly ? fmaf(kB, x[k], kC * y[k]) : fmaf(kA, x[k], y[k]);
+          for (int k = 0; k < 16; ++k) y[g * 16 + k] = __uint_as_float(v[k]) * mult;
+        }
+        if (c == kPieces - 1) {
+          // this warp has read its part of the accumulator: hand it back to the MMA issuer
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kPair == 1) mbar_arrive(tempty + acc);
+            else mbar_arrive_cluster(cluster_addr(tempty + acc, 0));
           }
-          if constexpr (kMode == kFinal) {
-            if (inside && col < args.n) {
+        }
+        if constexpr (kMode == kPoly) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) y[k] *= kInvScale;
-              final_store<T>(args, outs, mat, row, col, y, lr);
+          for (int g = 0; g < kPiece / 8; ++g) {
+            float x[8];
+            join8(in_h[g], in_l[g], x);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              float& o = y[g * 8 + k];
+              o = fmaf(kB, x[k], kC * o);
+              if (row == col0 + g * 8 + k) o += kA * kScale;
             }
-          } else {
+          }
+        } else if constexpr (kMode == kFinal) {
+          if (args.has_momentum) {
+#pragma unroll
+            for (int k = 0; k < kPiece; ++k) y[k] = fmaf(keep, w[k], -step * y[k]);
+          }
+        }
+        if (c + 1 < kPieces) prefetch(c + 1);
+        if constexpr (kMode == kFinal) {
+          store_result<T>(args, outs, mat, row, col0, y);
+        } else {
+#pragma unroll
+          for (int g = 0; g < kPiece / 8; ++g) {
+            const int col = col0 + g * 8;
             __half hi[8], lo[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) split(y[k], hi[k], lo[k]);
-            if (inside) {
+            for (int k = 0; k < 8; ++k) split(y[g * 8 + k], hi[k], lo[k]);
+            if (row < args.m && col < int(args.ld)) {
               const int64_t at = int64_t(row) * args.ld + col;
               *reinterpret_cast<uint4*>(out_hi + at) =
                   make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
@@ -590,7 +819,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
                   make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
                              pack2(lo[6], lo[7]));
             }
-            if (kSym && tr != tc && row < args.m) {
+            if (kMirror && tr != tc && row < args.m) {
               // the mirror image: for one column the warp's 32 rows are consecutive
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
@@ -604,18 +833,16 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tempty + acc);
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair == 2) cluster_sync();  // the pair is done with TMEM and remote barriers
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_free(tmem_base, kTmemCols);
+    tmem_free<kPair>(tmem_base, kTmemCols);
   }
 }
 
@@ -673,10 +900,17 @@ int sm_count(int device) {
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// Steps taken on the Gram matrix at once (the blocks of an iteration): wide matrices only.  Measured
+// for twelve matrices: see run().
+int block_steps(int64_t m, int64_t n, int left) {
+  if (2 * n < 3 * m) return 1;
+  return left == 4 ? 2 : (left < kMaxBlock ? left : kMaxBlock);
+}
+
 // Where each part of the workspace lies (bytes; every part a multiple of 256).
 struct Layout {
   int64_t m, n, ldn, ldm, plane_x, plane_a;
-  size_t x0, x1, a, b, partial, total;
+  size_t x0, x1, sym[6], partial, total;
   Layout(int64_t count, int64_t rows, int64_t cols) {
     m = rows < cols ? rows : cols;
     n = rows < cols ? cols : rows;
@@ -686,11 +920,15 @@ struct Layout {
     plane_a = m * ldm;
     const size_t bx = size_t(round_up(count * 2 * plane_x * 2, 256));
     const size_t ba = size_t(round_up(count * 2 * plane_a * 2, 256));
+    const int syms = block_steps(m, n, kMaxBlock) > 1 ? 6 : 2;
     x0 = 0;
     x1 = x0 + bx;
-    a = x1 + bx;
-    b = a + ba;
-    partial = b + ba;
+    size_t at = x1 + bx;
+    for (int i = 0; i < 6; ++i) {
+      sym[i] = at;
+      if (i < syms) at += ba;
+    }
+    partial = at;
     total = partial + size_t(round_up(count * kNormBlocks * int64_t(sizeof(double)), 256));
   }
 };
@@ -704,83 +942,218 @@ int check_args(int32_t count, int64_t rows, int64_t cols, int32_t dtype, int32_t
   return KAT_OK;
 }
 
-template <int kMode, typename T>
-int launch_gemm(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& args,
-                const PtrTable& outs, int sms, cudaStream_t stream) {
-  auto kernel = kat_muon_gemm_kernel<kMode, T>;
+template <typename... Params, typename... Args>
+bool launch_after(void (*kernel)(Params...), dim3 grid, int threads, uint32_t smem, int cluster,
+                  cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(uint32_t(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = uint32_t(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess;
+}
+
+struct Device {
+  int sms;
+  int pairs;   // CTA pairs that fit at once
+};
+
+template <int kMode, typename T, int kPair>
+int launch_pair(const CUtensorMap& p, const CUtensorMap& q0, const CUtensorMap& q1, GemmArgs args,
+                const PtrTable& outs, int sets, int count, const Device& dev, cudaStream_t stream) {
+  auto kernel = kat_muon_gemm_kernel<kMode, T, kPair>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kSmemBytes)) != cudaSuccess)
     return KAT_ERR_CUDA;
-  const int grid = args.total_tiles < sms ? args.total_tiles : sms;
-  kernel<<<grid, kThreads, kSmemBytes, stream>>>(p, q, args, outs);
-  return cudaGetLastError() == cudaSuccess ? KAT_OK : KAT_ERR_CUDA;
+  const int tm = (args.m + kTM * kPair - 1) / (kTM * kPair);
+  const int tn = (args.n + kTM * kPair - 1) / (kTM * kPair);
+  args.row_tiles = tm;
+  args.tiles = kMode == kSym || kMode == kPoly ? tm * (tm + 1) / 2 : tm * tn;
+  args.set_tiles = args.tiles * count;
+  args.total_tiles = args.set_tiles * sets;
+  const int slots = kPair == 2 ? dev.pairs : dev.sms;
+  const int grid = args.total_tiles < slots ? args.total_tiles : slots;
+  return launch_after(kernel, dim3(uint32_t(grid * kPair)), kThreads, kSmemBytes, kPair, stream, p,
+                      q0, q1, args, outs)
+             ? KAT_OK
+             : KAT_ERR_CUDA;
+}
+
+// One CTA to a tile or a pair to a tile four times as large, by the estimated time of the waves.
+template <int kMode, typename T>
+int launch_gemm(const CUtensorMap& p, const CUtensorMap& q0, const CUtensorMap& q1,
+                const GemmArgs& args, const PtrTable& outs, int sets, int count, const Device& dev,
+                cudaStream_t stream) {
+  auto tiles = [&](int64_t side) {
+    const int64_t tm = (args.m + side - 1) / side, tn = (args.n + side - 1) / side;
+    return (kMode == kSym || kMode == kPoly ? tm * (tm + 1) / 2 : tm * tn) * count * sets;
+  };
+  const int64_t waves1 = (tiles(kTM) + dev.sms - 1) / dev.sms;
+  const int64_t waves2 = dev.pairs > 0 ? (tiles(2 * kTM) + dev.pairs - 1) / dev.pairs : 0;
+  if (dev.pairs > 0 && waves2 * 3 <= waves1 * 2)
+    return launch_pair<kMode, T, 2>(p, q0, q1, args, outs, sets, count, dev, stream);
+  return launch_pair<kMode, T, 1>(p, q0, q1, args, outs, sets, count, dev, stream);
 }
 
 template <typename T>
 int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int64_t rows,
-        int64_t cols, int32_t steps, uint8_t* ws, int sms, cudaStream_t stream) {
+        int64_t cols, int32_t steps, uint8_t* ws, const Device& dev, bool vec,
+        cudaStream_t stream) {
   const Layout L(count, rows, cols);
   __half* x[2] = {reinterpret_cast<__half*>(ws + L.x0), reinterpret_cast<__half*>(ws + L.x1)};
-  __half* a = reinterpret_cast<__half*>(ws + L.a);
-  __half* b = reinterpret_cast<__half*>(ws + L.b);
-  double* partial = reinterpret_cast<double*>(ws + L.partial);
-  const int transposed = rows > cols;
-
-  int64_t want = (u.size + kNormThreads * 16 - 1) / (kNormThreads * 16);
-  const int norm_blocks = int(want < kNormBlocks ? want : kNormBlocks);
-  kat_muon_norm_kernel<T><<<dim3(norm_blocks, count), kNormThreads, 0, stream>>>(u, partial);
-  const int row_tiles = int((rows + kSplitTile - 1) / kSplitTile);
-  const int col_tiles = int((cols + kSplitTile - 1) / kSplitTile);
-  kat_muon_split_kernel<T><<<dim3(uint32_t(row_tiles) * col_tiles, count), 256, 0, stream>>>(
-      u, partial, norm_blocks, x[0], rows, cols, L.ldn, L.plane_x, transposed, col_tiles);
-  if (cudaGetLastError() != cudaSuccess) return KAT_ERR_CUDA;
-
-  CUtensorMap xk[2], xmn[2], ma, mb;
+  __half* sym[6];
+  CUtensorMap xk[2], xmn[2], ms[6];
   for (int i = 0; i < 2; ++i)
     if (!make_map(&xk[i], x[i], 2 * count, L.m, L.n, L.ldn, kTM) ||
         !make_map(&xmn[i], x[i], 2 * count, L.m, L.n, L.ldn, kTK))
       return KAT_ERR_CUDA;
-  if (!make_map(&ma, a, 2 * count, L.m, L.m, L.ldm, kTM) ||
-      !make_map(&mb, b, 2 * count, L.m, L.m, L.ldm, kTM))
-    return KAT_ERR_CUDA;
+  const int syms = L.sym[5] != L.sym[2] ? 6 : 2;
+  for (int i = 0; i < syms; ++i) {
+    sym[i] = reinterpret_cast<__half*>(ws + L.sym[i]);
+    if (!make_map(&ms[i], sym[i], 2 * count, L.m, L.m, L.ldm, kTM)) return KAT_ERR_CUDA;
+  }
+  double* partial = reinterpret_cast<double*>(ws + L.partial);
+  const int transposed = rows > cols;
 
-  const int tm = int((L.m + kTM - 1) / kTM), tn = int((L.n + kTN - 1) / kTN);
-  GemmArgs sym{};
-  sym.m = sym.n = int32_t(L.m);
-  sym.row_tiles = sym.col_tiles = tm;
-  sym.tiles = tm * (tm + 1) / 2;
-  sym.total_tiles = sym.tiles * count;
-  sym.ld = L.ldm;
-  sym.plane = L.plane_a;
+  const int64_t per = int64_t(kNormThreads) * (vec ? 16 : 4);
+  const int64_t want = (u.size + per - 1) / per;
+  const int norm_blocks = int(want < kNormBlocks ? want : kNormBlocks);
+  const dim3 norm_grid{uint32_t(norm_blocks), uint32_t(count)};
+  const int row_tiles = int((rows + kSplitTile - 1) / kSplitTile);
+  const int col_tiles = int((cols + kSplitTile - 1) / kSplitTile);
+  const dim3 split_grid{uint32_t(row_tiles) * uint32_t(col_tiles), uint32_t(count)};
+  bool ok;
+  if (vec) {
+    kat_muon_norm_kernel<T, 8><<<norm_grid, kNormThreads, 0, stream>>>(u, partial);
+    ok = launch_after(kat_muon_split_kernel<T, 8>, split_grid, kSplitThreads, 0, 1, stream, u,
+                      static_cast<const double*>(partial), norm_blocks, x[0], rows, cols, L.ldn,
+                      L.plane_x, transposed, col_tiles);
+  } else {
+    kat_muon_norm_kernel<T, 1><<<norm_grid, kNormThreads, 0, stream>>>(u, partial);
+    ok = launch_after(kat_muon_split_kernel<T, 1>, split_grid, kSplitThreads, 0, 1, stream, u,
+                      static_cast<const double*>(partial), norm_blocks, x[0], rows, cols, L.ldn,
+                      L.plane_x, transposed, col_tiles);
+  }
+  if (!ok || cudaGetLastError() != cudaSuccess) return KAT_ERR_CUDA;
+
+  const int k_m = int((L.m + kTK - 1) / kTK), k_n = int((L.n + kTK - 1) / kTK);
+  GemmArgs sq{};
+  sq.m = sq.n = int32_t(L.m);
+  sq.ld = L.ldm;
+  sq.plane = L.plane_a;
+  sq.k_blocks = k_m;
+  sq.mult[0] = 1.0f / kScale;
   fin.m = int32_t(L.m);
   fin.n = int32_t(L.n);
-  fin.row_tiles = tm;
-  fin.col_tiles = tn;
-  fin.tiles = tm * tn;
-  fin.total_tiles = fin.tiles * count;
-  fin.k_blocks = int((L.m + kTK - 1) / kTK);
+  fin.k_blocks = k_m;
   fin.ld = L.ldn;
   fin.plane = L.plane_x;
   fin.transposed = transposed;
   fin.out_ld = cols;
-  for (int s = 0; s < steps; ++s) {
-    const int cur = s & 1;
-    GemmArgs g = sym;
-    g.k_blocks = int((L.n + kTK - 1) / kTK);
-    g.in = g.out = a;
-    if (int rc = launch_gemm<kGram, float>(xk[cur], xk[cur], g, outs, sms, stream)) return rc;
-    g.k_blocks = fin.k_blocks;
-    g.in = a;
-    g.out = b;
-    if (int rc = launch_gemm<kPoly, float>(ma, ma, g, outs, sms, stream)) return rc;
-    fin.in = x[cur];
-    fin.out = x[cur ^ 1];
-    const int rc = s + 1 < steps
-                       ? launch_gemm<kApply, float>(mb, xmn[cur], fin, outs, sms, stream)
-                       : launch_gemm<kFinal, T>(mb, xmn[cur], fin, outs, sms, stream);
+
+  // m x m product out0 = p q0, and where q1 >= 0 out1 = p q1 in the same launch
+  auto square = [&](int p, int q0, int out0, float mult0, int q1 = -1, int out1 = 0,
+                    float mult1 = 0.0f) {
+    GemmArgs g = sq;
+    const int sets = q1 >= 0 ? 2 : 1;
+    g.mult[0] = mult0;
+    g.out[0] = sym[out0];
+    g.mult[1] = mult1;
+    g.out[1] = sym[out1];
+    return launch_gemm<kSym, float>(ms[p], ms[q0], ms[sets == 2 ? q1 : q0], g, outs, sets, count,
+                                    dev, stream);
+  };
+  const float to_plane = 1.0f / kScale;
+  int cur = 0;
+  for (int done = 0; done < steps;) {
+    const int block = block_steps(L.m, L.n, steps - done);
+    // gram
+    GemmArgs g = sq;
+    g.k_blocks = k_n;
+    g.out[0] = sym[0];
+    if (int rc = launch_gemm<kSym, float>(xk[cur], xk[cur], xk[cur], g, outs, 1, count, dev, stream))
+      return rc;
+    // sym[0] = A, [1] and [2] the P's in turn, [3] = P A, [4] and [5] the products of P's
+    int q = 1;         // where the product of the block's P's so far is
+    float q_scale = kScale;
+    for (int t = 0; t < block; ++t) {
+      const int p = 1 + (t & 1);
+      g = sq;
+      g.in = sym[0];
+      g.out[0] = sym[p];
+      if (int rc = launch_gemm<kPoly, float>(ms[0], ms[0], ms[0], g, outs, 1, count, dev, stream))
+        return rc;
+      const bool more = t + 1 < block;
+      const int next = 4 + (t & 1);
+      int rc = KAT_OK;
+      if (t > 0 && more) rc = square(p, 0, 3, to_plane, q, next, to_plane / 4.0f);
+      else if (t > 0) rc = square(p, q, next, to_plane / 4.0f);
+      else if (more) rc = square(p, 0, 3, to_plane);
+      if (rc) return rc;
+      if (t > 0) {
+        q = next;
+        q_scale /= 4.0f;
+      }
+      if (more)
+        if (int r2 = square(3, p, 0, to_plane)) return r2;
+    }
+    done += block;
+    fin.out[0] = x[cur ^ 1];
+    int rc;
+    if (done < steps) {
+      fin.mult[0] = 1.0f / q_scale;
+      rc = launch_gemm<kApply, float>(ms[q], xmn[cur], xmn[cur], fin, outs, 1, count, dev, stream);
+    } else {
+      fin.mult[0] = 1.0f / (q_scale * kScale);
+      rc = launch_gemm<kFinal, T>(ms[q], xmn[cur], xmn[cur], fin, outs, 1, count, dev, stream);
+    }
     if (rc) return rc;
+    cur ^= 1;
   }
   return KAT_OK;
+}
+
+// CTA pairs of these kernels that fit on `device` at once (cached), 0 if none.
+int pair_count(int device) {
+  static std::mutex mu;
+  static int cache[64] = {0};
+  std::lock_guard<std::mutex> lock(mu);
+  if (device < 0 || device >= 64) return 0;
+  if (cache[device] == 0) {
+    int best = -1;
+    auto kernel = kat_muon_gemm_kernel<kApply, float, 2>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             int(kSmemBytes)) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = kSmemBytes;
+      cfg.gridDim = dim3(128);
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) best = n;
+    }
+    cudaGetLastError();
+    cache[device] = best;
+  }
+  return cache[device] > 0 ? cache[device] : 0;
 }
 
 int dispatch(const Update& u, const PtrTable& outs, const GemmArgs& fin, int32_t count,
@@ -790,18 +1163,22 @@ int dispatch(const Update& u, const PtrTable& outs, const GemmArgs& fin, int32_t
   if (ws == nullptr || ws_bytes < L.total || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
     return KAT_ERR_WORKSPACE;
   // tiles of all matrices are counted in 32 bits
-  const int64_t tm = (L.m + kTM - 1) / kTM, tn = (L.n + kTN - 1) / kTN;
+  const int64_t tm = (L.m + kTM - 1) / kTM, tn = (L.n + kTM - 1) / kTM;
   if (tm * tn * count >= (int64_t(1) << 30)) return KAT_ERR_BAD_SHAPE;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KAT_ERR_CUDA;
-  const int sms = sm_count(dev);
-  if (sms <= 0) return KAT_ERR_CUDA;
+  const Device d{sm_count(dev), pair_count(dev)};
+  if (d.sms <= 0) return KAT_ERR_CUDA;
+  bool vec = cols % 8 == 0;   // the inputs' rows take 16-byte accesses
+  for (int i = 0; i < count; ++i)
+    vec = vec && ((reinterpret_cast<uintptr_t>(u.x.p[i]) | reinterpret_cast<uintptr_t>(u.m.p[i])) &
+                  15u) == 0;
   uint8_t* w = static_cast<uint8_t*>(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case KAT_DTYPE_F32: return run<float>(u, outs, fin, count, rows, cols, steps, w, sms, st);
-    case KAT_DTYPE_F16: return run<__half>(u, outs, fin, count, rows, cols, steps, w, sms, st);
-    default: return run<__nv_bfloat16>(u, outs, fin, count, rows, cols, steps, w, sms, st);
+    case KAT_DTYPE_F32: return run<float>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
+    case KAT_DTYPE_F16: return run<__half>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
+    default: return run<__nv_bfloat16>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
   }
 }
 
