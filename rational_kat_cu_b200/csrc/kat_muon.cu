@@ -8,8 +8,10 @@
 //   apply   X' = P X                    rows of P against X itself, read with its columns contiguous
 //                                       (an MN-major shared-memory operand): X is never transposed
 // gram, poly and all other m x m products are symmetric: only the tiles on and below the diagonal
-// are computed, and each is written twice, once transposed.  The last apply writes the output or
-// updates the weights.
+// are computed and stored.  Where a product needs a block above it, it reads the block below with
+// its columns contiguous, the same way as X: each k-block's instruction descriptor says which way
+// its operands lie.  (Writing each tile a second time, transposed, took as long as the MMAs.)  The
+// last apply writes the output or updates the weights.
 //
 // Wide matrices take up to three steps at once on the Gram matrix: the next step's is
 // A' = P A P (all of these commute), and X is multiplied once by the product of the P's:
@@ -53,7 +55,9 @@ constexpr uint32_t kPlaneBytes = kTM * kTK * 2;        // one operand plane of a
 constexpr uint32_t kStageBytes = 4 * kPlaneBytes;      // P hi, P lo, Q hi, Q lo
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
-constexpr uint32_t kSmemBytes = 1024 + kStages * kStageBytes + 256;
+constexpr int kPiece = 32;         // rows and columns an epilogue warp handles at once
+constexpr uint32_t kStagingBytes = 2 * kPiece * kPiece * 2;   // of a warp: a piece in two planes
+constexpr uint32_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStagingBytes + 256;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 constexpr long long kWaitCycles = 4000000000LL;
 
@@ -65,7 +69,7 @@ constexpr int kMaxBlock = 3;   // steps taken on the Gram matrix at once
 
 __device__ int g_muon_status;
 
-enum Mode { kSym = 0, kPoly = 1, kApply = 2, kFinal = 3 };
+enum Mode { kGram = 0, kSym = 1, kPoly = 2, kApply = 3, kFinal = 4 };
 
 struct PtrTable {
   const void* p[kMaxMats];
@@ -133,6 +137,26 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int32_t x,
+                                             int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_read() {   // earlier stores have read their source
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
@@ -260,11 +284,13 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
   return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(kBoxBytes >> 4) << 16) |
          (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
-// Instruction descriptor: fp32 accumulator (bits 4-5 = 1), fp16 operands (7-9, 10-12 = 0), B's
-// major-ness in bit 16, N >> 3 in 17-22, M >> 4 in 24-28; tiles are 128 or (a CTA pair) 256 square.
-__host__ __device__ constexpr uint32_t idesc_of(bool mn_major_q, int pair) {
-  return (1u << 4) | (mn_major_q ? (1u << 16) : 0u) | (uint32_t((kTM * pair) >> 3) << 17) |
-         (uint32_t((kTM * pair) >> 4) << 24);
+// Instruction descriptor: fp32 accumulator (bits 4-5 = 1), fp16 operands (7-9, 10-12 = 0), the
+// operands' major-ness in bits 15 and 16 (1: MN-major), N >> 3 in 17-22, M >> 4 in 24-28; tiles are
+// 128 or (a CTA pair) 256 square.
+template <int kPair>
+__device__ __forceinline__ uint32_t idesc_of(bool mn_p, bool mn_q) {
+  return (1u << 4) | (mn_p ? (1u << 15) : 0u) | (mn_q ? (1u << 16) : 0u) |
+         (uint32_t((kTM * kPair) >> 3) << 17) | (uint32_t((kTM * kPair) >> 4) << 24);
 }
 
 // ---------------------------------------------------------------------------
@@ -491,75 +517,20 @@ struct GemmArgs {
   int32_t total_tiles;     // of both sets
   int32_t k_blocks;
   float mult[2];           // accumulator -> plane (or, last, output) value, by set
-  const __half* in;        // poly: planes of A, leading dimension and plane as the output's
-  __half* out[2];          // planes written, by set
+  const __half* in;        // poly: planes of A
   int64_t ld, plane;
   // final step
   int32_t transposed;
   int64_t out_ld;          // columns of the caller's matrices
   int32_t has_momentum;    // update weights instead of writing the result
-  int32_t vec;             // the caller's rows take 16-byte accesses
   float lr, weight_decay, scale;
   const float* lr_device;
 };
 
-constexpr int kPiece = 32;   // columns a warp takes from the accumulator at once
-
-// A thread's kPiece output values of one row (col .. col + 31): the weights they are added to,
-// loaded before the accumulator is waited for ...
-template <typename T>
-__device__ __forceinline__ void load_weights(const GemmArgs& args, const PtrTable& outs, int mat,
-                                             int row, int col, float (&w)[kPiece]) {
-  const T* base = static_cast<const T*>(outs.p[mat]);
-  if (row >= args.m) return;
-  if (args.transposed) {
-#pragma unroll
-    for (int k = 0; k < kPiece; ++k)
-      if (col + k < args.n) w[k] = load1(base + int64_t(col + k) * args.out_ld + row);
-  } else {
-    const T* p = base + int64_t(row) * args.out_ld + col;
-    if (args.vec) {
-#pragma unroll
-      for (int g = 0; g < kPiece / 8; ++g)
-        if (col + g * 8 < args.n)
-          load_values<T, 8>(p + g * 8, *reinterpret_cast<float(*)[8]>(&w[g * 8]));
-    } else {
-#pragma unroll
-      for (int k = 0; k < kPiece; ++k)
-        if (col + k < args.n) w[k] = load1(p + k);
-    }
-  }
-}
-// ... and the results written.
-template <typename T>
-__device__ __forceinline__ void store_result(const GemmArgs& args, const PtrTable& outs, int mat,
-                                             int row, int col, const float (&o)[kPiece]) {
-  T* base = static_cast<T*>(const_cast<void*>(outs.p[mat]));
-  if (row >= args.m) return;
-  if (args.transposed) {
-#pragma unroll
-    for (int k = 0; k < kPiece; ++k)
-      if (col + k < args.n) base[int64_t(col + k) * args.out_ld + row] = from_float<T>(o[k]);
-  } else {
-    T* p = base + int64_t(row) * args.out_ld + col;
-    if (args.vec) {
-#pragma unroll
-      for (int g = 0; g < kPiece / 8; ++g) {
-        if (col + g * 8 < args.n) {
-          union { uint4 q[sizeof(T) / 2]; T e[8]; } v;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v.e[k] = from_float<T>(o[g * 8 + k]);
-#pragma unroll
-          for (int q = 0; q < int(sizeof(T) / 2); ++q)
-            reinterpret_cast<uint4*>(p + g * 8)[q] = v.q[q];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < kPiece; ++k)
-        if (col + k < args.n) p[k] = from_float<T>(o[k]);
-    }
-  }
+// Staging of a warp.  Planes: 32 rows of 64 bytes, 16-byte granules swizzled as TMA's 64-byte mode
+// has it (granule index XOR address bits 7-8), so that neither rows nor granules collide.
+__device__ __forceinline__ uint32_t plane_offset(int row, int granule) {
+  return uint32_t(row) * 64u + uint32_t((granule ^ ((row >> 1) & 3)) << 4);
 }
 
 template <int kMode, typename T, int kPair>
@@ -567,15 +538,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
                      const __grid_constant__ CUtensorMap tm_q0,
                      const __grid_constant__ CUtensorMap tm_q1,
+                     const __grid_constant__ CUtensorMap tm_out0,
+                     const __grid_constant__ CUtensorMap tm_out1,
                      const __grid_constant__ GemmArgs args,
                      const __grid_constant__ PtrTable outs) {
-  constexpr bool kMirror = kMode == kSym || kMode == kPoly;
+  constexpr bool kLower = kMode == kGram || kMode == kSym || kMode == kPoly;  // symmetric output
+  constexpr bool kSymP = kMode != kGram, kSymQ = kMode == kSym || kMode == kPoly;
+  constexpr bool kColsQ = kMode == kApply || kMode == kFinal;   // Q is X, by its columns
   constexpr int kTile = kTM * kPair;                  // output tile, square
   constexpr uint32_t kTmemCols = 2 * kTile;           // two accumulators
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  uint8_t* staging = smem + kStages * kStageBytes;   // [epilogue warp]
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingBytes);
   uint64_t* empty = full + kStages;   // in each CTA
   uint64_t* tfull = empty + kStages;  // in each CTA
   uint64_t* tempty = tfull + 2;       // rank 0's counts the epilogue warps of both CTAs
@@ -603,6 +579,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_map(&tm_p);
     prefetch_map(&tm_q0);
+    if (kMode != kFinal) prefetch_map(&tm_out0);
   }
   if (warp == 1) tmem_alloc<kPair>(tmem_slot, kTmemCols);
   tc_fence_before();
@@ -618,7 +595,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     if (set) tile -= args.set_tiles;
     mat = tile / args.tiles;
     const int t = tile - mat * args.tiles;
-    if (kMirror) {
+    if (kLower) {
       tr = int((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);
       while ((tr + 1) * (tr + 2) / 2 <= t) ++tr;
       while (tr * (tr + 1) / 2 > t) --tr;
@@ -650,15 +627,17 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
             if constexpr (kPair == 1) tma_load_3d(dst, map, full + stage, x, y, z);
             else tma_load_3d_pair(dst, map, bar, x, y, z);
           };
+          const bool mn_p = kSymP && kb * kTK / kTile > tr;
+          const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            load(s + h * kPlaneBytes, &tm_p, kb * kTK, p0, 2 * mat + h);
-            uint8_t* q = s + (2 + h) * kPlaneBytes;
-            if (kMirror) {
-              load(q, tm_q, kb * kTK, q0, 2 * mat + h);
-            } else {
-              load(q, tm_q, q0, kb * kTK, 2 * mat + h);
-              load(q + kBoxBytes, tm_q, q0 + 64, kb * kTK, 2 * mat + h);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {   // boxes of 64 x 64: 64 rows, or 64 columns
+              const int p = p0 + b * 64, q = q0 + b * 64, k = kb * kTK;
+              load(s + h * kPlaneBytes + b * kBoxBytes, &tm_p, mn_p ? p : k, mn_p ? k : p,
+                   2 * mat + h);
+              load(s + (2 + h) * kPlaneBytes + b * kBoxBytes, tm_q, mn_q ? q : k, mn_q ? k : q,
+                   2 * mat + h);
             }
           }
           if (++stage == kStages) { stage = 0; phase ^= 1u; wrapped = true; }
@@ -682,6 +661,8 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       };
       for (int tile = slot0; tile < args.total_tiles && ok; tile += slots, ++local) {
         const int acc = local & 1;
+        int set, mat, tr, tc;
+        locate(tile, set, mat, tr, tc);
         if (!wait_phase(tempty + acc, ((local >> 1) & 1) ^ 1u, abort)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + uint32_t(acc * kTile);
@@ -689,18 +670,23 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
           if (!wait_phase(full + stage, phase, abort)) { ok = false; break; }
           tc_fence_after();
           const uint32_t s = smem_u32(smem + stage * kStageBytes);
-          const uint64_t p_hi = desc_k(s), p_lo = desc_k(s + kPlaneBytes);
-          const uint64_t q_hi = kMirror ? desc_k(s + 2 * kPlaneBytes) : desc_mn(s + 2 * kPlaneBytes);
-          const uint64_t q_lo = kMirror ? desc_k(s + 3 * kPlaneBytes) : desc_mn(s + 3 * kPlaneBytes);
+          const bool mn_p = kSymP && kb * kTK / kTile > tr;
+          const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
+          auto desc = [&](bool mn, int plane) {
+            return mn ? desc_mn(s + plane * kPlaneBytes) : desc_k(s + plane * kPlaneBytes);
+          };
+          const uint64_t p_hi = desc(mn_p, 0), p_lo = desc(mn_p, 1);
+          const uint64_t q_hi = desc(mn_q, 2), q_lo = desc(mn_q, 3);
           // a K = 16 slice further: 32 bytes inside the swizzled rows (K-major), two 8-k groups
           // (MN-major)
-          constexpr uint64_t kStepP = 32 >> 4, kStepQ = kMirror ? (32 >> 4) : (2048 >> 4);
-          constexpr uint32_t idesc = idesc_of(!kMirror, kPair);
+          const uint64_t step_p = mn_p ? (2048 >> 4) : (32 >> 4);
+          const uint64_t step_q = mn_q ? (2048 >> 4) : (32 >> 4);
+          const uint32_t idesc = idesc_of<kPair>(mn_p, mn_q);
 #pragma unroll
           for (int k = 0; k < kTK / kUmmaK; ++k) {
-            umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, (kb | k) != 0 ? 1u : 0u);
-            umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u);
-            umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u);
+            umma_f16<kPair>(d, p_hi + k * step_p, q_hi + k * step_q, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_f16<kPair>(d, p_hi + k * step_p, q_lo + k * step_q, idesc, 1u);
+            umma_f16<kPair>(d, p_lo + k * step_p, q_hi + k * step_q, idesc, 1u);
           }
           issued = true;
           commit_all(empty + stage);
@@ -721,6 +707,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     const int half = ew >> 2;
     const uint32_t lane_addr = tmem_base + (uint32_t(quad * 32) << 16);
     constexpr int kPieces = kTile / 2 / kPiece;   // of this warp's half of the columns
+    uint8_t* stage = staging + ew * kStagingBytes;
     float keep = 0.0f, step = 0.0f;
     if (kMode == kFinal && args.has_momentum) {
       const float lr = args.lr_device != nullptr ? *args.lr_device : args.lr;
@@ -734,23 +721,39 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       locate(tile, set, mat, tr, tc);
       const int row = tr * kTile + int(rank) * kTM + quad * 32 + lane;
       const int col_base = tc * kTile + half * (kTile / 2);
-      // what the epilogue reads is loaded a piece ahead, the first one while the MMAs run
-      uint4 in_h[kPiece / 8], in_l[kPiece / 8];
+      const int row0 = row - lane;
+      // What the epilogue reads is loaded a piece ahead, the first one while the MMAs run, along the
+      // rows in memory: of a plane 4 lanes take a row's 64 bytes; of the weights a lane takes a
+      // column (of the transposed ones a row).
+      uint4 in_v[2][4];
       float w[kPiece];
+      // final step: this lane's place in the first line of a piece in the caller's matrix (lines are
+      // the piece's rows, or its columns where transposed), and how many lines it has there
+      auto first_line = [&](int col0, int& lines) {
+        const int a = args.transposed ? col0 : row0, b = args.transposed ? row : col0 + lane;
+        lines = args.transposed ? (b < args.m ? args.n - a : 0) : (b < args.n ? args.m - a : 0);
+        return int64_t(a) * args.out_ld + b;
+      };
       auto prefetch = [&](int piece) {
-        const int col = col_base + piece * kPiece;
+        const int col0 = col_base + piece * kPiece;
         if constexpr (kMode == kPoly) {
-          const __half* hi = args.in + int64_t(mat) * 2 * args.plane + int64_t(row) * args.ld + col;
+          const int c = col0 + (lane & 3) * 8;
 #pragma unroll
-          for (int g = 0; g < kPiece / 8; ++g) {
-            in_h[g] = in_l[g] = make_uint4(0u, 0u, 0u, 0u);
-            if (row < args.m && col + g * 8 < int(args.ld)) {   // ld is a multiple of 8
-              in_h[g] = *reinterpret_cast<const uint4*>(hi + g * 8);
-              in_l[g] = *reinterpret_cast<const uint4*>(hi + args.plane + g * 8);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const int r = row0 + i * 8 + (lane >> 2);
+            const bool inside = r < args.m && c < int(args.ld);   // ld is a multiple of 8
+            const __half* at = args.in + int64_t(mat) * 2 * args.plane + int64_t(r) * args.ld + c;
+            in_v[0][i] = inside ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
+            in_v[1][i] = inside ? *reinterpret_cast<const uint4*>(at + args.plane)
+                                : make_uint4(0u, 0u, 0u, 0u);
           }
         } else if constexpr (kMode == kFinal) {
-          if (args.has_momentum) load_weights<T>(args, outs, mat, row, col, w);
+          if (args.has_momentum) {
+            int lines;
+            const T* p = static_cast<const T*>(outs.p[mat]) + first_line(col0, lines);
+#pragma unroll
+            for (int k = 0; k < kPiece; ++k, p += args.out_ld) w[k] = k < lines ? load1(p) : 0.0f;
+          }
         }
       };
       prefetch(0);
@@ -760,7 +763,6 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       if (!ok) break;
       (void)mbar_try(tfull + acc, (local >> 1) & 1);  // completed: acquire for every lane
       tc_fence_after();
-      __half* out_hi = args.out[set] + int64_t(mat) * 2 * args.plane;
       const float mult = args.mult[set];
 #pragma unroll 1
       for (int c = 0; c < kPieces; ++c) {
@@ -782,58 +784,83 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
             else mbar_arrive_cluster(cluster_addr(tempty + acc, 0));
           }
         }
-        if constexpr (kMode == kPoly) {
+        if constexpr (kMode == kFinal) {
+          float o[kPiece];   // element k of this lane's column (transposed: row)
+          if (args.transposed) {
 #pragma unroll
-          for (int g = 0; g < kPiece / 8; ++g) {
-            float x[8];
-            join8(in_h[g], in_l[g], x);
+            for (int k = 0; k < kPiece; ++k) o[k] = y[k];
+          } else {
+            // through the staging, each word at column XOR row: no two lanes in one bank either way
+            float* f = reinterpret_cast<float*>(stage);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              float& o = y[g * 8 + k];
-              o = fmaf(kB, x[k], kC * o);
-              if (row == col0 + g * 8 + k) o += kA * kScale;
-            }
+            for (int k = 0; k < kPiece; ++k) f[lane * kPiece + (k ^ lane)] = y[k];
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < kPiece; ++k) o[k] = f[k * kPiece + (lane ^ k)];
+            __syncwarp();
           }
-        } else if constexpr (kMode == kFinal) {
           if (args.has_momentum) {
 #pragma unroll
-            for (int k = 0; k < kPiece; ++k) y[k] = fmaf(keep, w[k], -step * y[k]);
+            for (int k = 0; k < kPiece; ++k) o[k] = fmaf(keep, w[k], -step * o[k]);
           }
-        }
-        if (c + 1 < kPieces) prefetch(c + 1);
-        if constexpr (kMode == kFinal) {
-          store_result<T>(args, outs, mat, row, col0, y);
+          if (c + 1 < kPieces) prefetch(c + 1);
+          int lines;
+          T* p = static_cast<T*>(const_cast<void*>(outs.p[mat])) + first_line(col0, lines);
+#pragma unroll
+          for (int k = 0; k < kPiece; ++k, p += args.out_ld)
+            if (k < lines) *p = from_float<T>(o[k]);
         } else {
+          // the staging's previous store has read it
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+          if constexpr (kMode == kPoly) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(stage + h * (kStagingBytes / 2) +
+                                          plane_offset(i * 8 + (lane >> 2), lane & 3)) = in_v[h][i];
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < kPiece / 8; ++g) {
+              float x[8];
+              join8(*reinterpret_cast<const uint4*>(stage + plane_offset(lane, g)),
+                    *reinterpret_cast<const uint4*>(stage + kStagingBytes / 2 +
+                                                    plane_offset(lane, g)), x);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                float& o = y[g * 8 + k];
+                o = fmaf(kB, x[k], kC * o);
+                if (row == col0 + g * 8 + k) o += kA * kScale;
+              }
+            }
+            __syncwarp();
+            if (c + 1 < kPieces) prefetch(c + 1);
+          }
 #pragma unroll
           for (int g = 0; g < kPiece / 8; ++g) {
-            const int col = col0 + g * 8;
             __half hi[8], lo[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) split(y[g * 8 + k], hi[k], lo[k]);
-            if (row < args.m && col < int(args.ld)) {
-              const int64_t at = int64_t(row) * args.ld + col;
-              *reinterpret_cast<uint4*>(out_hi + at) =
-                  make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
-                             pack2(hi[6], hi[7]));
-              *reinterpret_cast<uint4*>(out_hi + args.plane + at) =
-                  make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
-                             pack2(lo[6], lo[7]));
-            }
-            if (kMirror && tr != tc && row < args.m) {
-              // the mirror image: for one column the warp's 32 rows are consecutive
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                if (col + k < args.n) {
-                  const int64_t at = int64_t(col + k) * args.ld + row;
-                  out_hi[at] = hi[k];
-                  out_hi[args.plane + at] = lo[k];
-                }
-              }
-            }
+            *reinterpret_cast<uint4*>(stage + plane_offset(lane, g)) =
+                make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
+                           pack2(hi[6], hi[7]));
+            *reinterpret_cast<uint4*>(stage + kStagingBytes / 2 + plane_offset(lane, g)) =
+                make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
+                           pack2(lo[6], lo[7]));
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0 && row0 < args.m && col0 < args.n) {   // TMA leaves out what lies beyond
+            const CUtensorMap* out = set ? &tm_out1 : &tm_out0;
+            tma_store_3d(out, stage, col0, row0, 2 * mat);
+            tma_store_3d(out, stage + kStagingBytes / 2, col0, row0, 2 * mat + 1);
+            bulk_commit();
           }
         }
       }
     }
+    if (lane == 0) bulk_wait_all();
   }
 
   tc_fence_before();
@@ -870,17 +897,20 @@ EncodeTiledFn encoder() {
 }
 
 // Planes [2 x count][rows][ld] of which `cols` columns count: what lies beyond rows or cols is
-// read as zero, so no tile edge needs padding in memory.
+// read as zero and not written, so no tile edge needs padding in memory.  `store`: boxes of an
+// epilogue warp's 32 x 32 piece instead of an operand's 64 x 64.
 bool make_map(CUtensorMap* map, const __half* base, int64_t planes, int64_t rows, int64_t cols,
-              int64_t ld, uint32_t box_rows) {
+              int64_t ld, bool store) {
   EncodeTiledFn fn = encoder();
   if (fn == nullptr) return false;
   const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(planes)};
   const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(ld) * cuuint64_t(rows) * 2};
-  const cuuint32_t box[3] = {64, box_rows, 1};
+  const cuuint32_t box[3] = {store ? cuuint32_t(kPiece) : 64u,
+                             store ? cuuint32_t(kPiece) : cuuint32_t(kTK), 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box,
-            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -970,9 +1000,13 @@ struct Device {
   int pairs;   // CTA pairs that fit at once
 };
 
+// Operands and outputs of a product: P, and Q and out of each set.
+struct Maps {
+  CUtensorMap p, q[2], out[2];
+};
+
 template <int kMode, typename T, int kPair>
-int launch_pair(const CUtensorMap& p, const CUtensorMap& q0, const CUtensorMap& q1, GemmArgs args,
-                const PtrTable& outs, int sets, int count, const Device& dev, cudaStream_t stream) {
+int launch_pair(const Maps& m, GemmArgs args, const PtrTable& outs, int sets, int count, const Device& dev, cudaStream_t stream) {
   auto kernel = kat_muon_gemm_kernel<kMode, T, kPair>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kSmemBytes)) != cudaSuccess)
@@ -980,31 +1014,23 @@ int launch_pair(const CUtensorMap& p, const CUtensorMap& q0, const CUtensorMap& 
   const int tm = (args.m + kTM * kPair - 1) / (kTM * kPair);
   const int tn = (args.n + kTM * kPair - 1) / (kTM * kPair);
   args.row_tiles = tm;
-  args.tiles = kMode == kSym || kMode == kPoly ? tm * (tm + 1) / 2 : tm * tn;
+  args.tiles = kMode != kApply && kMode != kFinal ? tm * (tm + 1) / 2 : tm * tn;
   args.set_tiles = args.tiles * count;
   args.total_tiles = args.set_tiles * sets;
   const int slots = kPair == 2 ? dev.pairs : dev.sms;
   const int grid = args.total_tiles < slots ? args.total_tiles : slots;
-  return launch_after(kernel, dim3(uint32_t(grid * kPair)), kThreads, kSmemBytes, kPair, stream, p,
-                      q0, q1, args, outs)
+  return launch_after(kernel, dim3(uint32_t(grid * kPair)), kThreads, kSmemBytes, kPair, stream,
+                      m.p, m.q[0], m.q[1], m.out[0], m.out[1], args, outs)
              ? KAT_OK
              : KAT_ERR_CUDA;
 }
 
-// One CTA to a tile or a pair to a tile four times as large, by the estimated time of the waves.
+// CTA pairs on 256 x 256 tiles, or single CTAs on 128 x 128 tiles?
 template <int kMode, typename T>
-int launch_gemm(const CUtensorMap& p, const CUtensorMap& q0, const CUtensorMap& q1,
-                const GemmArgs& args, const PtrTable& outs, int sets, int count, const Device& dev,
-                cudaStream_t stream) {
-  auto tiles = [&](int64_t side) {
-    const int64_t tm = (args.m + side - 1) / side, tn = (args.n + side - 1) / side;
-    return (kMode == kSym || kMode == kPoly ? tm * (tm + 1) / 2 : tm * tn) * count * sets;
-  };
-  const int64_t waves1 = (tiles(kTM) + dev.sms - 1) / dev.sms;
-  const int64_t waves2 = dev.pairs > 0 ? (tiles(2 * kTM) + dev.pairs - 1) / dev.pairs : 0;
-  if (dev.pairs > 0 && waves2 * 3 <= waves1 * 2)
-    return launch_pair<kMode, T, 2>(p, q0, q1, args, outs, sets, count, dev, stream);
-  return launch_pair<kMode, T, 1>(p, q0, q1, args, outs, sets, count, dev, stream);
+int launch_gemm(bool pair, const Maps& m, const GemmArgs& args, const PtrTable& outs, int sets,
+                int count, const Device& dev, cudaStream_t stream) {
+  return pair ? launch_pair<kMode, T, 2>(m, args, outs, sets, count, dev, stream)
+              : launch_pair<kMode, T, 1>(m, args, outs, sets, count, dev, stream);
 }
 
 template <typename T>
@@ -1014,15 +1040,17 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   const Layout L(count, rows, cols);
   __half* x[2] = {reinterpret_cast<__half*>(ws + L.x0), reinterpret_cast<__half*>(ws + L.x1)};
   __half* sym[6];
-  CUtensorMap xk[2], xmn[2], ms[6];
+  CUtensorMap mx[2], ms[6], sx[2], ss[6];   // loads and stores of X and of the m x m matrices
   for (int i = 0; i < 2; ++i)
-    if (!make_map(&xk[i], x[i], 2 * count, L.m, L.n, L.ldn, kTM) ||
-        !make_map(&xmn[i], x[i], 2 * count, L.m, L.n, L.ldn, kTK))
+    if (!make_map(&mx[i], x[i], 2 * count, L.m, L.n, L.ldn, false) ||
+        !make_map(&sx[i], x[i], 2 * count, L.m, L.n, L.ldn, true))
       return KAT_ERR_CUDA;
   const int syms = L.sym[5] != L.sym[2] ? 6 : 2;
   for (int i = 0; i < syms; ++i) {
     sym[i] = reinterpret_cast<__half*>(ws + L.sym[i]);
-    if (!make_map(&ms[i], sym[i], 2 * count, L.m, L.m, L.ldm, kTM)) return KAT_ERR_CUDA;
+    if (!make_map(&ms[i], sym[i], 2 * count, L.m, L.m, L.ldm, false) ||
+        !make_map(&ss[i], sym[i], 2 * count, L.m, L.m, L.ldm, true))
+      return KAT_ERR_CUDA;
   }
   double* partial = reinterpret_cast<double*>(ws + L.partial);
   const int transposed = rows > cols;
@@ -1063,17 +1091,23 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   fin.transposed = transposed;
   fin.out_ld = cols;
 
+  // One choice for all products of the call (the symmetric ones store whole tiles of their own size
+  // on the diagonal), by the waves of the symmetric ones.
+  auto waves = [&](int64_t side, int64_t slots) {
+    const int64_t t = (L.m + side - 1) / side;
+    return slots > 0 ? (t * (t + 1) / 2 * count + slots - 1) / slots : 0;
+  };
+  const bool pair = dev.pairs > 0 && 3 * waves(2 * kTM, dev.pairs) <= 2 * waves(kTM, dev.sms);
+
   // m x m product out0 = p q0, and where q1 >= 0 out1 = p q1 in the same launch
   auto square = [&](int p, int q0, int out0, float mult0, int q1 = -1, int out1 = 0,
                     float mult1 = 0.0f) {
     GemmArgs g = sq;
     const int sets = q1 >= 0 ? 2 : 1;
     g.mult[0] = mult0;
-    g.out[0] = sym[out0];
     g.mult[1] = mult1;
-    g.out[1] = sym[out1];
-    return launch_gemm<kSym, float>(ms[p], ms[q0], ms[sets == 2 ? q1 : q0], g, outs, sets, count,
-                                    dev, stream);
+    const Maps m{ms[p], {ms[q0], ms[sets == 2 ? q1 : q0]}, {ss[out0], ss[out1]}};
+    return launch_gemm<kSym, float>(pair, m, g, outs, sets, count, dev, stream);
   };
   const float to_plane = 1.0f / kScale;
   int cur = 0;
@@ -1082,9 +1116,8 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
     // gram
     GemmArgs g = sq;
     g.k_blocks = k_n;
-    g.out[0] = sym[0];
-    if (int rc = launch_gemm<kSym, float>(xk[cur], xk[cur], xk[cur], g, outs, 1, count, dev, stream))
-      return rc;
+    const Maps gram{mx[cur], {mx[cur], mx[cur]}, {ss[0], ss[0]}};
+    if (int rc = launch_gemm<kGram, float>(pair, gram, g, outs, 1, count, dev, stream)) return rc;
     // sym[0] = A, [1] and [2] the P's in turn, [3] = P A, [4] and [5] the products of P's
     int q = 1;         // where the product of the block's P's so far is
     float q_scale = kScale;
@@ -1092,9 +1125,8 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
       const int p = 1 + (t & 1);
       g = sq;
       g.in = sym[0];
-      g.out[0] = sym[p];
-      if (int rc = launch_gemm<kPoly, float>(ms[0], ms[0], ms[0], g, outs, 1, count, dev, stream))
-        return rc;
+      const Maps poly{ms[0], {ms[0], ms[0]}, {ss[p], ss[p]}};
+      if (int rc = launch_gemm<kPoly, float>(pair, poly, g, outs, 1, count, dev, stream)) return rc;
       const bool more = t + 1 < block;
       const int next = 4 + (t & 1);
       int rc = KAT_OK;
@@ -1110,14 +1142,14 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
         if (int r2 = square(3, p, 0, to_plane)) return r2;
     }
     done += block;
-    fin.out[0] = x[cur ^ 1];
+    const Maps apply{ms[q], {mx[cur], mx[cur]}, {sx[cur ^ 1], sx[cur ^ 1]}};
     int rc;
     if (done < steps) {
       fin.mult[0] = 1.0f / q_scale;
-      rc = launch_gemm<kApply, float>(ms[q], xmn[cur], xmn[cur], fin, outs, 1, count, dev, stream);
+      rc = launch_gemm<kApply, float>(pair, apply, fin, outs, 1, count, dev, stream);
     } else {
       fin.mult[0] = 1.0f / (q_scale * kScale);
-      rc = launch_gemm<kFinal, T>(ms[q], xmn[cur], xmn[cur], fin, outs, 1, count, dev, stream);
+      rc = launch_gemm<kFinal, T>(pair, apply, fin, outs, 1, count, dev, stream);
     }
     if (rc) return rc;
     cur ^= 1;
@@ -1201,12 +1233,10 @@ int kat_orthogonalize(const void* const* x, void* const* out, int32_t count, int
   PtrTable outs{};
   GemmArgs fin{};
   u.size = rows * cols;
-  fin.vec = cols % 8 == 0;
   for (int i = 0; i < count; ++i) {
     if (x[i] == nullptr || out[i] == nullptr) return KAT_ERR_NULL_POINTER;
     u.x.p[i] = x[i];
     outs.p[i] = out[i];
-    if ((reinterpret_cast<uintptr_t>(out[i]) & 15u) != 0) fin.vec = 0;
   }
   return dispatch(u, outs, fin, count, rows, cols, dtype, steps, workspace, workspace_bytes,
                   stream);
@@ -1232,14 +1262,12 @@ int kat_muon_step(void* const* weights, const void* const* grads, float* const* 
   fin.lr_device = lr_device;
   fin.weight_decay = weight_decay;
   fin.scale = scale;
-  fin.vec = cols % 8 == 0;
   for (int i = 0; i < count; ++i) {
     if (weights[i] == nullptr || grads[i] == nullptr || momenta[i] == nullptr)
       return KAT_ERR_NULL_POINTER;
     u.x.p[i] = grads[i];
     u.m.p[i] = momenta[i];
     outs.p[i] = weights[i];
-    if ((reinterpret_cast<uintptr_t>(weights[i]) & 15u) != 0) fin.vec = 0;
   }
   return dispatch(u, outs, fin, count, rows, cols, dtype, steps, workspace, workspace_bytes,
                   stream);
