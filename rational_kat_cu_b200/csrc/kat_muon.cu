@@ -726,7 +726,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       // rows in memory: of a plane 4 lanes take a row's 64 bytes; of the weights a lane takes a
       // column (of the transposed ones a row).
       uint4 in_v[2][4];
-      float w[kPiece];
+      T w[kPiece];   // as stored: a conversion here would wait for each load before the next
       // final step: this lane's place in the first line of a piece in the caller's matrix (lines are
       // the piece's rows, or its columns where transposed), and how many lines it has there
       auto first_line = [&](int col0, int& lines) {
@@ -752,7 +752,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
             int lines;
             const T* p = static_cast<const T*>(outs.p[mat]) + first_line(col0, lines);
 #pragma unroll
-            for (int k = 0; k < kPiece; ++k, p += args.out_ld) w[k] = k < lines ? load1(p) : 0.0f;
+            for (int k = 0; k < kPiece; ++k, p += args.out_ld) if (k < lines) w[k] = *p;
           }
         }
       };
@@ -801,7 +801,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
           }
           if (args.has_momentum) {
 #pragma unroll
-            for (int k = 0; k < kPiece; ++k) o[k] = fmaf(keep, w[k], -step * o[k]);
+            for (int k = 0; k < kPiece; ++k) o[k] = fmaf(keep, load1(&w[k]), -step * o[k]);
           }
           if (c + 1 < kPieces) prefetch(c + 1);
           int lines;
