@@ -20,6 +20,11 @@
 // 3 m^2 n + 17 m^3 but loses digits where the singular values spread (relative error 2.7e-4 against
 // 1.4e-5 of fp32 products for singular values 1 / k; blocks of 3 and 2: 1.3e-5).
 //
+// Up to 128 rows one CTA takes a block's whole chain of m x m products, from A to the product of the
+// P's, in its shared memory: a product of that size is over in 2 us, half the time of a launch.
+// (Clusters that share a tile's K blocks and hand each other partial sums did not pay: the sums'
+// way through distributed shared memory took 7000 cycles, as long as the MMAs it saved.)
+//
 // Each product of two split matrices takes three MMAs (hi hi, hi lo, lo hi) on four operand planes.
 // With one CTA to a 128 x 128 tile the planes' way from L2 is what bounds it (64 KB a k-block for
 // 768 cycles of MMA); a CTA pair (cta_group::2) on a 256 x 256 tile loads the same bytes for twice
@@ -50,14 +55,14 @@ constexpr int kMaxSteps = 32;
 constexpr int kTM = 128;   // operand rows of a CTA: its tile rows, and its share of the columns
 constexpr int kTK = 64;    // k-block: 64 fp16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
-constexpr int kStages = 3;
 constexpr uint32_t kPlaneBytes = kTM * kTK * 2;        // one operand plane of a stage
-constexpr uint32_t kStageBytes = 4 * kPlaneBytes;      // P hi, P lo, Q hi, Q lo
+constexpr uint32_t kRingBytes = 12 * kPlaneBytes;      // stages: 3 of P and Q in two planes, 6 in one
+constexpr int kMaxStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kPiece = 32;         // rows and columns an epilogue warp handles at once
 constexpr uint32_t kStagingBytes = 2 * kPiece * kPiece * 2;   // of a warp: a piece in two planes
-constexpr uint32_t kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStagingBytes + 256;
+constexpr uint32_t kSmemBytes = 1024 + kRingBytes + kEpiWarps * kStagingBytes + 256;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 constexpr long long kWaitCycles = 4000000000LL;
 
@@ -288,9 +293,31 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
 // operands' major-ness in bits 15 and 16 (1: MN-major), N >> 3 in 17-22, M >> 4 in 24-28; tiles are
 // 128 or (a CTA pair) 256 square.
 template <int kPair>
-__device__ __forceinline__ uint32_t idesc_of(bool mn_p, bool mn_q) {
+__host__ __device__ constexpr uint32_t idesc_of(bool mn_p, bool mn_q) {
   return (1u << 4) | (mn_p ? (1u << 15) : 0u) | (mn_q ? (1u << 16) : 0u) |
          (uint32_t((kTM * kPair) >> 3) << 17) | (uint32_t((kTM * kPair) >> 4) << 24);
+}
+
+// The MMAs of one k-block: operands at shared addresses p and q, their second planes `step` further,
+// accumulator d.  Which way the operands lie is a template parameter: with descriptors that
+// depend on run-time values each MMA took 270 cycles to issue, four times its execution.
+template <int kPair, bool kMnP, bool kMnQ, int kPlanes>
+__device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, uint32_t step,
+                                            bool accumulate) {
+  const uint64_t p_hi = kMnP ? desc_mn(p) : desc_k(p), q_hi = kMnQ ? desc_mn(q) : desc_k(q);
+  const uint64_t p_lo = kMnP ? desc_mn(p + step) : desc_k(p + step);
+  const uint64_t q_lo = kMnQ ? desc_mn(q + step) : desc_k(q + step);
+  // a K = 16 slice further: 32 bytes inside the swizzled rows (K-major), two 8-k groups (MN-major)
+  constexpr uint64_t kStepP = kMnP ? (2048 >> 4) : (32 >> 4), kStepQ = kMnQ ? (2048 >> 4) : (32 >> 4);
+  constexpr uint32_t idesc = idesc_of<kPair>(kMnP, kMnQ);
+#pragma unroll
+  for (int k = 0; k < kTK / kUmmaK; ++k) {
+    umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, accumulate || k != 0 ? 1u : 0u);
+    if constexpr (kPlanes == 2) {
+      umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u);
+      umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -516,6 +543,7 @@ struct GemmArgs {
   int32_t set_tiles;       // of all matrices of one set of operands
   int32_t total_tiles;     // of both sets
   int32_t k_blocks;
+  int32_t planes;          // 2: hi and lo of each operand and output, 1: hi alone
   float mult[2];           // accumulator -> plane (or, last, output) value, by set
   const __half* in;        // poly: planes of A
   int64_t ld, plane;
@@ -526,6 +554,17 @@ struct GemmArgs {
   float lr, weight_decay, scale;
   const float* lr_device;
 };
+
+// 32 fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void read_piece(uint32_t taddr, float (&y)[kPiece]) {
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    uint32_t v[16];
+    tmem_ld16(taddr + uint32_t(g * 16), v);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y[g * 16 + k] = __uint_as_float(v[k]);
+  }
+}
 
 // Staging of a warp.  Planes: 32 rows of 64 bytes, 16-byte granules swizzled as TMA's 64-byte mode
 // has it (granule index XOR address bits 7-8), so that neither rows nor granules collide.
@@ -550,10 +589,10 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* staging = smem + kStages * kStageBytes;   // [epilogue warp]
+  uint8_t* staging = smem + kRingBytes;   // [epilogue warp]
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kStagingBytes);
-  uint64_t* empty = full + kStages;   // in each CTA
-  uint64_t* tfull = empty + kStages;  // in each CTA
+  uint64_t* empty = full + kMaxStages;   // in each CTA
+  uint64_t* tfull = empty + kMaxStages;  // in each CTA
   uint64_t* tempty = tfull + 2;       // rank 0's counts the epilogue warps of both CTAs
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -565,8 +604,10 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   const uint32_t rank = kPair == 2 ? cluster_rank() : 0u;
   const int slot0 = int(blockIdx.x) / kPair, slots = int(gridDim.x) / kPair;
 
+  const int planes = args.planes, stages = planes == 2 ? 3 : 6;
+  const uint32_t stage_bytes = uint32_t(planes) * 2 * kPlaneBytes;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(full + s, 1);
       mbar_init(empty + s, 1);
     }
@@ -606,6 +647,132 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     }
   };
 
+  // ---------------- what an epilogue warp does with a 32 x 32 piece of the output --------------
+  // A TMEM lane quadrant and a half of the tile's columns per warp.
+  const int ew = warp - 2;
+  const int quad = warp & 3;
+  const int half = ew >> 2;
+  const uint32_t lane_addr = tmem_base + (uint32_t(quad * 32) << 16);
+  uint8_t* stage_out = staging + ew * kStagingBytes;
+  int set = 0, mat = 0, row = 0, row0 = 0;   // of the current tile: this lane's row, the warp's first
+  float keep = 0.0f, step = 0.0f;
+  // What the epilogue reads is loaded a piece ahead, the first one while the MMAs run, along the
+  // rows in memory: of a plane 4 lanes take a row's 64 bytes; of the weights a lane takes a
+  // column (of the transposed ones a row).
+  uint4 in_v[2][4];
+  T w[kPiece];   // as stored: a conversion here would wait for each load before the next
+  // final step: this lane's place in the first line of a piece in the caller's matrix (lines are
+  // the piece's rows, or its columns where transposed), and how many lines it has there
+  auto first_line = [&](int col0, int& lines) {
+    const int a = args.transposed ? col0 : row0, b = args.transposed ? row : col0 + lane;
+    lines = args.transposed ? (b < args.m ? args.n - a : 0) : (b < args.n ? args.m - a : 0);
+    return int64_t(a) * args.out_ld + b;
+  };
+  auto prefetch = [&](int col0) {
+    if constexpr (kMode == kPoly) {
+      const int c = col0 + (lane & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = row0 + i * 8 + (lane >> 2);
+        const bool inside = r < args.m && c < int(args.ld);   // ld is a multiple of 8
+        const __half* at = args.in + int64_t(mat) * 2 * args.plane + int64_t(r) * args.ld + c;
+        in_v[0][i] = inside ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
+        in_v[1][i] = inside && args.planes == 2 ? *reinterpret_cast<const uint4*>(at + args.plane)
+                                                : make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else if constexpr (kMode == kFinal) {
+      if (args.has_momentum) {
+        int lines;
+        const T* p = static_cast<const T*>(outs.p[mat]) + first_line(col0, lines);
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k, p += args.out_ld)
+          if (k < lines) w[k] = *p;
+      }
+    }
+  };
+  // The piece at column col0 of the output; next: the column to prefetch then, or -1.
+  auto finish = [&](int col0, float (&y)[kPiece], int next) {
+    const float mult = args.mult[set];
+#pragma unroll
+    for (int k = 0; k < kPiece; ++k) y[k] *= mult;
+    if constexpr (kMode == kFinal) {
+      float o[kPiece];   // element k of this lane's column (transposed: row)
+      if (args.transposed) {
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) o[k] = y[k];
+      } else {
+        // through the staging, each word at column XOR row: no two lanes in one bank either way
+        float* f = reinterpret_cast<float*>(stage_out);
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) f[lane * kPiece + (k ^ lane)] = y[k];
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) o[k] = f[k * kPiece + (lane ^ k)];
+        __syncwarp();
+      }
+      if (args.has_momentum) {
+#pragma unroll
+        for (int k = 0; k < kPiece; ++k) o[k] = fmaf(keep, load1(&w[k]), -step * o[k]);
+      }
+      if (next >= 0) prefetch(next);
+      int lines;
+      T* p = static_cast<T*>(const_cast<void*>(outs.p[mat])) + first_line(col0, lines);
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k, p += args.out_ld)
+        if (k < lines) *p = from_float<T>(o[k]);
+    } else {
+      // the staging's previous store has read it
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();
+      if constexpr (kMode == kPoly) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage_out + h * (kStagingBytes / 2) +
+                                      plane_offset(i * 8 + (lane >> 2), lane & 3)) = in_v[h][i];
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < kPiece / 8; ++g) {
+          float x[8];
+          join8(*reinterpret_cast<const uint4*>(stage_out + plane_offset(lane, g)),
+                *reinterpret_cast<const uint4*>(stage_out + kStagingBytes / 2 +
+                                                plane_offset(lane, g)), x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            float& o = y[g * 8 + k];
+            o = fmaf(kB, x[k], kC * o);
+            if (row == col0 + g * 8 + k) o += kA * kScale;
+          }
+        }
+        __syncwarp();
+        if (next >= 0) prefetch(next);
+      }
+#pragma unroll
+      for (int g = 0; g < kPiece / 8; ++g) {
+        __half hi[8], lo[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) split(y[g * 8 + k], hi[k], lo[k]);
+        *reinterpret_cast<uint4*>(stage_out + plane_offset(lane, g)) =
+            make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
+                       pack2(hi[6], hi[7]));
+        *reinterpret_cast<uint4*>(stage_out + kStagingBytes / 2 + plane_offset(lane, g)) =
+            make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
+                       pack2(lo[6], lo[7]));
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0 && row0 < args.m && col0 < args.n) {   // TMA leaves out what lies beyond
+        const CUtensorMap* out = set ? &tm_out1 : &tm_out0;
+        tma_store_3d(out, stage_out, col0, row0, 2 * mat);
+        if (args.planes == 2)
+          tma_store_3d(out, stage_out + kStagingBytes / 2, col0, row0, 2 * mat + 1);
+        bulk_commit();
+      }
+    }
+  };
+  constexpr int kPieces = kTile / 2 / kPiece;   // of a warp's half of the columns
+
   if (warp == 0) {
     // ---------------- TMA producer: this CTA's 128 rows of P, its 128 rows or columns of Q ------
     if (lane == 0) {
@@ -613,39 +780,38 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       uint32_t phase = 0;
       bool ok = true, wrapped = false;
       for (int tile = slot0; tile < args.total_tiles && ok; tile += slots) {
-        int set, mat, tr, tc;
-        locate(tile, set, mat, tr, tc);
-        const CUtensorMap* tm_q = set ? &tm_q1 : &tm_q0;
+        int tset, tmat, tr, tc;
+        locate(tile, tset, tmat, tr, tc);
+        const CUtensorMap* tm_q = tset ? &tm_q1 : &tm_q0;
         const int p0 = tr * kTile + int(rank) * kTM, q0 = tc * kTile + int(rank) * kTM;
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!wait_phase(empty + stage, phase ^ 1u, abort)) { ok = false; break; }
-          uint8_t* s = smem + stage * kStageBytes;
+          uint8_t* s = smem + stage * stage_bytes;
           uint32_t bar = smem_u32(full + stage);
           if constexpr (kPair == 2) bar = cluster_addr(full + stage, 0);
-          if (rank == 0) mbar_expect_tx(full + stage, kPair * kStageBytes);
+          if (rank == 0) mbar_expect_tx(full + stage, kPair * stage_bytes);
           auto load = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
             if constexpr (kPair == 1) tma_load_3d(dst, map, full + stage, x, y, z);
             else tma_load_3d_pair(dst, map, bar, x, y, z);
           };
           const bool mn_p = kSymP && kb * kTK / kTile > tr;
           const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < planes; ++h) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {   // boxes of 64 x 64: 64 rows, or 64 columns
               const int p = p0 + b * 64, q = q0 + b * 64, k = kb * kTK;
               load(s + h * kPlaneBytes + b * kBoxBytes, &tm_p, mn_p ? p : k, mn_p ? k : p,
-                   2 * mat + h);
-              load(s + (2 + h) * kPlaneBytes + b * kBoxBytes, tm_q, mn_q ? q : k, mn_q ? k : q,
-                   2 * mat + h);
+                   2 * tmat + h);
+              load(s + (planes + h) * kPlaneBytes + b * kBoxBytes, tm_q, mn_q ? q : k, mn_q ? k : q,
+                   2 * tmat + h);
             }
           }
-          if (++stage == kStages) { stage = 0; phase ^= 1u; wrapped = true; }
+          if (++stage == stages) { stage = 0; phase ^= 1u; wrapped = true; }
         }
       }
       if (!ok && rank == 0) {
         // given up: the copies in flight land before the block (or the pair) ends
-        for (int s = 0; s < kStages; ++s)
+        for (int s = 0; s < stages; ++s)
           if (s < stage || wrapped) drain_phase(full + s, s < stage ? phase : phase ^ 1u);
       }
     }
@@ -661,36 +827,37 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       };
       for (int tile = slot0; tile < args.total_tiles && ok; tile += slots, ++local) {
         const int acc = local & 1;
-        int set, mat, tr, tc;
-        locate(tile, set, mat, tr, tc);
+        int tset, tmat, tr, tc;
+        locate(tile, tset, tmat, tr, tc);
         if (!wait_phase(tempty + acc, ((local >> 1) & 1) ^ 1u, abort)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + uint32_t(acc * kTile);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!wait_phase(full + stage, phase, abort)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t s = smem_u32(smem + stage * kStageBytes);
+          const uint32_t s = smem_u32(smem + stage * stage_bytes);
           const bool mn_p = kSymP && kb * kTK / kTile > tr;
           const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
-          auto desc = [&](bool mn, int plane) {
-            return mn ? desc_mn(s + plane * kPlaneBytes) : desc_k(s + plane * kPlaneBytes);
-          };
-          const uint64_t p_hi = desc(mn_p, 0), p_lo = desc(mn_p, 1);
-          const uint64_t q_hi = desc(mn_q, 2), q_lo = desc(mn_q, 3);
-          // a K = 16 slice further: 32 bytes inside the swizzled rows (K-major), two 8-k groups
-          // (MN-major)
-          const uint64_t step_p = mn_p ? (2048 >> 4) : (32 >> 4);
-          const uint64_t step_q = mn_q ? (2048 >> 4) : (32 >> 4);
-          const uint32_t idesc = idesc_of<kPair>(mn_p, mn_q);
-#pragma unroll
-          for (int k = 0; k < kTK / kUmmaK; ++k) {
-            umma_f16<kPair>(d, p_hi + k * step_p, q_hi + k * step_q, idesc, (kb | k) != 0 ? 1u : 0u);
-            umma_f16<kPair>(d, p_hi + k * step_p, q_lo + k * step_q, idesc, 1u);
-            umma_f16<kPair>(d, p_lo + k * step_p, q_hi + k * step_q, idesc, 1u);
+          if (planes == 2) {
+            if (mn_p) {
+              if (mn_q) issue_block<kPair, true, true, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
+              else issue_block<kPair, true, false, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
+            } else {
+              if (mn_q) issue_block<kPair, false, true, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
+              else issue_block<kPair, false, false, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
+            }
+          } else {
+            if (mn_p) {
+              if (mn_q) issue_block<kPair, true, true, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
+              else issue_block<kPair, true, false, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
+            } else {
+              if (mn_q) issue_block<kPair, false, true, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
+              else issue_block<kPair, false, false, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
+            }
           }
           issued = true;
           commit_all(empty + stage);
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
         if (ok) commit_all(tfull + acc);
       }
@@ -701,14 +868,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       }
     }
   } else {
-    // ---------------- epilogue: a TMEM lane quadrant and a column half per warp ----------------
-    const int ew = warp - 2;
-    const int quad = warp & 3;
-    const int half = ew >> 2;
-    const uint32_t lane_addr = tmem_base + (uint32_t(quad * 32) << 16);
-    constexpr int kPieces = kTile / 2 / kPiece;   // of this warp's half of the columns
-    uint8_t* stage = staging + ew * kStagingBytes;
-    float keep = 0.0f, step = 0.0f;
+    // ---------------- epilogue ----------------
     if (kMode == kFinal && args.has_momentum) {
       const float lr = args.lr_device != nullptr ? *args.lr_device : args.lr;
       keep = 1.0f - lr * args.weight_decay;
@@ -717,64 +877,22 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     int local = 0;
     for (int tile = slot0; tile < args.total_tiles; tile += slots, ++local) {
       const int acc = local & 1;
-      int set, mat, tr, tc;
+      int tr, tc;
       locate(tile, set, mat, tr, tc);
-      const int row = tr * kTile + int(rank) * kTM + quad * 32 + lane;
+      row0 = tr * kTile + int(rank) * kTM + quad * 32;
+      row = row0 + lane;
       const int col_base = tc * kTile + half * (kTile / 2);
-      const int row0 = row - lane;
-      // What the epilogue reads is loaded a piece ahead, the first one while the MMAs run, along the
-      // rows in memory: of a plane 4 lanes take a row's 64 bytes; of the weights a lane takes a
-      // column (of the transposed ones a row).
-      uint4 in_v[2][4];
-      T w[kPiece];   // as stored: a conversion here would wait for each load before the next
-      // final step: this lane's place in the first line of a piece in the caller's matrix (lines are
-      // the piece's rows, or its columns where transposed), and how many lines it has there
-      auto first_line = [&](int col0, int& lines) {
-        const int a = args.transposed ? col0 : row0, b = args.transposed ? row : col0 + lane;
-        lines = args.transposed ? (b < args.m ? args.n - a : 0) : (b < args.n ? args.m - a : 0);
-        return int64_t(a) * args.out_ld + b;
-      };
-      auto prefetch = [&](int piece) {
-        const int col0 = col_base + piece * kPiece;
-        if constexpr (kMode == kPoly) {
-          const int c = col0 + (lane & 3) * 8;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = row0 + i * 8 + (lane >> 2);
-            const bool inside = r < args.m && c < int(args.ld);   // ld is a multiple of 8
-            const __half* at = args.in + int64_t(mat) * 2 * args.plane + int64_t(r) * args.ld + c;
-            in_v[0][i] = inside ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
-            in_v[1][i] = inside ? *reinterpret_cast<const uint4*>(at + args.plane)
-                                : make_uint4(0u, 0u, 0u, 0u);
-          }
-        } else if constexpr (kMode == kFinal) {
-          if (args.has_momentum) {
-            int lines;
-            const T* p = static_cast<const T*>(outs.p[mat]) + first_line(col0, lines);
-#pragma unroll
-            for (int k = 0; k < kPiece; ++k, p += args.out_ld) if (k < lines) w[k] = *p;
-          }
-        }
-      };
-      prefetch(0);
+      prefetch(col_base);
       int ok = 1;
       if (lane == 0) ok = wait_phase(tfull + acc, (local >> 1) & 1, abort) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       (void)mbar_try(tfull + acc, (local >> 1) & 1);  // completed: acquire for every lane
       tc_fence_after();
-      const float mult = args.mult[set];
 #pragma unroll 1
       for (int c = 0; c < kPieces; ++c) {
-        const int col0 = col_base + c * kPiece;
         float y[kPiece];
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t v[16];
-          tmem_ld16(lane_addr + uint32_t(acc * kTile + half * (kTile / 2) + c * kPiece + g * 16), v);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) y[g * 16 + k] = __uint_as_float(v[k]) * mult;
-        }
+        read_piece(lane_addr + uint32_t(acc * kTile + half * (kTile / 2) + c * kPiece), y);
         if (c == kPieces - 1) {
           // this warp has read its part of the accumulator: hand it back to the MMA issuer
           tc_fence_before();
@@ -784,80 +902,8 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
             else mbar_arrive_cluster(cluster_addr(tempty + acc, 0));
           }
         }
-        if constexpr (kMode == kFinal) {
-          float o[kPiece];   // element k of this lane's column (transposed: row)
-          if (args.transposed) {
-#pragma unroll
-            for (int k = 0; k < kPiece; ++k) o[k] = y[k];
-          } else {
-            // through the staging, each word at column XOR row: no two lanes in one bank either way
-            float* f = reinterpret_cast<float*>(stage);
-#pragma unroll
-            for (int k = 0; k < kPiece; ++k) f[lane * kPiece + (k ^ lane)] = y[k];
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < kPiece; ++k) o[k] = f[k * kPiece + (lane ^ k)];
-            __syncwarp();
-          }
-          if (args.has_momentum) {
-#pragma unroll
-            for (int k = 0; k < kPiece; ++k) o[k] = fmaf(keep, load1(&w[k]), -step * o[k]);
-          }
-          if (c + 1 < kPieces) prefetch(c + 1);
-          int lines;
-          T* p = static_cast<T*>(const_cast<void*>(outs.p[mat])) + first_line(col0, lines);
-#pragma unroll
-          for (int k = 0; k < kPiece; ++k, p += args.out_ld)
-            if (k < lines) *p = from_float<T>(o[k]);
-        } else {
-          // the staging's previous store has read it
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
-          if constexpr (kMode == kPoly) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint4*>(stage + h * (kStagingBytes / 2) +
-                                          plane_offset(i * 8 + (lane >> 2), lane & 3)) = in_v[h][i];
-            __syncwarp();
-#pragma unroll
-            for (int g = 0; g < kPiece / 8; ++g) {
-              float x[8];
-              join8(*reinterpret_cast<const uint4*>(stage + plane_offset(lane, g)),
-                    *reinterpret_cast<const uint4*>(stage + kStagingBytes / 2 +
-                                                    plane_offset(lane, g)), x);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                float& o = y[g * 8 + k];
-                o = fmaf(kB, x[k], kC * o);
-                if (row == col0 + g * 8 + k) o += kA * kScale;
-              }
-            }
-            __syncwarp();
-            if (c + 1 < kPieces) prefetch(c + 1);
-          }
-#pragma unroll
-          for (int g = 0; g < kPiece / 8; ++g) {
-            __half hi[8], lo[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) split(y[g * 8 + k], hi[k], lo[k]);
-            *reinterpret_cast<uint4*>(stage + plane_offset(lane, g)) =
-                make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
-                           pack2(hi[6], hi[7]));
-            *reinterpret_cast<uint4*>(stage + kStagingBytes / 2 + plane_offset(lane, g)) =
-                make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
-                           pack2(lo[6], lo[7]));
-          }
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0 && row0 < args.m && col0 < args.n) {   // TMA leaves out what lies beyond
-            const CUtensorMap* out = set ? &tm_out1 : &tm_out0;
-            tma_store_3d(out, stage, col0, row0, 2 * mat);
-            tma_store_3d(out, stage + kStagingBytes / 2, col0, row0, 2 * mat + 1);
-            bulk_commit();
-          }
-        }
+        const int col0 = col_base + c * kPiece;
+        finish(col0, y, c + 1 < kPieces ? col0 + kPiece : -1);
       }
     }
     if (lane == 0) bulk_wait_all();
@@ -870,6 +916,188 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     __syncwarp();
     tc_fence_after();
     tmem_free<kPair>(tmem_base, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// A block of steps on the Gram matrix, m <= 128: one CTA to a matrix.
+// ---------------------------------------------------------------------------
+
+struct ChainArgs {
+  int32_t m, steps, planes;
+};
+
+constexpr int kChainThreads = 512;
+// A matrix in shared memory: two planes of two boxes of 128 rows x 64 columns, as TMA swizzles them.
+constexpr uint32_t kChainPlane = 2 * kPlaneBytes;
+constexpr uint32_t kChainMatrix = 2 * kChainPlane;
+constexpr uint32_t kChainSmemBytes = 1024 + 3 * kChainMatrix + 64;
+static_assert(kChainSmemBytes <= 227 * 1024, "shared memory");
+
+// Place of the 16-byte granule of columns c .. c + 7 (c a multiple of 8) of row r in a plane.
+__device__ __forceinline__ uint32_t chain_offset(int r, int c) {
+  return uint32_t(c >> 6) * kPlaneBytes + uint32_t(r) * 128u +
+         uint32_t((((c >> 3) & 7) ^ (r & 7)) << 4);
+}
+
+// From A to the product Q of the `steps` P's:
+//   P = aI + bA + cAA,  Q = P Q (first: P),  A = (P A) P.
+// A, P and Q stay in shared memory; every product is complete in tensor memory before its result
+// overwrites an operand.  All of them are symmetric, so rows serve as columns throughout.
+__global__ void __launch_bounds__(kChainThreads, 1)
+kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
+                      const __grid_constant__ CUtensorMap tm_q,
+                      const __grid_constant__ ChainArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* s_a = smem;
+  uint8_t* s_p = s_a + kChainMatrix;
+  uint8_t* s_q = s_p + kChainMatrix;
+  uint64_t* loaded = reinterpret_cast<uint64_t*>(s_q + kChainMatrix);
+  uint64_t* done = loaded + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  pdl_launch_next();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mat = blockIdx.x;
+  if (threadIdx.x == 0) {
+    mbar_init(loaded, 1);
+    mbar_init(done, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&tm_a);
+    prefetch_map(&tm_q);
+  }
+  if (warp == 0) tmem_alloc<1>(tmem_slot, kTM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait_previous();
+
+  const bool two = args.planes == 2;
+  if (threadIdx.x == 0) {
+    // rows and columns behind m arrive as zeros
+    mbar_expect_tx(loaded, uint32_t(args.planes) * kChainPlane);
+    for (int h = 0; h < args.planes; ++h)
+      for (int b = 0; b < 4; ++b)
+        tma_load_3d(s_a + h * kChainPlane + b * kBoxBytes, &tm_a, loaded, (b >> 1) * 64,
+                    (b & 1) * 64, 2 * mat + h);
+  }
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+    int ok = 1;
+    if (lane == 0) ok = wait_phase(bar, parity, abort) ? 1 : 0;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    if (ok) (void)mbar_try(bar, parity);  // completed: acquire for every lane
+    return ok != 0;
+  };
+  bool ok = __syncthreads_and(wait_all(loaded, 0)) != 0;   // the block gives up together
+
+  // a warp's part of a result: 32 rows, 32 columns
+  const int row = (warp & 3) * 32 + lane, col_base = (warp >> 2) * kPiece;
+  const uint32_t taddr = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(col_base);
+  uint32_t parity = 0;
+
+  // The product of two matrices into tensor memory, complete on return.
+  auto product = [&](const uint8_t* p, const uint8_t* q) {
+    fence_async_shared();   // the operands were written by this block's threads
+    tc_fence_before();      // and the last result has been read
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort == 0) {
+      tc_fence_after();
+      const uint32_t sp = smem_u32(p), sq = smem_u32(q);
+      if (two) {
+        issue_block<1, false, false, 2>(tmem, sp, sq, kChainPlane, false);
+        if (args.m > kTK)
+          issue_block<1, false, false, 2>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane, true);
+      } else {
+        issue_block<1, false, false, 1>(tmem, sp, sq, kChainPlane, false);
+        if (args.m > kTK)
+          issue_block<1, false, false, 1>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane, true);
+      }
+      umma_commit<1>(smem_u32(done));
+    }
+    ok = __syncthreads_and(wait_all(done, parity)) != 0;
+    parity ^= 1u;
+    tc_fence_after();
+  };
+  // The result times mult, kept as a matrix in `to` (and `also`); poly: b A + c result + a I.
+  auto keep = [&](uint8_t* to, uint8_t* also, float mult, bool poly) {
+    float y[kPiece];
+    read_piece(taddr, y);
+#pragma unroll
+    for (int g = 0; g < kPiece / 8; ++g) {
+      const int col = col_base + g * 8;
+      const uint32_t at = chain_offset(row, col);
+      __half hi[8], lo[8];
+      float x[8];
+      if (poly)
+        join8(*reinterpret_cast<const uint4*>(s_a + at),
+              two ? *reinterpret_cast<const uint4*>(s_a + kChainPlane + at)
+                  : make_uint4(0u, 0u, 0u, 0u), x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float v = y[g * 8 + k] * mult;
+        if (poly) {
+          v = fmaf(kB, x[k], kC * v);
+          if (row == col + k) v += kA * kScale;
+        }
+        split(v, hi[k], lo[k]);
+      }
+      const uint4 h = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
+                                 pack2(hi[6], hi[7]));
+      const uint4 l = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
+                                 pack2(lo[6], lo[7]));
+      *reinterpret_cast<uint4*>(to + at) = h;
+      *reinterpret_cast<uint4*>(to + kChainPlane + at) = l;
+      if (also != nullptr) {
+        *reinterpret_cast<uint4*>(also + at) = h;
+        *reinterpret_cast<uint4*>(also + kChainPlane + at) = l;
+      }
+    }
+  };
+  const float to_plane = 1.0f / kScale;
+  for (int t = 0; t < args.steps && ok; ++t) {
+    product(s_a, s_a);
+    if (!ok) break;
+    keep(s_p, t == 0 ? s_q : nullptr, to_plane, true);
+    if (t > 0) {
+      product(s_p, s_q);
+      if (!ok) break;
+      keep(s_q, nullptr, to_plane / 4.0f, false);
+    }
+    if (t + 1 < args.steps) {
+      product(s_p, s_a);
+      if (!ok) break;
+      keep(s_a, nullptr, to_plane, false);
+      product(s_a, s_p);
+      if (!ok) break;
+      keep(s_a, nullptr, to_plane, false);
+    }
+  }
+  fence_async_shared();
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (*abort == 0) {
+      // Q as it lies: four boxes of 64 x 64, cut at m
+      for (int h = 0; h < args.planes; ++h)
+        for (int b = 0; b < 4; ++b)
+          if ((b >> 1) * 64 < args.m && (b & 1) * 64 < args.m)
+            tma_store_3d(&tm_q, s_q + h * kChainPlane + b * kBoxBytes, (b >> 1) * 64, (b & 1) * 64,
+                         2 * mat + h);
+      bulk_commit();
+      bulk_wait_all();
+    } else {
+      drain_phase(loaded, 0);   // given up: the copies in flight land before the block ends
+    }
+  }
+  if (warp == 0) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free<1>(tmem, kTM);
   }
 }
 
@@ -930,10 +1158,10 @@ int sm_count(int device) {
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Steps taken on the Gram matrix at once (the blocks of an iteration): wide matrices only.  Measured
-// for twelve matrices: see run().
+// Steps taken on the Gram matrix at once (the blocks of an iteration): wide matrices, whose products
+// with X cost more, and those of up to 128 rows, for which a block is one launch.
 int block_steps(int64_t m, int64_t n, int left) {
-  if (2 * n < 3 * m) return 1;
+  if (m > kTM && 2 * n < 3 * m) return 1;
   return left == 4 ? 2 : (left < kMaxBlock ? left : kMaxBlock);
 }
 
@@ -950,7 +1178,7 @@ struct Layout {
     plane_a = m * ldm;
     const size_t bx = size_t(round_up(count * 2 * plane_x * 2, 256));
     const size_t ba = size_t(round_up(count * 2 * plane_a * 2, 256));
-    const int syms = block_steps(m, n, kMaxBlock) > 1 ? 6 : 2;
+    const int syms = m > kTM && block_steps(m, n, kMaxBlock) > 1 ? 6 : 2;
     x0 = 0;
     x1 = x0 + bx;
     size_t at = x1 + bx;
@@ -1006,18 +1234,12 @@ struct Maps {
 };
 
 template <int kMode, typename T, int kPair>
-int launch_pair(const Maps& m, GemmArgs args, const PtrTable& outs, int sets, int count, const Device& dev, cudaStream_t stream) {
+int launch_pair(const Maps& m, const GemmArgs& args, const PtrTable& outs, int slots,
+                cudaStream_t stream) {
   auto kernel = kat_muon_gemm_kernel<kMode, T, kPair>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kSmemBytes)) != cudaSuccess)
     return KAT_ERR_CUDA;
-  const int tm = (args.m + kTM * kPair - 1) / (kTM * kPair);
-  const int tn = (args.n + kTM * kPair - 1) / (kTM * kPair);
-  args.row_tiles = tm;
-  args.tiles = kMode != kApply && kMode != kFinal ? tm * (tm + 1) / 2 : tm * tn;
-  args.set_tiles = args.tiles * count;
-  args.total_tiles = args.set_tiles * sets;
-  const int slots = kPair == 2 ? dev.pairs : dev.sms;
   const int grid = args.total_tiles < slots ? args.total_tiles : slots;
   return launch_after(kernel, dim3(uint32_t(grid * kPair)), kThreads, kSmemBytes, kPair, stream,
                       m.p, m.q[0], m.q[1], m.out[0], m.out[1], args, outs)
@@ -1027,15 +1249,21 @@ int launch_pair(const Maps& m, GemmArgs args, const PtrTable& outs, int sets, in
 
 // CTA pairs on 256 x 256 tiles, or single CTAs on 128 x 128 tiles?
 template <int kMode, typename T>
-int launch_gemm(bool pair, const Maps& m, const GemmArgs& args, const PtrTable& outs, int sets,
-                int count, const Device& dev, cudaStream_t stream) {
-  return pair ? launch_pair<kMode, T, 2>(m, args, outs, sets, count, dev, stream)
-              : launch_pair<kMode, T, 1>(m, args, outs, sets, count, dev, stream);
+int launch_gemm(bool pair, const Maps& m, GemmArgs args, const PtrTable& outs, int sets, int count,
+                const Device& dev, cudaStream_t stream) {
+  const int side = pair ? 2 * kTM : kTM;
+  const int tm = (args.m + side - 1) / side, tn = (args.n + side - 1) / side;
+  args.row_tiles = tm;
+  args.tiles = kMode != kApply && kMode != kFinal ? tm * (tm + 1) / 2 : tm * tn;
+  args.set_tiles = args.tiles * count;
+  args.total_tiles = args.set_tiles * sets;
+  return pair ? launch_pair<kMode, T, 2>(m, args, outs, dev.pairs, stream)
+              : launch_pair<kMode, T, 1>(m, args, outs, dev.sms, stream);
 }
 
 template <typename T>
 int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int64_t rows,
-        int64_t cols, int32_t steps, uint8_t* ws, const Device& dev, bool vec,
+        int64_t cols, int32_t steps, int late, uint8_t* ws, const Device& dev, bool vec,
         cudaStream_t stream) {
   const Layout L(count, rows, cols);
   __half* x[2] = {reinterpret_cast<__half*>(ws + L.x0), reinterpret_cast<__half*>(ws + L.x1)};
@@ -1082,6 +1310,7 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   sq.ld = L.ldm;
   sq.plane = L.plane_a;
   sq.k_blocks = k_m;
+  sq.planes = fin.planes = 2;
   sq.mult[0] = 1.0f / kScale;
   fin.m = int32_t(L.m);
   fin.n = int32_t(L.n);
@@ -1113,6 +1342,10 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   int cur = 0;
   for (int done = 0; done < steps;) {
     const int block = block_steps(L.m, L.n, steps - done);
+    // the last steps in one plane, if the caller's type leaves them room
+    const bool last = done + block == steps;
+    if (steps - done <= late) sq.planes = 1;
+    fin.planes = sq.planes == 1 || (last && late > 0) ? 1 : 2;
     // gram
     GemmArgs g = sq;
     g.k_blocks = k_n;
@@ -1121,7 +1354,17 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
     // sym[0] = A, [1] and [2] the P's in turn, [3] = P A, [4] and [5] the products of P's
     int q = 1;         // where the product of the block's P's so far is
     float q_scale = kScale;
-    for (int t = 0; t < block; ++t) {
+    const bool chained = L.m <= kTM;
+    if (chained) {
+      const ChainArgs chain{int32_t(L.m), block, sq.planes};
+      if (cudaFuncSetAttribute(kat_muon_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               int(kChainSmemBytes)) != cudaSuccess ||
+          !launch_after(kat_muon_chain_kernel, dim3(uint32_t(count)), kChainThreads,
+                        kChainSmemBytes, 1, stream, ms[0], ms[1], chain))
+        return KAT_ERR_CUDA;
+      for (int t = 1; t < block; ++t) q_scale /= 4.0f;
+    }
+    for (int t = chained ? block : 0; t < block; ++t) {
       const int p = 1 + (t & 1);
       g = sq;
       g.in = sym[0];
@@ -1157,35 +1400,42 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   return KAT_OK;
 }
 
-// CTA pairs of these kernels that fit on `device` at once (cached), 0 if none.
-int pair_count(int device) {
-  static std::mutex mu;
-  static int cache[64] = {0};
-  std::lock_guard<std::mutex> lock(mu);
-  if (device < 0 || device >= 64) return 0;
-  if (cache[device] == 0) {
-    int best = -1;
-    auto kernel = kat_muon_gemm_kernel<kApply, float, 2>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             int(kSmemBytes)) == cudaSuccess) {
-      cudaLaunchConfig_t cfg = {};
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      cfg.blockDim = dim3(kThreads);
-      cfg.dynamicSmemBytes = kSmemBytes;
-      cfg.gridDim = dim3(128);
-      int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) best = n;
-    }
-    cudaGetLastError();
-    cache[device] = best;
+// CTA pairs that fit on the current device at once, 0 if none.
+int pair_count() {
+  auto kernel = kat_muon_gemm_kernel<kApply, float, 2>;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(kSmemBytes)) == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.gridDim = dim3(128);
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
   }
-  return cache[device] > 0 ? cache[device] : 0;
+  cudaGetLastError();
+  return n;
+}
+
+// What the current device `device` holds (asked once).
+bool device_of(int device, Device* d) {
+  static std::mutex mu;
+  static Device cache[64] = {};
+  const int sms = sm_count(device);
+  if (sms <= 0) return false;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cache[device].sms == 0) {
+    cache[device].pairs = pair_count();
+    cache[device].sms = sms;
+  }
+  *d = cache[device];
+  return true;
 }
 
 int dispatch(const Update& u, const PtrTable& outs, const GemmArgs& fin, int32_t count,
@@ -1199,18 +1449,29 @@ int dispatch(const Update& u, const PtrTable& outs, const GemmArgs& fin, int32_t
   if (tm * tn * count >= (int64_t(1) << 30)) return KAT_ERR_BAD_SHAPE;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KAT_ERR_CUDA;
-  const Device d{sm_count(dev), pair_count(dev)};
-  if (d.sms <= 0) return KAT_ERR_CUDA;
+  Device d;
+  if (!device_of(dev, &d)) return KAT_ERR_CUDA;
   bool vec = cols % 8 == 0;   // the inputs' rows take 16-byte accesses
   for (int i = 0; i < count; ++i)
     vec = vec && ((reinterpret_cast<uintptr_t>(u.x.p[i]) | reinterpret_cast<uintptr_t>(u.m.p[i])) &
                   15u) == 0;
   uint8_t* w = static_cast<uint8_t*>(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // How many of the last steps take single planes.  Rounding their operands to 11 bits is no longer
+  // amplified: the result's error grows from 1e-5 to at most 1e-3 with one such step and 3e-3 with two
+  // (over spectra from flat to 32 strong directions a hundred times the rest).  A bf16 result is
+  // itself rounded by 2e-3; a weight of 16 bits by that much of the weight, of which a step's
+  // update is a small part.
+  const int late = dtype == KAT_DTYPE_F32 ? 0
+                   : fin.has_momentum   ? 2
+                                        : (dtype == KAT_DTYPE_BF16 ? 1 : 0);
   switch (dtype) {
-    case KAT_DTYPE_F32: return run<float>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
-    case KAT_DTYPE_F16: return run<__half>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
-    default: return run<__nv_bfloat16>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
+    case KAT_DTYPE_F32:
+      return run<float>(u, outs, fin, count, rows, cols, steps, late, w, d, vec, st);
+    case KAT_DTYPE_F16:
+      return run<__half>(u, outs, fin, count, rows, cols, steps, late, w, d, vec, st);
+    default:
+      return run<__nv_bfloat16>(u, outs, fin, count, rows, cols, steps, late, w, d, vec, st);
   }
 }
 

@@ -21,21 +21,25 @@ A, B, C = 3.4445, -4.7750, 2.0315
 HALF = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.float16, torch.bfloat16)}
 
 
-def reference(u, steps=5):
+def reference(u, steps=5, late=0):
     """(result, error allowed for it before rounding) of a matrix in 64 bits."""
     x = u.double()
     flip = x.shape[0] > x.shape[1]
     x = x.t() if flip else x
     norm = x.norm()
     x = x / norm if norm > 0 else x
-    unit = 2.0 ** -22 + math.sqrt(x.shape[1]) * 2.0 ** -23
-    share = 90 if 2 * x.shape[1] >= 3 * x.shape[0] else 30
+    sums = math.sqrt(x.shape[1]) * 2.0 ** -23
+    share = 90 if 2 * x.shape[1] >= 3 * x.shape[0] or x.shape[0] <= 128 else 30
     allowed = 0.0
-    for _ in range(steps):
+    for step in range(steps):
         a = x @ x.t()
+        unit = sums + 2.0 ** (-11 if steps - step <= late else -22)
         allowed = 3.9 * allowed + share * unit * float(x.norm())
         x = A * x + (B * a + C * (a @ a)) @ x
     return (x.t() if flip else x), allowed
+
+
+LATE = {torch.float32: 0, torch.float16: 0, torch.bfloat16: 1}
 
 
 def assert_close(got, want, allowed, dtype):
@@ -55,7 +59,7 @@ def normal(*shape, seed=0, dtype=torch.float32, device="cuda"):
 def test_sizes(cuda_device, shape, dtype):
     x = normal(*shape, dtype=dtype, seed=shape[0])
     before = x.clone()
-    want, allowed = reference(x)
+    want, allowed = reference(x, late=LATE[dtype])
     assert_close(kat.orthogonalize(x), want, allowed, dtype)
     assert torch.equal(x, before) and muon.device_status() == 0
 
@@ -69,7 +73,7 @@ def test_tiles_beyond_one_wave(cuda_device, shape, dtype):
     x = normal(*shape, seed=5, dtype=dtype)
     out = kat.orthogonalize(x)
     for i in range(shape[0]):
-        want, allowed = reference(x[i])
+        want, allowed = reference(x[i], late=LATE[dtype])
         assert_close(out[i], want, allowed, dtype)
     assert muon.device_status() == 0
 
@@ -85,10 +89,34 @@ def test_spread_singular_values(cuda_device):
 
 @pytest.mark.parametrize("shape", [(96, 130), (96, 160), (300, 1100)])
 @pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 8])
-def test_steps(cuda_device, steps, shape):
-    x = normal(*shape)
-    want, allowed = reference(x, steps)
-    assert_close(kat.orthogonalize(x, steps=steps), want, allowed, torch.float32)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_steps(cuda_device, steps, shape, dtype):
+    x = normal(*shape, dtype=dtype)
+    want, allowed = reference(x, steps, LATE[dtype])
+    assert_close(kat.orthogonalize(x, steps=steps), want, allowed, dtype)
+
+
+@pytest.mark.parametrize("count,m,n", [(1, 130, 140), (1, 250, 900), (2, 300, 310), (5, 128, 256),
+                                       (9, 200, 70), (30, 64, 64), (1, 768, 768)])
+def test_few_tiles(cuda_device, count, m, n):
+    """Fewer tiles than SMs; a block of steps in one CTA, and products of their own."""
+    x = normal(count, m, n, seed=m)
+    out = kat.orthogonalize(x)
+    for i in range(count):
+        want, allowed = reference(x[i])
+        assert_close(out[i], want, allowed, torch.float32)
+    assert muon.device_status() == 0
+
+
+def test_error_is_small(cuda_device):
+    """Far below the bounds above: 1e-4 of fp32 results, 3e-3 of bf16 ones with their rounding."""
+    for shape in ((300, 400), (256, 1000)):
+        x = normal(*shape)
+        want, _ = reference(x)
+        assert float((kat.orthogonalize(x).double() - want).norm() / want.norm()) < 1e-4
+        x = x.bfloat16()
+        want, _ = reference(x)
+        assert float((kat.orthogonalize(x).double() - want).norm() / want.norm()) < 3e-3
 
 
 def test_batches_and_strides(cuda_device):
@@ -138,7 +166,7 @@ def test_low_rank(cuda_device):
 def step_reference(w, g, m, lr, mu, nesterov, wd, steps=5):
     m = mu * m.double() + g.double()
     u = g.double() + mu * m if nesterov else m
-    o, allowed = reference(u, steps)
+    o, allowed = reference(u, steps, late=0 if w.dtype == torch.float32 else 2)
     s = 0.2 * math.sqrt(max(w.shape))
     return w.double() * (1 - lr * wd) - lr * s * o, m, lr * s * allowed
 
