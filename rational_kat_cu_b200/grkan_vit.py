@@ -18,6 +18,11 @@ uses torch's scaled_dot_product_attention; the linear layers are cuBLAS GEMMs, e
 their epilogues (fused_gemm.KANMlpFused: act2's forward in fc1's epilogue, its backward in the
 epilogue of fc2's input-gradient GEMM).
 
+Three options of the attention blocks, off by default, run on kernels of their own: `qk_norm`
+(queries and keys normalised for each head), `rope` (with it: their rotation by the patch's row and
+column) and `rel_pos_bias` (a learned bias by the displacement of two patches).
+make_optimizer(matrices="muon") updates the blocks' weight matrices by orthogonalised momentum.
+
 Training step: cross-entropy on the class logits, backward, optimizer step.  Data parallel
 is one process per GPU with DistributedDataParallel over NCCL; the KAT coefficient
 gradients either ride DDP's buckets (kat_exchange="ddp") or are left out of DDP and
@@ -29,14 +34,17 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, Optional, Sequence
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from . import fused_gemm
+from .head_norm import QKNormRope, rope_grid_table
 from .kat_1dgroup import KAT_Group
+from .muon import Muon
+from .position_bias import GridPositionBias
 
 
 @dataclass
@@ -53,6 +61,9 @@ class ViTConfig:
     drop: float = 0.0
     act: str = "kat"             # "kat" (GR-KAN) or "gelu" (plain ViT MLP)
     fused_gemm: bool = False     # KAN block: act2 in the fc1 / fc2-dgrad GEMM epilogues
+    qk_norm: bool = False        # queries and keys normalised for each head (CUDA only)
+    rope: bool = False           # ... and rotated by the patch's row and column (needs qk_norm)
+    rel_pos_bias: bool = False   # learned bias by the displacement of two patches (CUDA only)
 
     @property
     def num_tokens(self) -> int:
@@ -116,17 +127,28 @@ class GeluMLP(nn.Module):
 
 
 class Attention(nn.Module):
-    def __init__(self, dim: int, num_heads: int):
+    """Multi-head self-attention.  norm_rope: a `QKNormRope` applied to the projection's output;
+    pos_bias: a `GridPositionBias` added to the scores."""
+
+    def __init__(self, dim: int, num_heads: int, norm_rope: Optional[QKNormRope] = None,
+                 pos_bias: Optional[GridPositionBias] = None):
         super().__init__()
         self.num_heads = num_heads
         self.qkv = nn.Linear(dim, dim * 3)
         self.proj = nn.Linear(dim, dim)
+        self.norm_rope = norm_rope
+        self.pos_bias = pos_bias
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         B, L, C = x.shape
-        qkv = self.qkv(x).view(B, L, 3, self.num_heads, C // self.num_heads).permute(2, 0, 3, 1, 4)
-        q, k, v = qkv.unbind(0)   # (indexing would make its backward zero-fill the whole qkv)
-        o = F.scaled_dot_product_attention(q, k, v)
+        qkv = self.qkv(x)
+        if self.norm_rope is not None:
+            q, k, v = (t.transpose(1, 2) for t in self.norm_rope(qkv))
+        else:
+            qkv = qkv.view(B, L, 3, self.num_heads, C // self.num_heads).permute(2, 0, 3, 1, 4)
+            q, k, v = qkv.unbind(0)   # (indexing would make its backward zero-fill the whole qkv)
+        bias = None if self.pos_bias is None else self.pos_bias(q.dtype)
+        o = F.scaled_dot_product_attention(q, k, v, attn_mask=bias)
         return self.proj(o.transpose(1, 2).reshape(B, L, C))
 
 
@@ -135,8 +157,18 @@ class Block(nn.Module):
         super().__init__()
         dim = cfg.embed_dim
         hidden = int(dim * cfg.mlp_ratio)
+        side = cfg.image_size // cfg.patch_size
+        head_dim = dim // cfg.num_heads
+        norm_rope = pos_bias = None
+        if cfg.rope and not cfg.qk_norm:
+            raise ValueError("ViTConfig: rope needs qk_norm (they are one pass)")
+        if cfg.qk_norm:
+            table = rope_grid_table(side, side, head_dim, prefix=1) if cfg.rope else None
+            norm_rope = QKNormRope(head_dim, cfg.num_heads, table=table)
+        if cfg.rel_pos_bias:
+            pos_bias = GridPositionBias(cfg.num_heads, side, side, prefix=1)
         self.norm1 = nn.LayerNorm(dim, eps=1e-6)
-        self.attn = Attention(dim, cfg.num_heads)
+        self.attn = Attention(dim, cfg.num_heads, norm_rope, pos_bias)
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
         if cfg.act == "kat":
             self.mlp = KAN(dim, hidden, cfg.num_groups, drop=cfg.drop, device=kat_device,
@@ -220,14 +252,58 @@ def wrap_data_parallel(model: nn.Module, kat_exchange: str = "ddp", device_ids=N
     return DDP(model, device_ids=device_ids, **ddp_kwargs)
 
 
+class OptimizerSet:
+    """Optimizers that step together, each with parameters of its own."""
+
+    def __init__(self, optimizers: Sequence[torch.optim.Optimizer]):
+        self.optimizers = list(optimizers)
+
+    @property
+    def param_groups(self) -> List[dict]:
+        return [g for o in self.optimizers for g in o.param_groups]
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for o in self.optimizers:
+            o.zero_grad(set_to_none=set_to_none)
+
+    def step(self) -> None:
+        for o in self.optimizers:
+            o.step()
+
+    def state_dict(self) -> dict:
+        return {"optimizers": [o.state_dict() for o in self.optimizers]}
+
+    def load_state_dict(self, state: dict) -> None:
+        if len(state["optimizers"]) != len(self.optimizers):
+            raise ValueError(f"OptimizerSet: {len(self.optimizers)} optimizers, and the state of "
+                             f"{len(state['optimizers'])}")
+        for o, s in zip(self.optimizers, state["optimizers"]):
+            o.load_state_dict(s)
+
+
+def block_matrices(model: nn.Module) -> List[nn.Parameter]:
+    """The weight matrices of the linear layers in the model's blocks."""
+    model = getattr(model, "module", model)   # inside DistributedDataParallel
+    return [m.weight for m in model.blocks.modules() if isinstance(m, nn.Linear)]
+
+
 def make_optimizer(model: nn.Module, lr: float = 1e-4, weight_decay: float = 0.05,
-                   capturable: bool = False):
+                   capturable: bool = False, matrices: str = "adamw"):
     """AdamW; the fused CUDA implementation when the parameters are on a GPU (capturable=True
-    for use inside a CUDA graph)."""
+    for use inside a CUDA graph).  matrices="muon": the blocks' weight matrices go to `Muon` (CUDA
+    only; its updates have the size of AdamW's, so both take the same lr), the rest to AdamW."""
+    if matrices not in ("adamw", "muon"):
+        raise ValueError(f"matrices must be 'adamw' or 'muon', got {matrices!r}")
     params = list(model.parameters())
     fused = bool(params) and params[0].is_cuda
-    return torch.optim.AdamW(params, lr=lr, weight_decay=weight_decay, fused=fused,
-                             capturable=capturable and fused)
+    muon = block_matrices(model) if matrices == "muon" else []
+    chosen = {id(p) for p in muon}
+    adamw = torch.optim.AdamW([p for p in params if id(p) not in chosen], lr=lr,
+                              weight_decay=weight_decay, fused=fused,
+                              capturable=capturable and fused)
+    if not muon:
+        return adamw
+    return OptimizerSet([Muon(muon, lr=lr, weight_decay=weight_decay), adamw])
 
 
 def train_step(model: nn.Module, optimizer, images: torch.Tensor,

@@ -5,7 +5,10 @@ result by a change of its input is at most L = max(|p'|, |p(s)/s|) = 3.9 on [0, 
 error is at most (|a| + 2 |b| s^2 + 3 |c| s^4) u |X|_F < 30 u |X|_F (s <= 1.21), u being the
 error of one product relative to its operands' Frobenius norms: 2^-22 from the two planes of each
 operand and sqrt(K) 2^-23 from adding K terms in fp32 (rounding or cutting).  So the result is within
-30 u sum_j L^j |X_(steps - j)|_F of the exact one, plus half a step of the output's type."""
+30 u sum_j L^j |X_(steps - j)|_F of the exact one, plus half a step of the output's type.  Wide and
+small matrices (2 n >= 3 m, or m <= 128) take blocks of steps on their Gram matrix, with at most three
+times the products a step, each with the same error: 90 instead of 30.  The last step of a bf16 result
+and the last two of a 16-bit weight take single planes: u = 2^-11 from two operands of 11 bits."""
 
 import math
 
