@@ -2,8 +2,8 @@
 // include/kat_position_bias.h).
 //
 // Distance form.  The bias is constant along diagonals.  Forward: a block looks its diagonals'
-// values up once into shared memory; a thread owns 8 columns and walks down the rows, where its
-// window of 8 values moves by one: one shared-memory read and a shift for every 16-byte
+// values up once into shared memory; a thread owns 16 bytes of columns and walks down the rows, where its
+// window of 16 bytes moves by one: one shared-memory read and a shift for every 16-byte
 // store.  Backward: a thread owns 15 neighbouring diagonals and keeps their sums in registers: it
 // takes 8 x 8 cells at a time, stepping 8 rows down and 8 columns right, so that every cell is
 // read once, in 16-byte accesses, and no two threads add to one sum.  The cells come by cp.async
@@ -11,7 +11,7 @@
 // flight (dout[16,4096,4096] bf16: 132 us, 62 % of the copy rate).  Where rows do not start on 16
 // bytes, a thread owns one diagonal and a warp reads 32 neighbouring cells of a row.
 //
-// Index form.  Forward: the table's columns of a few heads in shared memory, 8 cells of the index
+// Index form.  Forward: the table's columns of a few heads in shared memory, cells of the index
 // read once for all of them.  Backward: a slab of whole rows goes to shared memory in 16-byte
 // accesses; then one thread sums each segment (cells of one bucket, listed by the caller) there.
 //
@@ -31,11 +31,12 @@ namespace {
 
 constexpr int64_t kMaxLength = (int64_t(1) << 31) - 64;
 
+// Read-only loads: the compiler may gather them before the stores to shared memory they alternate with.
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   switch (dtype) {
-    case KAT_DTYPE_F32: return static_cast<const float*>(p)[i];
-    case KAT_DTYPE_F16: return __half2float(static_cast<const __half*>(p)[i]);
-    default: return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    case KAT_DTYPE_F32: return __ldg(static_cast<const float*>(p) + i);
+    case KAT_DTYPE_F16: return __half2float(__ldg(static_cast<const __half*>(p) + i));
+    default: return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
   }
 }
 __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
@@ -53,11 +54,9 @@ template <typename T> __device__ __forceinline__ typename Bits<T>::U bits_of(flo
   return Codec<T>::pack1(v);
 }
 
-// 8 neighbouring values of a row as words; `keep` of them count, the others become zero.
-template <typename T> struct Window {
-  static constexpr int kWords = 2 * int(sizeof(T));
-  uint32_t w[kWords];
-};
+// 16 bytes of neighbouring values of a row.  One 16-byte store a thread and row, the lanes next to each
+// other (two stores to a thread, 32 bytes apart from lane to lane, took three times as long).
+template <typename T> constexpr int kCols = 16 / int(sizeof(T));
 
 // ---------------------------------------------------------------------------
 // Distance form, forward.
@@ -82,11 +81,12 @@ kat_distance_bias_fwd_kernel(const __grid_constant__ DistanceFwd a) {
   extern __shared__ uint32_t fwd_smem[];
   U* f = reinterpret_cast<U*>(fwd_smem);
   const int h = blockIdx.y;
-  const int64_t j0 = int64_t(blockIdx.x % a.col_blocks) * a.tx * 8;
+  constexpr int kC = kCols<T>;
+  const int64_t j0 = int64_t(blockIdx.x % a.col_blocks) * a.tx * kC;
   const int64_t i0 = int64_t(blockIdx.x / a.col_blocks) * a.ty * a.rows;
   const int span = a.ty * a.rows;
   const int64_t first = j0 - (i0 + span - 1) - a.offset;   // distance of f[0]
-  for (int k = threadIdx.x; k < 8 * a.tx + span - 1; k += kFwdThreads) {
+  for (int k = threadIdx.x; k < kC * a.tx + span - 1; k += kFwdThreads) {
     const int64_t d = first + k;
     if (a.causal && d > 0) {
       f[k] = bits_of<T>(-__int_as_float(0x7f800000));
@@ -98,45 +98,38 @@ kat_distance_bias_fwd_kernel(const __grid_constant__ DistanceFwd a) {
   }
   __syncthreads();
   const int tx = threadIdx.x % a.tx, ty = threadIdx.x / a.tx;
-  const int64_t j = j0 + 8 * tx;
+  const int64_t j = j0 + kC * tx;
   const int64_t i = i0 + int64_t(ty) * a.rows;
   if (j >= a.ld || i >= a.lq) return;
   // columns behind lk are zero
-  uint32_t keep[Window<T>::kWords];
+  uint32_t keep[4], w[4];
+  const U* at = f + kC * tx + span - 1 - ty * a.rows;   // (i, j)
 #pragma unroll
-  for (int k = 0; k < Window<T>::kWords; ++k) {
+  for (int k = 0; k < 4; ++k) {
     if constexpr (sizeof(T) == 4) {
       keep[k] = j + k < a.lk ? 0xffffffffu : 0u;
+      w[k] = at[k];
     } else {
       keep[k] = (j + 2 * k < a.lk ? 0xffffu : 0u) | (j + 2 * k + 1 < a.lk ? 0xffff0000u : 0u);
+      w[k] = uint32_t(at[2 * k]) | (uint32_t(at[2 * k + 1]) << 16);
     }
   }
-  const U* at = f + 8 * tx + span - 1 - ty * a.rows;   // (i, j)
-  Window<T> v;
-#pragma unroll
-  for (int k = 0; k < Window<T>::kWords; ++k) {
-    if constexpr (sizeof(T) == 4) v.w[k] = at[k];
-    else v.w[k] = uint32_t(at[2 * k]) | (uint32_t(at[2 * k + 1]) << 16);
-  }
   uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t(h) * a.lq + i) * a.ld + j);
-  const int64_t step = a.ld * int64_t(sizeof(T)) / 16;
+  const int64_t step = a.ld / kC;
   const int rows = int(a.lq - i < a.rows ? a.lq - i : a.rows);
   for (int r = 0; r < rows; ++r) {
-#pragma unroll
-    for (int q = 0; q < Window<T>::kWords / 4; ++q)
-      out[q] = make_uint4(v.w[4 * q] & keep[4 * q], v.w[4 * q + 1] & keep[4 * q + 1],
-                          v.w[4 * q + 2] & keep[4 * q + 2], v.w[4 * q + 3] & keep[4 * q + 3]);
+    *out = make_uint4(w[0] & keep[0], w[1] & keep[1], w[2] & keep[2], w[3] & keep[3]);
     out += step;
     if (r + 1 == rows) break;
     // one row down: every value moves one column right
     const uint32_t next = *--at;
 #pragma unroll
-    for (int k = Window<T>::kWords - 1; k > 0; --k) {
-      if constexpr (sizeof(T) == 4) v.w[k] = v.w[k - 1];
-      else v.w[k] = __funnelshift_l(v.w[k - 1], v.w[k], 16);
+    for (int k = 3; k > 0; --k) {
+      if constexpr (sizeof(T) == 4) w[k] = w[k - 1];
+      else w[k] = __funnelshift_l(w[k - 1], w[k], 16);
     }
-    if constexpr (sizeof(T) == 4) v.w[0] = next;
-    else v.w[0] = (v.w[0] << 16) | next;
+    if constexpr (sizeof(T) == 4) w[0] = next;
+    else w[0] = (w[0] << 16) | next;
   }
 }
 
@@ -380,13 +373,13 @@ struct IndexFwd {
   const void* table;
   const int32_t* index;
   void* out;
-  int64_t chunks;          // lq * ld / 8
+  int64_t chunks;          // lq * ld cells, 16 bytes of the output to a chunk
   int32_t table_dtype, num_buckets, heads;
   int32_t group;           // heads of a block
 };
 
-// Neighbouring cells of a grid's row have neighbouring buckets, 8 apart from lane to lane: one word
-// more every 32 keeps them in different banks.
+// Neighbouring cells of a grid's row have neighbouring buckets, a power of two apart from lane to lane:
+// one place more every 32 keeps them in different banks.
 __device__ __forceinline__ int spread(int b) { return b + (b >> 5); }
 
 template <typename T, bool kSmem>
@@ -399,27 +392,52 @@ kat_index_bias_fwd_kernel(const __grid_constant__ IndexFwd a) {
   const int heads = a.heads - h0 < a.group ? a.heads - h0 : a.group;
   const int pitch = spread(a.num_buckets) + 1;   // the last one is the zero of cells without bias
   if constexpr (kSmem) {
-#pragma unroll 4
-    for (int b = threadIdx.x; b < a.num_buckets; b += kIdxThreads)
-      for (int h = 0; h < heads; ++h)
-        f[h * pitch + spread(b)] =
-            bits_of<T>(load_any(a.table, a.table_dtype, int64_t(b) * a.heads + h0 + h));
+    // table rows four at a time, four of their heads each, all loads before the stores
+    for (int b0 = threadIdx.x; b0 < a.num_buckets; b0 += 4 * kIdxThreads) {
+      for (int g = 0; g < heads; g += 4) {
+        float v[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int b = b0 + i * kIdxThreads;
+            v[i][h] = b < a.num_buckets && g + h < heads
+                          ? load_any(a.table, a.table_dtype, int64_t(b) * a.heads + h0 + g + h)
+                          : 0.0f;
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int b = b0 + i * kIdxThreads;
+            if (b < a.num_buckets && g + h < heads) f[(g + h) * pitch + spread(b)] = bits_of<T>(v[i][h]);
+          }
+      }
+    }
     for (int h = threadIdx.x; h < heads; h += kIdxThreads)
       f[h * pitch + spread(a.num_buckets)] = U(0);
     __syncthreads();
   }
   for (int64_t k = int64_t(blockIdx.x) * kIdxThreads + threadIdx.x; k < a.chunks;
        k += int64_t(gridDim.x) * kIdxThreads) {
-    const int4 lo = __ldg(reinterpret_cast<const int4*>(a.index) + 2 * k);
-    const int4 hi = __ldg(reinterpret_cast<const int4*>(a.index) + 2 * k + 1);
-    const int b[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    int at[8];
+    constexpr int kC = kCols<T>;
+    int at[kC];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) at[e] = kSmem ? spread(b[e]) : b[e];
+    for (int q = 0; q < kC / 4; ++q) {
+      const int4 v = __ldg(reinterpret_cast<const int4*>(a.index) + k * (kC / 4) + q);
+      at[4 * q] = v.x;
+      at[4 * q + 1] = v.y;
+      at[4 * q + 2] = v.z;
+      at[4 * q + 3] = v.w;
+    }
+    if constexpr (kSmem) {
+#pragma unroll
+      for (int e = 0; e < kC; ++e) at[e] = spread(at[e]);
+    }
     for (int h = 0; h < heads; ++h) {
-      uint32_t v[8];
+      uint32_t v[kC];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < kC; ++e) {
         if constexpr (kSmem) {
           v[e] = f[h * pitch + at[e]];
         } else {
@@ -429,15 +447,12 @@ kat_index_bias_fwd_kernel(const __grid_constant__ IndexFwd a) {
                                                     int64_t(at[e]) * a.heads + h0 + h)));
         }
       }
-      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
-                                            (int64_t(h0 + h) * a.chunks + k) * 8);
-      if constexpr (sizeof(T) == 4) {
-        out[0] = make_uint4(v[0], v[1], v[2], v[3]);
-        out[1] = make_uint4(v[4], v[5], v[6], v[7]);
-      } else {
-        out[0] = make_uint4(v[0] | (v[1] << 16), v[2] | (v[3] << 16), v[4] | (v[5] << 16),
-                            v[6] | (v[7] << 16));
-      }
+      uint4* out = reinterpret_cast<uint4*>(a.out) + int64_t(h0 + h) * a.chunks + k;
+      if constexpr (sizeof(T) == 4)
+        *out = make_uint4(v[0], v[1], v[2], v[3]);
+      else
+        *out = make_uint4(v[0] | (v[1] << 16), v[2] | (v[3] << 16), v[4] | (v[5] << 16),
+                          v[6] | (v[7] << 16));
     }
   }
 }
@@ -451,7 +466,8 @@ struct IndexBwd {
   const int32_t* slab_begin;
   const int32_t* seg_place;
   int64_t segments;
-  int32_t slab_rows;
+  int32_t slab_rows, slab_bytes;
+  int32_t heads, group;    // heads in all, and of a block
   float* part;             // [head][place of the segment]
 };
 
@@ -460,51 +476,67 @@ struct IndexBwd {
 // once, and the cells are read `skew` places further.  (Spreading pieces from registers over padded
 // rows instead cost four times the shared-memory wavefronts: dout[16,1025,1025] fp32 61 us.)
 // Otherwise cell by cell, into rows of the cells' pitch.
+// The list of the slab's cells goes to shared memory too, once for the block's heads.
 template <typename T, bool kFlat>
 __global__ void __launch_bounds__(kIdxBwdThreads)
 kat_index_bias_bwd_kernel(const __grid_constant__ IndexBwd a) {
   using U = typename Bits<T>::U;
   extern __shared__ uint4 slab_smem[];
-  const U* s = reinterpret_cast<const U*>(slab_smem);
-  const int64_t h = blockIdx.y;
+  uint4* list_smem = slab_smem + a.slab_bytes / 16;
   const int64_t i0 = int64_t(blockIdx.x) * a.slab_rows;
   const uint32_t rows = uint32_t(a.lq - i0 < a.slab_rows ? a.lq - i0 : a.slab_rows);
-  const U* base = static_cast<const U*>(a.dout) + h * a.sh + i0 * a.si;
   const uint32_t pitch = uint32_t(a.pitch), lk = uint32_t(a.lk);
-  if constexpr (kFlat) {
-    constexpr uint32_t kPer = 16 / sizeof(T);
-    const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T);
-    const uint32_t cells = (rows - 1) * pitch + lk;      // up to the last row's last cell
-    U* to = reinterpret_cast<U*>(slab_smem);
-    const uint32_t to0 = static_cast<uint32_t>(__cvta_generic_to_shared(slab_smem));
-    for (uint32_t k = threadIdx.x; k * kPer < cells + skew; k += kIdxBwdThreads) {
-      const int32_t first = int32_t(k * kPer) - int32_t(skew);   // the piece's first cell
-      if (first >= 0 && first + kPer <= cells) {
+  const int32_t seg_first = __ldg(a.slab_begin + blockIdx.x);
+  const int32_t seg_end = __ldg(a.slab_begin + blockIdx.x + 1);
+  const int32_t cell_first = __ldg(a.seg_begin + seg_first);
+  const uint16_t* list;
+  // `count` elements from `from` into `to`, as they lie: the place of the first one there
+  auto copy_run = [&](auto* to_raw, const auto* from, uint32_t count) {
+    constexpr uint32_t kPer = 16 / sizeof(*from);
+    const uint32_t skew = uint32_t(reinterpret_cast<uintptr_t>(from) & 15u) / sizeof(*from);
+    auto* to = to_raw;
+    const uint32_t to0 = static_cast<uint32_t>(__cvta_generic_to_shared(to_raw));
+    for (uint32_t k = threadIdx.x; k * kPer < count + skew; k += kIdxBwdThreads) {
+      const int32_t first = int32_t(k * kPer) - int32_t(skew);   // the piece's first element
+      if (first >= 0 && first + kPer <= count) {
         asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(to0 + k * 16u),
-                     "l"(base + first) : "memory");
+                     "l"(from + first) : "memory");
       } else {   // the run's ends
         for (uint32_t e = 0; e < kPer; ++e)
-          if (first + int32_t(e) >= 0 && first + e < cells) to[k * kPer + e] = __ldg(base + first + e);
+          if (first + int32_t(e) >= 0 && first + e < count)
+            to[k * kPer + e] = __ldg(from + first + e);
+      }
+    }
+    return to + skew;
+  };
+  list = copy_run(reinterpret_cast<uint16_t*>(list_smem), a.cells + cell_first,
+                  uint32_t(__ldg(a.seg_begin + seg_end) - cell_first));
+  const int h0 = blockIdx.y * a.group;
+  const int h1 = h0 + a.group < a.heads ? h0 + a.group : a.heads;
+  for (int64_t h = h0; h < h1; ++h) {
+    const U* base = static_cast<const U*>(a.dout) + h * a.sh + i0 * a.si;
+    const U* s = reinterpret_cast<const U*>(slab_smem);
+    if constexpr (kFlat) {
+      s = copy_run(reinterpret_cast<U*>(slab_smem), base, (rows - 1) * pitch + lk);
+    } else {
+      U* to = reinterpret_cast<U*>(slab_smem);
+      for (uint32_t k = threadIdx.x; k < rows * lk; k += kIdxBwdThreads) {
+        const uint32_t r = k / lk, j = k % lk;
+        to[r * pitch + j] = __ldg(base + int64_t(r) * a.si + int64_t(j) * a.sj);
       }
     }
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-    s += skew;
-  } else {
-    U* to = reinterpret_cast<U*>(slab_smem);
-    for (uint32_t k = threadIdx.x; k < rows * lk; k += kIdxBwdThreads) {
-      const uint32_t r = k / lk, j = k % lk;
-      to[r * pitch + j] = __ldg(base + int64_t(r) * a.si + int64_t(j) * a.sj);
-    }
-  }
-  __syncthreads();
-  const int32_t end = __ldg(a.slab_begin + blockIdx.x + 1);
-  for (int32_t g = __ldg(a.slab_begin + blockIdx.x) + int(threadIdx.x); g < end; g += kIdxBwdThreads) {
-    float sum = 0.0f;
-    const int32_t last = __ldg(a.seg_begin + g + 1);
+    __syncthreads();
+    for (int32_t g = seg_first + int(threadIdx.x); g < seg_end; g += kIdxBwdThreads) {
+      float sum = 0.0f;
+      const int32_t place = __ldg(a.seg_place + g);
+      const int32_t last = __ldg(a.seg_begin + g + 1) - cell_first;
 #pragma unroll 4
-    for (int32_t k = __ldg(a.seg_begin + g); k < last; ++k)
-      sum += Codec<T>::unpack1(s[__ldg(a.cells + k)]);
-    a.part[h * a.segments + __ldg(a.seg_place + g)] = sum;
+      for (int32_t k = __ldg(a.seg_begin + g) - cell_first; k < last; ++k)
+        sum += Codec<T>::unpack1(s[list[k]]);
+      a.part[h * a.segments + place] = sum;
+    }
+    __syncthreads();
   }
 }
 
@@ -637,16 +669,23 @@ int launch_index_fwd(IndexFwd a, cudaStream_t st) {
 }
 
 template <typename T, bool kFlat>
-int launch_index_bwd_v(const IndexBwd& a, dim3 grid, cudaStream_t st) {
-  const size_t bytes = size_t(a.slab_rows) * size_t(a.pitch) * sizeof(T) + 16;
+int launch_index_bwd_v(IndexBwd a, int64_t slabs, cudaStream_t st) {
+  const size_t cells = size_t(a.slab_rows) * size_t(a.pitch);
+  a.slab_bytes = int32_t((cells * sizeof(T) + 16 + 15) / 16 * 16);   // a run may start 15 bytes in
+  const size_t bytes = size_t(a.slab_bytes) + cells * 2 + 16;
+  // as many heads to a block as leave two blocks for every SM
+  a.group = 1;
+  while (a.group < a.heads && slabs * ((a.heads + 2 * a.group - 1) / (2 * a.group)) >= 2 * 148)
+    a.group *= 2;
   if (int rc = set_smem(kat_index_bias_bwd_kernel<T, kFlat>, bytes)) return rc;
+  const dim3 grid{uint32_t(slabs), uint32_t((a.heads + a.group - 1) / a.group)};
   kat_index_bias_bwd_kernel<T, kFlat><<<grid, kIdxBwdThreads, bytes, st>>>(a);
   return launched();
 }
 template <typename T>
-int launch_index_bwd(const IndexBwd& a, dim3 grid, cudaStream_t st) {
-  return a.sj == 1 && a.si == a.pitch ? launch_index_bwd_v<T, true>(a, grid, st)
-                                      : launch_index_bwd_v<T, false>(a, grid, st);
+int launch_index_bwd(const IndexBwd& a, int64_t slabs, cudaStream_t st) {
+  return a.sj == 1 && a.si == a.pitch ? launch_index_bwd_v<T, true>(a, slabs, st)
+                                      : launch_index_bwd_v<T, false>(a, slabs, st);
 }
 
 }  // namespace
@@ -674,7 +713,8 @@ int kat_distance_bias_fwd(const void* table, int32_t table_dtype, int32_t num_bu
   a.heads = heads;
   a.reach = reach;
   a.causal = causal != 0;
-  const int64_t chunks = a.ld / 8;
+  const int per = 16 / elem_size(out_dtype);   // columns of a thread
+  const int64_t chunks = a.ld / per;
   a.tx = 1;
   while (a.tx < kFwdThreads && a.tx < chunks) a.tx *= 2;
   a.ty = kFwdThreads / a.tx;
@@ -689,7 +729,7 @@ int kat_distance_bias_fwd(const void* table, int32_t table_dtype, int32_t num_bu
   if (n >= (int64_t(1) << 31) || col_blocks >= (int64_t(1) << 31)) return KAT_ERR_BAD_SHAPE;
   a.col_blocks = int32_t(col_blocks);
   const size_t smem =
-      (size_t(8 * a.tx + a.ty * a.rows - 1) * elem_size(out_dtype) + 3) / 4 * 4;
+      (size_t(per * a.tx + a.ty * a.rows - 1) * elem_size(out_dtype) + 3) / 4 * 4;
   const dim3 grid{uint32_t(n), uint32_t(heads)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (out_dtype) {
@@ -774,7 +814,7 @@ int kat_index_bias_fwd(const void* table, int32_t table_dtype, int32_t num_bucke
   a.table = table;
   a.index = index;
   a.out = out;
-  a.chunks = lq * (round8(lk) / 8);
+  a.chunks = lq * (round8(lk) / (16 / elem_size(out_dtype)));
   a.table_dtype = table_dtype;
   a.num_buckets = num_buckets;
   a.heads = heads;
@@ -834,13 +874,13 @@ int kat_index_bias_bwd(const void* dout, int32_t dout_dtype, const int64_t* dout
   a.seg_place = seg_place;
   a.segments = segments;
   a.slab_rows = slab_rows;
+  a.heads = heads;
   a.part = static_cast<float*>(workspace);
-  const dim3 grid{uint32_t(slabs), uint32_t(heads)};
   int rc = KAT_OK;
   switch (dout_dtype) {
-    case KAT_DTYPE_F32: rc = launch_index_bwd<float>(a, grid, st); break;
-    case KAT_DTYPE_F16: rc = launch_index_bwd<__half>(a, grid, st); break;
-    default: rc = launch_index_bwd<__nv_bfloat16>(a, grid, st); break;
+    case KAT_DTYPE_F32: rc = launch_index_bwd<float>(a, slabs, st); break;
+    case KAT_DTYPE_F16: rc = launch_index_bwd<__half>(a, slabs, st); break;
+    default: rc = launch_index_bwd<__nv_bfloat16>(a, slabs, st); break;
   }
   if (rc) return rc;
   const int64_t sums = int64_t(num_buckets) * heads;

@@ -16,7 +16,8 @@ implementation: CPU tables raise, and a missing library raises on first use.
 
 from __future__ import annotations
 
-import ctypes
+import functools
+import struct
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -34,6 +35,7 @@ MAX_BUCKETS = 1 << 24
 MAX_LENGTH = (1 << 31) - 64
 MAX_REACH = 1 << 24
 INT32_MIN, INT32_MAX = -(1 << 31), (1 << 31) - 1
+_PACK_STRIDE = struct.Struct("=3q")
 
 
 def _round8(n: int) -> int:
@@ -231,15 +233,15 @@ def _check_table(name: str, table: Tensor, num_buckets: int, dtype: torch.dtype)
                          f"{tuple(table.shape)}")
 
 
-def _stride(t: Tensor):
-    return (ctypes.c_int64 * 3)(*t.stride())
+def _stride(t: Tensor) -> bytes:
+    return _PACK_STRIDE.pack(*t.stride())
 
 
 def _output(heads: int, lq: int, lk: int, device: torch.device,
             dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
     """The padded rows and the view of them that is returned."""
     out = torch.empty((heads, lq, _round8(lk)), device=device, dtype=dtype)
-    return out, (out if lk % 8 == 0 else out[:, :, :lk])
+    return out, (out if lk % 8 == 0 else out.narrow(2, 0, lk))
 
 
 def _distance_forward(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int,
@@ -252,6 +254,11 @@ def _distance_forward(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int,
         buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), buckets.reach, lq, lk,
         offset, causal, out.data_ptr(), DTYPES[dtype]))
     return view
+
+
+@functools.lru_cache(maxsize=4096)
+def _distance_workspace(heads: int, lq: int, lk: int) -> int:
+    return _native.lib().kat_distance_bias_bwd_workspace_bytes(heads, lq, lk)
 
 
 class DistanceBiasFunction(torch.autograd.Function):
@@ -269,7 +276,7 @@ class DistanceBiasFunction(torch.autograd.Function):
         _, begin, end = buckets.on(device)
         nb = buckets.num_buckets
         d = torch.empty((nb, heads), device=device, dtype=dtype)
-        size = lib.kat_distance_bias_bwd_workspace_bytes(heads, lq, lk)
+        size = _distance_workspace(heads, lq, lk)
         ws = torch.empty(size, device=device, dtype=torch.uint8)
         _native.check("kat_distance_bias_bwd", _native.on_stream(
             device, lib.kat_distance_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
@@ -303,7 +310,7 @@ class IndexBiasFunction(torch.autograd.Function):
         lib, device = _native.lib(), grad.device
         _, cells, padded, seg_begin, slab_begin, seg_place, bucket_begin = b.on(device)
         d = torch.empty((b.num_buckets, heads), device=device, dtype=dtype)
-        size = lib.kat_index_bias_bwd_workspace_bytes(heads, b.segments)
+        size = 4 * heads * b.segments    # kat_index_bias_bwd_workspace_bytes
         ws = torch.empty(size, device=device, dtype=torch.uint8)
         _native.check("kat_index_bias_bwd", _native.on_stream(
             device, lib.kat_index_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
