@@ -324,14 +324,20 @@ __device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, 
 // Planes.
 // ---------------------------------------------------------------------------
 
-// hi + lo = v to 22 bits (v is already scaled).
-__device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(v - __half2float(hi));
-}
-__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
-  const __half2 h = __halves2half2(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// 8 scaled values in planes: hi + lo = v to 22 bits.  Two values to a conversion: one at a time they
+// took most of an epilogue.
+__device__ __forceinline__ void split8(const float* v, uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 a = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    const float2 f = __half22float2(a);
+    const __half2 b = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+    h[i] = *reinterpret_cast<const uint32_t*>(&a);
+    l[i] = *reinterpret_cast<const uint32_t*>(&b);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 // 8 values of both planes added up.
 __device__ __forceinline__ void join8(const uint4& h, const uint4& l, float (&v)[8]) {
@@ -519,16 +525,16 @@ kat_muon_split_kernel(const __grid_constant__ Update u, const double* __restrict
     const int ti = piece / 8, tj = piece % 8 * 8;
     const int64_t i = i0 + ti, j = j0 + tj;
     if (i >= height || j >= ld) continue;                // ld is a multiple of 8
-    __half h[8], l[8];
+    float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float f = transposed ? tile[tj + e][ti] : tile[ti][tj + e];
-      split(float(double(f) * scale), h[e], l[e]);       // the norm may lie outside fp32's range
+      v[e] = float(double(f) * scale);                   // the norm may lie outside fp32's range
     }
-    *reinterpret_cast<uint4*>(hi + i * ld + j) =
-        make_uint4(pack2(h[0], h[1]), pack2(h[2], h[3]), pack2(h[4], h[5]), pack2(h[6], h[7]));
-    *reinterpret_cast<uint4*>(lo + i * ld + j) =
-        make_uint4(pack2(l[0], l[1]), pack2(l[2], l[3]), pack2(l[4], l[5]), pack2(l[6], l[7]));
+    uint4 h, l;
+    split8(v, h, l);
+    *reinterpret_cast<uint4*>(hi + i * ld + j) = h;
+    *reinterpret_cast<uint4*>(lo + i * ld + j) = l;
   }
 }
 
@@ -721,7 +727,13 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       for (int k = 0; k < kPiece; ++k, p += args.out_ld)
         if (k < lines) *p = from_float<T>(o[k]);
     } else {
-      // the staging's previous store has read it
+      // the planes are ready before the staging's previous store is waited for (poly's: its own
+      // input goes through the staging first)
+      uint4 h[kPiece / 8], l[kPiece / 8];
+      if constexpr (kMode != kPoly) {
+#pragma unroll
+        for (int g = 0; g < kPiece / 8; ++g) split8(&y[g * 8], h[g], l[g]);
+      }
       if (lane == 0) bulk_wait_read();
       __syncwarp();
       if constexpr (kMode == kPoly) {
@@ -750,15 +762,9 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       }
 #pragma unroll
       for (int g = 0; g < kPiece / 8; ++g) {
-        __half hi[8], lo[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) split(y[g * 8 + k], hi[k], lo[k]);
-        *reinterpret_cast<uint4*>(stage_out + plane_offset(lane, g)) =
-            make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
-                       pack2(hi[6], hi[7]));
-        *reinterpret_cast<uint4*>(stage_out + kStagingBytes / 2 + plane_offset(lane, g)) =
-            make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
-                       pack2(lo[6], lo[7]));
+        if constexpr (kMode == kPoly) split8(&y[g * 8], h[g], l[g]);
+        *reinterpret_cast<uint4*>(stage_out + plane_offset(lane, g)) = h[g];
+        *reinterpret_cast<uint4*>(stage_out + kStagingBytes / 2 + plane_offset(lane, g)) = l[g];
       }
       fence_async_shared();
       __syncwarp();
@@ -1031,25 +1037,21 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
     for (int g = 0; g < kPiece / 8; ++g) {
       const int col = col_base + g * 8;
       const uint32_t at = chain_offset(row, col);
-      __half hi[8], lo[8];
-      float x[8];
+      float x[8], v[8];
       if (poly)
         join8(*reinterpret_cast<const uint4*>(s_a + at),
               two ? *reinterpret_cast<const uint4*>(s_a + kChainPlane + at)
                   : make_uint4(0u, 0u, 0u, 0u), x);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        float v = y[g * 8 + k] * mult;
+        v[k] = y[g * 8 + k] * mult;
         if (poly) {
-          v = fmaf(kB, x[k], kC * v);
-          if (row == col + k) v += kA * kScale;
+          v[k] = fmaf(kB, x[k], kC * v[k]);
+          if (row == col + k) v[k] += kA * kScale;
         }
-        split(v, hi[k], lo[k]);
       }
-      const uint4 h = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]),
-                                 pack2(hi[6], hi[7]));
-      const uint4 l = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]),
-                                 pack2(lo[6], lo[7]));
+      uint4 h, l;
+      split8(v, h, l);
       *reinterpret_cast<uint4*>(to + at) = h;
       *reinterpret_cast<uint4*>(to + kChainPlane + at) = l;
       if (also != nullptr) {
