@@ -54,8 +54,9 @@ template <typename T> __device__ __forceinline__ typename Bits<T>::U bits_of(flo
   return Codec<T>::pack1(v);
 }
 
-// 16 bytes of neighbouring values of a row.  One 16-byte store a thread and row, the lanes next to each
-// other (two stores to a thread, 32 bytes apart from lane to lane, took three times as long).
+// 16 bytes of neighbouring values of a row: one 16-byte store a thread and row, the lanes next to each
+// other (with two stores to a thread, 32 bytes apart from lane to lane, the forward of index[1025,1025],
+// 16 heads fp32 took 34 us instead of 24).
 template <typename T> constexpr int kCols = 16 / int(sizeof(T));
 
 // ---------------------------------------------------------------------------

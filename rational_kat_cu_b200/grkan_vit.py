@@ -163,7 +163,8 @@ class Block(nn.Module):
         if cfg.rope and not cfg.qk_norm:
             raise ValueError("ViTConfig: rope needs qk_norm (they are one pass)")
         if cfg.qk_norm:
-            table = rope_grid_table(side, side, head_dim, prefix=1) if cfg.rope else None
+            table = (rope_grid_table(side, side, head_dim, prefix=1, device="cpu")
+                     if cfg.rope else None)
             norm_rope = QKNormRope(head_dim, cfg.num_heads, table=table)
         if cfg.rel_pos_bias:
             pos_bias = GridPositionBias(cfg.num_heads, side, side, prefix=1)

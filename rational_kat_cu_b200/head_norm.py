@@ -403,13 +403,13 @@ class QKNormRope(nn.Module):
         self.register_buffer("sin", sin, persistent=False)
 
     def _apply(self, fn, recurse=True):
-        # the table stays fp32 where the module goes to another floating type
+        # the table moves, but keeps its values and stays fp32: where the module goes to another
+        # floating type, and where its storage is made anew (to_empty)
         tables = (self.cos, self.sin)
         super()._apply(fn, recurse)
         for name, t in zip(("cos", "sin"), tables):
-            now = getattr(self, name)
-            if t is not None and now.dtype != t.dtype:
-                setattr(self, name, t.to(now.device))
+            if t is not None and not t.is_meta:
+                setattr(self, name, t.to(getattr(self, name).device))
         return self
 
     def forward(self, qkv: Tensor,

@@ -8,12 +8,14 @@ matrix moves by about the same amount.  With X = u / |u|_F, `steps` times
 
 on the tcgen05 kernels of libkat_rational.so (include/kat_muon.h).  Matrices of one shape and
 type share their launches.  Operands are pairs of fp16 planes (22 bits) with fp32 accumulation: the
-result's relative error is about 1e-5, below any 16-bit rounding.  There is no CPU implementation: CPU tensors raise,
-and a missing library raises on first use.
+result's relative error is about 1e-5, below any 16-bit rounding (the last steps of 16-bit results
+take single planes where their own rounding hides it).  There is no CPU implementation: CPU tensors
+raise, and a missing library raises on first use.
 """
 
 from __future__ import annotations
 
+import bisect
 import ctypes
 import math
 from typing import Iterable, List, Sequence, Union
@@ -68,7 +70,9 @@ def _runs(count: int, rows: int, cols: int):
 @torch.no_grad()
 def orthogonalize(x: Tensor, steps: int = 5) -> Tensor:
     """The Newton-Schulz polar factor of each matrix of x [..., rows, cols], in x's type.  Zero
-    matrices stay zero; a matrix with a NaN or an infinity becomes NaN.  Not differentiable."""
+    matrices stay zero; a matrix with a NaN or an infinity becomes NaN.  Not differentiable.
+    The same call gives the same bits; a matrix alone and the same matrix among others may take
+    tiles of different sizes and then differ within the error above."""
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: expected [..., rows, cols], got {tuple(x.shape)}")
     _check_steps("orthogonalize", steps)
@@ -117,6 +121,13 @@ def _check_step_lists(weights, grads, momenta) -> None:
     for (a, size), (b, _) in zip(written, written[1:]):
         if a + size > b:
             raise ValueError("muon_step: two of the weights and momenta share memory")
+    for g in grads:
+        if g.numel():
+            a = g.data_ptr()
+            size = (1 + sum((n - 1) * s for n, s in zip(g.shape, g.stride()))) * g.element_size()
+            i = bisect.bisect_left(written, (a + size, 0))
+            if i and written[i - 1][0] + written[i - 1][1] > a:
+                raise ValueError("muon_step: a gradient shares memory with a weight or momentum")
 
 
 @torch.no_grad()
@@ -137,6 +148,8 @@ def muon_step(weights: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seque
     _check_steps("muon_step", steps)
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     _check_step_lists(weights, grads, momenta)
+    if not weights:
+        return
     lr_ptr, lr_value = None, 0.0
     if isinstance(lr, Tensor):
         if lr.is_cuda:
@@ -225,6 +238,10 @@ class Muon(torch.optim.Optimizer):
             params: List[Tensor] = [p for p in group["params"] if p.grad is not None]
             for p in params:
                 if "momentum_buffer" not in self.state[p]:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: the first step of a parameter cannot be captured "
+                                           "(every replay would begin its momentum anew): take one "
+                                           "step before")
                     self.state[p]["momentum_buffer"] = torch.zeros(
                         p.shape, device=p.device, dtype=torch.float32)
             muon_step(params, [p.grad for p in params],

@@ -32,6 +32,7 @@ DTYPES = {torch.float32: _native.KAT_DTYPE_F32, torch.float16: _native.KAT_DTYPE
 SLAB_CELLS = 16384    # KAT_BIAS_SLAB_CELLS
 SEGMENT = 32          # KAT_BIAS_SEGMENT
 MAX_BUCKETS = 1 << 24
+MAX_DISTANCE_BUCKETS = 1024   # their borders are exact, in integers of that many digits
 MAX_LENGTH = (1 << 31) - 64
 MAX_REACH = 1 << 24
 INT32_MIN, INT32_MAX = -(1 << 31), (1 << 31) - 1
@@ -40,6 +41,14 @@ _PACK_STRIDE = struct.Struct("=3q")
 
 def _round8(n: int) -> int:
     return (n + 7) // 8 * 8
+
+
+def _copied(tensors: Tuple[Tensor, ...], device: torch.device) -> Tuple[Tensor, ...]:
+    """Copies on `device` that any stream may use."""
+    copies = tuple(t.to(device) for t in tensors)
+    if device.type == "cuda":
+        torch.cuda.current_stream(device).synchronize()
+    return copies
 
 
 class DistanceBuckets:
@@ -53,8 +62,8 @@ class DistanceBuckets:
 
     def __init__(self, num_buckets: int = 32, max_distance: int = 128,
                  bidirectional: bool = True, device=None):
-        if num_buckets < 2 or num_buckets > MAX_BUCKETS:
-            raise ValueError(f"DistanceBuckets: num_buckets must be 2..{MAX_BUCKETS}, got "
+        if num_buckets < 2 or num_buckets > MAX_DISTANCE_BUCKETS:
+            raise ValueError(f"DistanceBuckets: num_buckets must be 2..{MAX_DISTANCE_BUCKETS}, got "
                              f"{num_buckets}")
         if bidirectional and (num_buckets % 2 or num_buckets < 4):
             raise ValueError(f"DistanceBuckets: two directions need an even number of buckets, "
@@ -69,8 +78,8 @@ class DistanceBuckets:
         # starts[b]: the least distance of bucket b of a side
         self.starts = list(range(half)) + self._borders(side, half, max_distance)
         reach = max(self.starts[-1], 1)
-        by_size = torch.bucketize(torch.arange(reach + 1), torch.tensor(self.starts),
-                                  right=True) - 1
+        by_size = torch.bucketize(torch.arange(reach + 1, device="cpu"),
+                                  torch.tensor(self.starts, device="cpu"), right=True) - 1
         behind = by_size.flip(0)[:-1]                   # d = -reach .. -1
         ahead = by_size + side if bidirectional else torch.zeros_like(by_size)
         self.reach = reach
@@ -99,10 +108,10 @@ class DistanceBuckets:
     def _runs(self) -> Tuple[Tensor, Tensor]:
         """First and last distance of each bucket (the outermost without an end; empty buckets
         end before they begin)."""
-        d = torch.arange(-self.reach, self.reach + 1)
+        d = torch.arange(-self.reach, self.reach + 1, device="cpu")
         of = self._of.long()
-        begin = torch.zeros(self.num_buckets, dtype=torch.int64)
-        end = torch.full((self.num_buckets,), -1, dtype=torch.int64)
+        begin = torch.zeros(self.num_buckets, dtype=torch.int64, device="cpu")
+        end = torch.full((self.num_buckets,), -1, dtype=torch.int64, device="cpu")
         first = torch.ones_like(of, dtype=torch.bool)
         first[1:] = of[1:] != of[:-1]
         last = torch.ones_like(first)
@@ -122,7 +131,7 @@ class DistanceBuckets:
         """(bucket_of, run_begin, run_end) on `device`, kept there (the first use on a device
         copies them: not inside a graph capture)."""
         if device not in self._on:
-            self._on[device] = tuple(t.to(device) for t in (self._of, self._begin, self._end))
+            self._on[device] = _copied((self._of, self._begin, self._end), device)
         return self._on[device]
 
     def __repr__(self) -> str:
@@ -188,13 +197,15 @@ class IndexBuckets:
             seg_place.to(torch.int32),
             torch.searchsorted(sorted_bucket,
                                torch.arange(num_buckets + 1, device=dev)).to(torch.int32))
+        if dev.type == "cuda":      # any stream may use them
+            torch.cuda.current_stream(dev).synchronize()
         self._on: Dict[torch.device, Tuple[Tensor, ...]] = {dev: self._tensors}
 
     def on(self, device: torch.device) -> Tuple[Tensor, ...]:
-        """(index, cells, padded_cells, seg_begin, slab_begin, seg_place, bucket_begin) on `device`, kept there
-        (the first use on a device copies them: not inside a graph capture)."""
+        """(index, cells, padded_cells, seg_begin, slab_begin, seg_place, bucket_begin) on `device`,
+        kept there (the first use on a device copies them: not inside a graph capture)."""
         if device not in self._on:
-            self._on[device] = tuple(t.to(device) for t in self._tensors)
+            self._on[device] = _copied(self._tensors, device)
         return self._on[device]
 
     def __repr__(self) -> str:
@@ -208,11 +219,11 @@ def grid_index(rows: int, cols: int, prefix: int = 0) -> Tuple[Tensor, int]:
     if rows < 1 or cols < 1 or prefix < 0:
         raise ValueError(f"grid_index: need rows, cols >= 1 and prefix >= 0, got {rows}, {cols} "
                          f"and {prefix}")
-    y = torch.arange(rows).repeat_interleave(cols)
-    x = torch.arange(cols).repeat(rows)
+    y = torch.arange(rows, device="cpu").repeat_interleave(cols)
+    x = torch.arange(cols, device="cpu").repeat(rows)
     pairs = (2 * rows - 1) * (2 * cols - 1)
     n = prefix + rows * cols
-    index = torch.empty(n, n, dtype=torch.int64)
+    index = torch.empty(n, n, dtype=torch.int64, device="cpu")
     index[prefix:, prefix:] = ((y[:, None] - y + rows - 1) * (2 * cols - 1)
                                + x[:, None] - x + cols - 1)
     index[:prefix, prefix:] = pairs

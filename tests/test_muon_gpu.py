@@ -197,7 +197,8 @@ def test_step_refusals_leave_everything(cuda_device):
     half = torch.zeros(8, 8, device="cuda", dtype=torch.float16)
     for ws, gs, ms in (([w, w], [g, g], [m, m.clone()]), ([w], [g], [w]), ([w], [half], [m]),
                        ([w], [g], [half]), ([w.t()[:, :7]], [g[:, :7]], [m[:, :7]]),
-                       ([w], [g[:4]], [m]), ([w], [g.to_sparse()], [m])):
+                       ([w], [g[:4]], [m]), ([w], [g.to_sparse()], [m]), ([w], [m], [m]),
+                       ([w], [w], [m])):
         with pytest.raises((ValueError, TypeError)):
             kat.muon_step(ws, gs, ms, lr=0.1)
     for lr in (torch.zeros(2, device="cuda"), torch.zeros(1, device="cuda").half()):
@@ -252,6 +253,38 @@ def test_optimizer_streams_and_graph(cuda_device):
         torch.cuda.synchronize()
         for p in (b, c, d):
             assert torch.equal(a, p)
+
+
+def test_first_step_is_not_captured(cuda_device):
+    """A captured first step would set the momentum to zero on every replay."""
+    p = torch.nn.Parameter(normal(16, 16))
+    p.grad = normal(16, 16, seed=1)
+    opt = kat.Muon([p], lr=0.1)
+    kat.muon_step([], [], [], lr=0.1)
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    before = p.detach().clone()
+    opt.step()
+    assert not torch.equal(p, before)
+
+
+def test_alone_and_in_a_batch(cuda_device):
+    """Together the matrices take the large tiles, alone the small ones.  A diagonal tile holds both
+    halves of a symmetric product, p_i q_j + p_i q_j' + p_i' q_j added in that order; beyond the
+    diagonal tiles the upper half is read from the lower, where the last two come in the other
+    order.  So the bits differ; each result is within its bound, and the two within their sum."""
+    for shape, dtype in (((12, 768, 768), torch.float32), ((9, 500, 1700), torch.bfloat16)):
+        x = normal(*shape, seed=3, dtype=dtype)
+        out = kat.orthogonalize(x)
+        for i in (0, shape[0] - 1):
+            want, allowed = reference(x[i], late=LATE[dtype])
+            alone = kat.orthogonalize(x[i])
+            assert_close(alone, want, allowed, dtype)
+            assert_close(out[i], want, allowed, dtype)
+            most = 2 * (allowed + HALF[dtype] * float(want.norm()))
+            assert float((alone.double() - out[i].double()).norm()) <= most
 
 
 def test_repeatable(cuda_device):

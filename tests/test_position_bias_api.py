@@ -45,7 +45,7 @@ def test_distance_buckets(args):
 
 def test_distance_buckets_refuse():
     for bad in ((1, 128, False), (2, 128, True), (5, 128, True), (32, 8, True), (32, 16, False),
-                (32, 1 << 25, True)):
+                (32, 1 << 25, True), (1026, 4096, True)):
         with pytest.raises(ValueError, match="DistanceBuckets"):
             kat.DistanceBuckets(*bad)
 

@@ -57,6 +57,9 @@ def test_entry_points_refuse():
         assert f(problem(), stream(heads=0, x=None, dy=None, out=None)) == E.KAT_OK
     assert fwd(problem(), stream(x=None)) == E.KAT_ERR_NULL_POINTER
     assert bwd(problem(), stream(dy=None)) == E.KAT_ERR_NULL_POINTER
+    assert bwd(problem(), stream(x=None, dweight=256)) == E.KAT_ERR_NULL_POINTER
+    for f in (fwd, bwd):
+        assert f(problem(tokens=1 << 32), stream(heads=0)) == E.KAT_OK
     assert fwd(problem(), stream(), count=0) == E.KAT_ERR_BAD_SHAPE
     assert fwd(problem(), *[stream()] * 4) == E.KAT_ERR_BAD_SHAPE
     assert lib.kat_qk_norm_rope_bwd_workspace_bytes(0, 1, 0) == 0

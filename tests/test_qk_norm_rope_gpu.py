@@ -232,6 +232,16 @@ def test_empty(cuda_device):
     assert outs[0].shape == q.shape
     grads = torch.autograd.grad(outs, (q, w), outs)
     assert grads[0].shape == q.shape and not grads[1].any()
+    # heads on one side only, and lengths that mean nothing without them
+    full, none = normal(2, 3, 4, 64).requires_grad_(), torch.empty(2, 3, 0, 64, device="cuda")
+    v = torch.full((64,), 2.0, device="cuda", requires_grad=True)
+    for q, k in ((full, none), (none, full)):
+        torch.empty(1 << 12, device="cuda").fill_(7.0)      # what a fresh tensor may find
+        out = kat.qk_norm_rope(q, k, w, v)
+        got = torch.autograd.grad(out, (full, w, v), out)
+        assert got[0].any() and bool(got[1].any()) != bool(got[2].any())
+    endless = torch.empty(1, 1 << 32, 0, 64, device="cuda")
+    assert kat.qk_norm_rope(endless, endless)[0].shape == endless.shape
 
 
 def test_differences(cuda_device):

@@ -64,3 +64,18 @@ def test_optimizers_share_the_parameters():
         p.grad = torch.ones_like(p)
     opt.zero_grad()
     assert all(p.grad is None for p in model.parameters())
+
+
+def test_tables_survive_a_start_on_the_meta_device():
+    cfg = tiny_cfg(qk_norm=True, rope=True, rel_pos_bias=True)
+    want = gv.GRKANViT(cfg, kat_device="cpu").blocks[1].attn
+    with torch.device("meta"):
+        model = gv.GRKANViT(cfg, kat_device="cpu")
+        buckets = kat.DistanceBuckets(8, 20)
+    attn = model.to_empty(device="cpu").blocks[1].attn
+    assert torch.equal(attn.norm_rope.cos, want.norm_rope.cos)
+    assert torch.equal(attn.norm_rope.sin, want.norm_rope.sin)
+    for a, b in zip(attn.pos_bias.buckets.on(torch.device("cpu")),
+                    want.pos_bias.buckets.on(torch.device("cpu"))):
+        assert torch.equal(a, b)
+    assert torch.equal(buckets._of, kat.DistanceBuckets(8, 20)._of)
