@@ -57,7 +57,7 @@ constexpr int kTK = 64;    // k-block: 64 fp16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
 constexpr uint32_t kPlaneBytes = kTM * kTK * 2;        // one operand plane of a stage
 constexpr uint32_t kRingBytes = 12 * kPlaneBytes;      // stages: 3 of P and Q in two planes, 6 in one
-constexpr int kMaxStages = 6;
+constexpr int kMaxStages = 8;                          // (half tiles: 4 and 8)
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kPiece = 32;         // rows and columns an epilogue warp handles at once
@@ -291,25 +291,27 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
 }
 // Instruction descriptor: fp32 accumulator (bits 4-5 = 1), fp16 operands (7-9, 10-12 = 0), the
 // operands' major-ness in bits 15 and 16 (1: MN-major), N >> 3 in 17-22, M >> 4 in 24-28; tiles are
-// 128 or (a CTA pair) 256 square.
-template <int kPair>
+// 128 rows by kCols columns or (a CTA pair) 256 square.
+template <int kPair, int kCols>
 __host__ __device__ constexpr uint32_t idesc_of(bool mn_p, bool mn_q) {
   return (1u << 4) | (mn_p ? (1u << 15) : 0u) | (mn_q ? (1u << 16) : 0u) |
-         (uint32_t((kTM * kPair) >> 3) << 17) | (uint32_t((kTM * kPair) >> 4) << 24);
+         (uint32_t((kCols * kPair) >> 3) << 17) | (uint32_t((kTM * kPair) >> 4) << 24);
 }
 
-// The MMAs of one k-block: operands at shared addresses p and q, their second planes `step` further,
-// accumulator d.  Which way the operands lie is a template parameter: with descriptors that
+template <auto V> struct Const { static constexpr auto value = V; };
+
+// The MMAs of one k-block: operands at shared addresses p and q, their second planes `step_p` and
+// `step_q` further, accumulator d.  Which way the operands lie is a template parameter: with descriptors that
 // depend on run-time values each MMA took 270 cycles to issue, four times its execution.
-template <int kPair, bool kMnP, bool kMnQ, int kPlanes>
-__device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, uint32_t step,
-                                            bool accumulate) {
+template <int kPair, int kCols, bool kMnP, bool kMnQ, int kPlanes>
+__device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, uint32_t step_p,
+                                            uint32_t step_q, bool accumulate) {
   const uint64_t p_hi = kMnP ? desc_mn(p) : desc_k(p), q_hi = kMnQ ? desc_mn(q) : desc_k(q);
-  const uint64_t p_lo = kMnP ? desc_mn(p + step) : desc_k(p + step);
-  const uint64_t q_lo = kMnQ ? desc_mn(q + step) : desc_k(q + step);
+  const uint64_t p_lo = kMnP ? desc_mn(p + step_p) : desc_k(p + step_p);
+  const uint64_t q_lo = kMnQ ? desc_mn(q + step_q) : desc_k(q + step_q);
   // a K = 16 slice further: 32 bytes inside the swizzled rows (K-major), two 8-k groups (MN-major)
   constexpr uint64_t kStepP = kMnP ? (2048 >> 4) : (32 >> 4), kStepQ = kMnQ ? (2048 >> 4) : (32 >> 4);
-  constexpr uint32_t idesc = idesc_of<kPair>(kMnP, kMnQ);
+  constexpr uint32_t idesc = idesc_of<kPair, kCols>(kMnP, kMnQ);
 #pragma unroll
   for (int k = 0; k < kTK / kUmmaK; ++k) {
     umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, accumulate || k != 0 ? 1u : 0u);
@@ -578,7 +580,8 @@ __device__ __forceinline__ uint32_t plane_offset(int row, int granule) {
   return uint32_t(row) * 64u + uint32_t((granule ^ ((row >> 1) & 3)) << 4);
 }
 
-template <int kMode, typename T, int kPair>
+// kCols: columns of the output that a CTA's rows of Q make, 128, or 64 (half tiles, single CTAs only).
+template <int kMode, typename T, int kPair, int kCols>
 __global__ void __launch_bounds__(kThreads, 1)
 kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
                      const __grid_constant__ CUtensorMap tm_q0,
@@ -591,7 +594,11 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   constexpr bool kSymP = kMode != kGram, kSymQ = kMode == kSym || kMode == kPoly;
   constexpr bool kColsQ = kMode == kApply || kMode == kFinal;   // Q is X, by its columns
   constexpr int kTile = kTM * kPair;                  // output tile, square
-  constexpr uint32_t kTmemCols = 2 * kTile;           // two accumulators
+  constexpr int kParts = kTM / kCols;                 // of its columns, each a tile of its own here
+  constexpr int kAccCols = kCols * kPair;
+  constexpr uint32_t kTmemCols = 2 * kAccCols;        // two accumulators
+  constexpr uint32_t kQBytes = kPlaneBytes / kParts;  // an operand plane of Q in a stage
+  static_assert(kParts == 1 || kPair == 1, "pairs take whole tiles");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -610,8 +617,8 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   const uint32_t rank = kPair == 2 ? cluster_rank() : 0u;
   const int slot0 = int(blockIdx.x) / kPair, slots = int(gridDim.x) / kPair;
 
-  const int planes = args.planes, stages = planes == 2 ? 3 : 6;
-  const uint32_t stage_bytes = uint32_t(planes) * 2 * kPlaneBytes;
+  const int planes = args.planes, stages = (kParts == 1 ? 6 : 8) / planes;
+  const uint32_t stage_bytes = uint32_t(planes) * (kPlaneBytes + kQBytes);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(full + s, 1);
@@ -636,8 +643,11 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait_previous();
 
-  // Tile -> set, matrix, row tile, column tile (row >= column where the product is symmetric).
-  auto locate = [&](int tile, int& set, int& mat, int& tr, int& tc) {
+  // Tile -> set, matrix, row tile, column tile (row >= column where the product is symmetric) and
+  // the first column in it.
+  auto locate = [&](int tile, int& set, int& mat, int& tr, int& tc, int& part) {
+    part = tile % kParts * kCols;
+    tile /= kParts;
     set = kMode == kSym && tile >= args.set_tiles ? 1 : 0;
     if (set) tile -= args.set_tiles;
     mat = tile / args.tiles;
@@ -777,7 +787,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       }
     }
   };
-  constexpr int kPieces = kTile / 2 / kPiece;   // of a warp's half of the columns
+  constexpr int kPieces = kAccCols / 2 / kPiece;   // of a warp's half of the columns
 
   if (warp == 0) {
     // ---------------- TMA producer: this CTA's 128 rows of P, its 128 rows or columns of Q ------
@@ -786,10 +796,10 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       uint32_t phase = 0;
       bool ok = true, wrapped = false;
       for (int tile = slot0; tile < args.total_tiles && ok; tile += slots) {
-        int tset, tmat, tr, tc;
-        locate(tile, tset, tmat, tr, tc);
+        int tset, tmat, tr, tc, part;
+        locate(tile, tset, tmat, tr, tc, part);
         const CUtensorMap* tm_q = tset ? &tm_q1 : &tm_q0;
-        const int p0 = tr * kTile + int(rank) * kTM, q0 = tc * kTile + int(rank) * kTM;
+        const int p0 = tr * kTile + int(rank) * kTM, q0 = tc * kTile + part + int(rank) * kTM;
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!wait_phase(empty + stage, phase ^ 1u, abort)) { ok = false; break; }
           uint8_t* s = smem + stage * stage_bytes;
@@ -808,8 +818,9 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
               const int p = p0 + b * 64, q = q0 + b * 64, k = kb * kTK;
               load(s + h * kPlaneBytes + b * kBoxBytes, &tm_p, mn_p ? p : k, mn_p ? k : p,
                    2 * tmat + h);
-              load(s + (planes + h) * kPlaneBytes + b * kBoxBytes, tm_q, mn_q ? q : k, mn_q ? k : q,
-                   2 * tmat + h);
+              if (b < kCols / 64)
+                load(s + planes * kPlaneBytes + h * kQBytes + b * kBoxBytes, tm_q, mn_q ? q : k,
+                     mn_q ? k : q, 2 * tmat + h);
             }
           }
           if (++stage == stages) { stage = 0; phase ^= 1u; wrapped = true; }
@@ -833,34 +844,31 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       };
       for (int tile = slot0; tile < args.total_tiles && ok; tile += slots, ++local) {
         const int acc = local & 1;
-        int tset, tmat, tr, tc;
-        locate(tile, tset, tmat, tr, tc);
+        int tset, tmat, tr, tc, part;
+        locate(tile, tset, tmat, tr, tc, part);
         if (!wait_phase(tempty + acc, ((local >> 1) & 1) ^ 1u, abort)) break;
         tc_fence_after();
-        const uint32_t d = tmem_base + uint32_t(acc * kTile);
+        const uint32_t d = tmem_base + uint32_t(acc * kAccCols);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
           if (!wait_phase(full + stage, phase, abort)) { ok = false; break; }
           tc_fence_after();
           const uint32_t s = smem_u32(smem + stage * stage_bytes);
           const bool mn_p = kSymP && kb * kTK / kTile > tr;
           const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
-          if (planes == 2) {
-            if (mn_p) {
-              if (mn_q) issue_block<kPair, true, true, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
-              else issue_block<kPair, true, false, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
-            } else {
-              if (mn_q) issue_block<kPair, false, true, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
-              else issue_block<kPair, false, false, 2>(d, s, s + 2 * kPlaneBytes, kPlaneBytes, kb != 0);
-            }
-          } else {
-            if (mn_p) {
-              if (mn_q) issue_block<kPair, true, true, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
-              else issue_block<kPair, true, false, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
-            } else {
-              if (mn_q) issue_block<kPair, false, true, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
-              else issue_block<kPair, false, false, 1>(d, s, s + kPlaneBytes, kPlaneBytes, kb != 0);
-            }
-          }
+          auto issue = [&](auto mn_p_, auto mn_q_, auto planes_) {
+            issue_block<kPair, kCols, mn_p_.value, mn_q_.value, planes_.value>(
+                d, s, s + planes_.value * kPlaneBytes, kPlaneBytes, kQBytes, kb != 0);
+          };
+          auto issue_q = [&](auto mn_p_, auto planes_) {
+            if (mn_q) issue(mn_p_, Const<true>{}, planes_);
+            else issue(mn_p_, Const<false>{}, planes_);
+          };
+          auto issue_p = [&](auto planes_) {
+            if (mn_p) issue_q(Const<true>{}, planes_);
+            else issue_q(Const<false>{}, planes_);
+          };
+          if (planes == 2) issue_p(Const<2>{});
+          else issue_p(Const<1>{});
           issued = true;
           commit_all(empty + stage);
           if (++stage == stages) { stage = 0; phase ^= 1u; }
@@ -883,11 +891,11 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     int local = 0;
     for (int tile = slot0; tile < args.total_tiles; tile += slots, ++local) {
       const int acc = local & 1;
-      int tr, tc;
-      locate(tile, set, mat, tr, tc);
+      int tr, tc, part;
+      locate(tile, set, mat, tr, tc, part);
       row0 = tr * kTile + int(rank) * kTM + quad * 32;
       row = row0 + lane;
-      const int col_base = tc * kTile + half * (kTile / 2);
+      const int col_base = tc * kTile + part + half * (kAccCols / 2);
       prefetch(col_base);
       int ok = 1;
       if (lane == 0) ok = wait_phase(tfull + acc, (local >> 1) & 1, abort) ? 1 : 0;
@@ -898,7 +906,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
 #pragma unroll 1
       for (int c = 0; c < kPieces; ++c) {
         float y[kPiece];
-        read_piece(lane_addr + uint32_t(acc * kTile + half * (kTile / 2) + c * kPiece), y);
+        read_piece(lane_addr + uint32_t(acc * kAccCols + half * (kAccCols / 2) + c * kPiece), y);
         if (c == kPieces - 1) {
           // this warp has read its part of the accumulator: hand it back to the MMA issuer
           tc_fence_before();
@@ -1015,13 +1023,15 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
       tc_fence_after();
       const uint32_t sp = smem_u32(p), sq = smem_u32(q);
       if (two) {
-        issue_block<1, false, false, 2>(tmem, sp, sq, kChainPlane, false);
+        issue_block<1, kTM, false, false, 2>(tmem, sp, sq, kChainPlane, kChainPlane, false);
         if (args.m > kTK)
-          issue_block<1, false, false, 2>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane, true);
+          issue_block<1, kTM, false, false, 2>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
+                                              kChainPlane, true);
       } else {
-        issue_block<1, false, false, 1>(tmem, sp, sq, kChainPlane, false);
+        issue_block<1, kTM, false, false, 1>(tmem, sp, sq, kChainPlane, kChainPlane, false);
         if (args.m > kTK)
-          issue_block<1, false, false, 1>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane, true);
+          issue_block<1, kTM, false, false, 1>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
+                                              kChainPlane, true);
       }
       umma_commit<1>(smem_u32(done));
     }
@@ -1235,10 +1245,10 @@ struct Maps {
   CUtensorMap p, q[2], out[2];
 };
 
-template <int kMode, typename T, int kPair>
-int launch_pair(const Maps& m, const GemmArgs& args, const PtrTable& outs, int slots,
+template <int kMode, typename T, int kPair, int kCols>
+int launch_tiles(const Maps& m, const GemmArgs& args, const PtrTable& outs, int slots,
                 cudaStream_t stream) {
-  auto kernel = kat_muon_gemm_kernel<kMode, T, kPair>;
+  auto kernel = kat_muon_gemm_kernel<kMode, T, kPair, kCols>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kSmemBytes)) != cudaSuccess)
     return KAT_ERR_CUDA;
@@ -1249,7 +1259,9 @@ int launch_pair(const Maps& m, const GemmArgs& args, const PtrTable& outs, int s
              : KAT_ERR_CUDA;
 }
 
-// CTA pairs on 256 x 256 tiles, or single CTAs on 128 x 128 tiles?
+// CTA pairs on 256 x 256 tiles, or single CTAs on 128 x 128 tiles?  Of those, halves of 64 columns where
+// even these are one wave: a k-block then takes half the MMAs and three quarters of the bytes (one
+// [768,768] bf16, 21 to 36 tiles a product: 187 -> 168 us; 3 x [197,1000], 9 to 24 tiles: 180 -> 153).
 template <int kMode, typename T>
 int launch_gemm(bool pair, const Maps& m, GemmArgs args, const PtrTable& outs, int sets, int count,
                 const Device& dev, cudaStream_t stream) {
@@ -1259,8 +1271,12 @@ int launch_gemm(bool pair, const Maps& m, GemmArgs args, const PtrTable& outs, i
   args.tiles = kMode != kApply && kMode != kFinal ? tm * (tm + 1) / 2 : tm * tn;
   args.set_tiles = args.tiles * count;
   args.total_tiles = args.set_tiles * sets;
-  return pair ? launch_pair<kMode, T, 2>(m, args, outs, dev.pairs, stream)
-              : launch_pair<kMode, T, 1>(m, args, outs, dev.sms, stream);
+  if (pair) return launch_tiles<kMode, T, 2, kTM>(m, args, outs, dev.pairs, stream);
+  if (2 * args.total_tiles <= dev.sms) {
+    args.total_tiles *= 2;
+    return launch_tiles<kMode, T, 1, kTM / 2>(m, args, outs, dev.sms, stream);
+  }
+  return launch_tiles<kMode, T, 1, kTM>(m, args, outs, dev.sms, stream);
 }
 
 template <typename T>
@@ -1404,7 +1420,7 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
 
 // CTA pairs that fit on the current device at once, 0 if none.
 int pair_count() {
-  auto kernel = kat_muon_gemm_kernel<kApply, float, 2>;
+  auto kernel = kat_muon_gemm_kernel<kApply, float, 2, kTM>;
   int n = 0;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kSmemBytes)) == cudaSuccess) {
