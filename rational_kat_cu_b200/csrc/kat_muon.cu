@@ -194,25 +194,38 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
                  : "memory");
   }
 }
-// D[tmem] (+)= P[smem] Q[smem]^T for one K = 16 slice, fp16 operands.
+// D[tmem] (+)= P[smem] Q[smem]^T for one K = 16 slice, fp16 operands.  The whole warp comes here with
+// the same operands, and its `leader` lane issues.
 template <int kPair>
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t p_desc, uint64_t q_desc,
-                                         uint32_t idesc, uint32_t accumulate) {
+                                         uint32_t idesc, uint32_t accumulate, uint32_t leader) {
   if constexpr (kPair == 1) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
   } else {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(p_desc), "l"(q_desc), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
   }
+}
+// One lane of a whole warp.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t mine;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(mine));
+  return mine;
 }
 // Arrive on the mbarrier at shared::cluster address `bar` when every MMA this thread issued so far
 // has completed.
@@ -302,10 +315,12 @@ template <auto V> struct Const { static constexpr auto value = V; };
 
 // The MMAs of one k-block: operands at shared addresses p and q, their second planes `step_p` and
 // `step_q` further, accumulator d.  Which way the operands lie is a template parameter: with descriptors that
-// depend on run-time values each MMA took 270 cycles to issue, four times its execution.
+// depend on run-time values each MMA took 270 cycles to issue, four times its execution.  And the whole
+// warp comes here: in a branch of one lane each took 83 cycles, now 65 at most (one [768,768] bf16: 168
+// -> 145 us).
 template <int kPair, int kCols, bool kMnP, bool kMnQ, int kPlanes>
 __device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, uint32_t step_p,
-                                            uint32_t step_q, bool accumulate) {
+                                            uint32_t step_q, bool accumulate, uint32_t leader) {
   const uint64_t p_hi = kMnP ? desc_mn(p) : desc_k(p), q_hi = kMnQ ? desc_mn(q) : desc_k(q);
   const uint64_t p_lo = kMnP ? desc_mn(p + step_p) : desc_k(p + step_p);
   const uint64_t q_lo = kMnQ ? desc_mn(q + step_q) : desc_k(q + step_q);
@@ -314,10 +329,11 @@ __device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, 
   constexpr uint32_t idesc = idesc_of<kPair, kCols>(kMnP, kMnQ);
 #pragma unroll
   for (int k = 0; k < kTK / kUmmaK; ++k) {
-    umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, accumulate || k != 0 ? 1u : 0u);
+    umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, accumulate || k != 0 ? 1u : 0u,
+                    leader);
     if constexpr (kPlanes == 2) {
-      umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u);
-      umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u);
+      umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u, leader);
+      umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u, leader);
     }
   }
 }
@@ -834,7 +850,12 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (rank 0 of a pair issues for both CTAs) ----------------
-    if (lane == 0 && rank == 0) {
+    // The whole warp walks the tiles, so that what the MMAs take lies in uniform registers.
+    if (rank == 0) {
+      const uint32_t leader = elect_lane();
+      auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait_phase(bar, parity, abort)) != 0;
+      };
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool issued = false, ok = true;
@@ -846,18 +867,19 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
         const int acc = local & 1;
         int tset, tmat, tr, tc, part;
         locate(tile, tset, tmat, tr, tc, part);
-        if (!wait_phase(tempty + acc, ((local >> 1) & 1) ^ 1u, abort)) break;
+        if (!wait_warp(tempty + acc, ((local >> 1) & 1) ^ 1u)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + uint32_t(acc * kAccCols);
         for (int kb = 0; kb < args.k_blocks; ++kb) {
-          if (!wait_phase(full + stage, phase, abort)) { ok = false; break; }
+          if (!wait_warp(full + stage, phase)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t s = smem_u32(smem + stage * stage_bytes);
-          const bool mn_p = kSymP && kb * kTK / kTile > tr;
-          const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
+          const uint32_t s = smem_u32(smem) + uint32_t(stage) * stage_bytes;
+          const bool mn_p = kSymP && __any_sync(0xffffffffu, kb * kTK / kTile > tr);
+          const bool mn_q = kColsQ || (kSymQ && __any_sync(0xffffffffu, kb * kTK / kTile > tc));
           auto issue = [&](auto mn_p_, auto mn_q_, auto planes_) {
             issue_block<kPair, kCols, mn_p_.value, mn_q_.value, planes_.value>(
-                d, s, s + planes_.value * kPlaneBytes, kPlaneBytes, kQBytes, kb != 0);
+                d, s, s + planes_.value * kPlaneBytes, kPlaneBytes, kQBytes, kb != 0,
+                leader);
           };
           auto issue_q = [&](auto mn_p_, auto planes_) {
             if (mn_q) issue(mn_p_, Const<true>{}, planes_);
@@ -870,12 +892,12 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
           if (planes == 2) issue_p(Const<2>{});
           else issue_p(Const<1>{});
           issued = true;
-          commit_all(empty + stage);
+          if (leader) commit_all(empty + stage);
           if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
-        if (ok) commit_all(tfull + acc);
+        if (ok && leader) commit_all(tfull + acc);
       }
-      if (issued) {
+      if (issued && leader) {
         // Every MMA has completed before the tensor memory is freed.
         umma_commit<kPair>(kPair == 1 ? smem_u32(drain) : cluster_addr(drain, 0));
         drain_phase(drain, 0);
@@ -1019,21 +1041,24 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
     fence_async_shared();   // the operands were written by this block's threads
     tc_fence_before();      // and the last result has been read
     __syncthreads();
-    if (threadIdx.x == 0 && *abort == 0) {
+    if (warp == 0 && __all_sync(0xffffffffu, *abort == 0)) {
+      const uint32_t leader = elect_lane();
       tc_fence_after();
       const uint32_t sp = smem_u32(p), sq = smem_u32(q);
       if (two) {
-        issue_block<1, kTM, false, false, 2>(tmem, sp, sq, kChainPlane, kChainPlane, false);
+        issue_block<1, kTM, false, false, 2>(tmem, sp, sq, kChainPlane, kChainPlane, false,
+                                        leader);
         if (args.m > kTK)
           issue_block<1, kTM, false, false, 2>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
-                                              kChainPlane, true);
+                                              kChainPlane, true, leader);
       } else {
-        issue_block<1, kTM, false, false, 1>(tmem, sp, sq, kChainPlane, kChainPlane, false);
+        issue_block<1, kTM, false, false, 1>(tmem, sp, sq, kChainPlane, kChainPlane, false,
+                                        leader);
         if (args.m > kTK)
           issue_block<1, kTM, false, false, 1>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
-                                              kChainPlane, true);
+                                              kChainPlane, true, leader);
       }
-      umma_commit<1>(smem_u32(done));
+      if (leader) umma_commit<1>(smem_u32(done));
     }
     ok = __syncthreads_and(wait_all(done, parity)) != 0;
     parity ^= 1u;
@@ -1262,6 +1287,7 @@ int launch_tiles(const Maps& m, const GemmArgs& args, const PtrTable& outs, int 
 // CTA pairs on 256 x 256 tiles, or single CTAs on 128 x 128 tiles?  Of those, halves of 64 columns where
 // even these are one wave: a k-block then takes half the MMAs and three quarters of the bytes (one
 // [768,768] bf16, 21 to 36 tiles a product: 187 -> 168 us; 3 x [197,1000], 9 to 24 tiles: 180 -> 153).
+// What bounds a product then is the planes' way into shared memory, 45 to 50 bytes a cycle of an SM.
 template <int kMode, typename T>
 int launch_gemm(bool pair, const Maps& m, GemmArgs args, const PtrTable& outs, int sets, int count,
                 const Device& dev, cudaStream_t stream) {
