@@ -23,8 +23,9 @@
  * Conventions as in kat_rational.h: the caller owns every buffer, nothing is allocated, work is
  * enqueued on `stream` of the current device, argument errors are reported before anything is
  * enqueued.  The matrices of one call have one shape and are contiguous, r, c in [1, 65536]; the
- * pointer arrays are host memory and are read before the call returns.  Results do not depend on
- * the other matrices of the call and are the same from run to run.
+ * pointer arrays are host memory and are read before the call returns.  Results are the same from
+ * run to run and do not depend on what the other matrices hold; how many there are chooses the
+ * tiles, and with them the order of some sums, within the error above.
  */
 #ifndef KAT_MUON_H_
 #define KAT_MUON_H_
