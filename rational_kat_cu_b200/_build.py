@@ -7,6 +7,8 @@ than the library.  `build(debug=True)` writes libkat_rational_debug.so from the 
 with -DKAT_DEBUG_BOUNDS=1: every global access, workspace slot and plan invariant of the
 activation kernels is checked, and a violation sets KAT_DEVICE_BOUNDS in the device status
 word instead of being made (the GPU-side stand-in for compute-sanitizer; tests only).
+With the library it compiles libkat_torch.so (csrc/kat_torch.cpp, no CUDA code): torch operators
+with C++ autograd nodes over some of the C entries.
 """
 
 from __future__ import annotations
@@ -32,7 +34,9 @@ HEADERS = [os.path.join(REPO_DIR, "include", "kat_rational.h"),
            os.path.join(REPO_DIR, "include", "kat_position_bias.h"),
            os.path.join(PKG_DIR, "csrc", "kat_math.cuh"),
            os.path.join(PKG_DIR, "csrc", "kat_plan.h")]
+TORCH_SOURCE = os.path.join(PKG_DIR, "csrc", "kat_torch.cpp")
 LIBRARY = os.path.join(PKG_DIR, "libkat_rational.so")
+TORCH_LIBRARY = os.path.join(PKG_DIR, "libkat_torch.so")
 DEBUG_LIBRARY = os.path.join(PKG_DIR, "libkat_rational_debug.so")
 
 NVCC_FLAGS = [
@@ -51,17 +55,51 @@ def find_nvcc() -> str:
     raise RuntimeError("nvcc not found: set NVCC or put the CUDA toolkit on PATH")
 
 
-def is_stale(target: str = LIBRARY) -> bool:
+def _older(target: str, sources) -> bool:
     if not os.path.exists(target):
         return True
     lib_t = os.path.getmtime(target)
-    return any(os.path.getmtime(p) > lib_t for p in (*SOURCES, *HEADERS, __file__))
+    return any(os.path.getmtime(p) > lib_t for p in sources)
+
+
+def is_stale(target: str = LIBRARY) -> bool:
+    """Whether `target` (with the library, the torch operators over it too) is to be compiled."""
+    if target == LIBRARY and _torch_stale():
+        return True
+    return _older(target, (*SOURCES, *HEADERS, __file__))
+
+
+def _torch_stale() -> bool:
+    return _older(TORCH_LIBRARY, (TORCH_SOURCE, *HEADERS, __file__))
+
+
+def build_torch(force: bool = False) -> str:
+    """Compile the torch operators if needed, against the installed torch; return their path."""
+    if not force and not _torch_stale():
+        return TORCH_LIBRARY
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", os.path.join(REPO_DIR, "include"), "-isystem", os.path.join(base, "include"),
+           "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), TORCH_SOURCE, "-o", TORCH_LIBRARY + ".tmp",
+           "-L", os.path.join(base, "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    os.replace(TORCH_LIBRARY + ".tmp", TORCH_LIBRARY)
+    return TORCH_LIBRARY
 
 
 def build(force: bool = False, verbose: bool = False, debug: bool = False) -> str:
     """Compile the library (or its bounds-checked debug build) if needed; return its path."""
     target = DEBUG_LIBRARY if debug else LIBRARY
-    if not force and not is_stale(target):
+    if not debug:
+        build_torch(force)
+    if not force and not _older(target, (*SOURCES, *HEADERS, __file__)):
         return target
     cmd = [find_nvcc(), *NVCC_FLAGS, "-I", os.path.join(REPO_DIR, "include"),
            *(["-DKAT_DEBUG_BOUNDS=1"] if debug else []), "-o", target + ".tmp", *SOURCES]

@@ -132,6 +132,7 @@ class KatError(RuntimeError):
 
 _lock = threading.Lock()
 _lib = None
+_ops: "_Ops | None" = None
 
 
 def library_path() -> str:
@@ -273,16 +274,44 @@ def check(func: str, status: int) -> None:
         raise KatError(func, status, strerror(status))
 
 
-def on_stream(device, call, *args) -> int:
-    """`call(*args, stream)` on the CUDA device `device`, with its current stream.  The raw queries
-    cost a tenth of torch.cuda.device and torch.cuda.current_stream, which small calls feel."""
-    import torch
+# The entries kat_torch.cpp calls, in the order of its `Entries`.
+_TORCH_ENTRIES = ("kat_rational_strerror", "kat_qk_norm_rope_fwd",
+                  "kat_qk_norm_rope_bwd_workspace_bytes", "kat_qk_norm_rope_bwd",
+                  "kat_distance_bias_fwd", "kat_distance_bias_bwd_workspace_bytes",
+                  "kat_distance_bias_bwd", "kat_index_bias_fwd",
+                  "kat_index_bias_bwd_workspace_bytes", "kat_index_bias_bwd")
 
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        return call(*args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+
+class _Ops:
+    """The torch operators of libkat_torch.so, over the entries of the loaded library."""
+
+    def __init__(self, handle: ctypes.CDLL):
+        import torch
+
+        path = _build.TORCH_LIBRARY
+        if not os.path.exists(path):
+            raise RuntimeError(f"libkat_torch.so not found at {path}; build it with "
+                               f"`python -m rational_kat_cu_b200._build`")
+        torch.ops.load_library(path)
+        table = (ctypes.c_void_p * len(_TORCH_ENTRIES))(
+            *[ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in _TORCH_ENTRIES])
+        ctypes.CDLL(path).kat_torch_bind(table)
+        ops = torch.ops.rational_kat_cu_b200
+        self.qk_norm_rope = ops.qk_norm_rope.default
+        self.qkv_norm_rope = ops.qkv_norm_rope.default
+        self.distance_bias = ops.distance_bias.default
+        self.index_bias = ops.index_bias.default
+
+
+def ops() -> _Ops:
+    """The torch operators (raises RuntimeError if a library has not been built)."""
+    global _ops
+    if _ops is None:
+        handle = lib()
+        with _lock:
+            if _ops is None:
+                _ops = _Ops(handle)
+    return _ops
 
 
 def device_status(device: int = 0, reset: bool = False) -> int:

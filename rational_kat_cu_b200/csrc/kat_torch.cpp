@@ -1,0 +1,478 @@
+// kat_torch.cpp — the q/k norm and the position biases as torch operators with their autograd nodes
+// (libkat_torch.so, loaded by _native.ops()).
+//
+// Everything is computed by libkat_rational.so through its C entries, whose addresses kat_torch_bind
+// takes.  What is here allocates outputs, fills the entries' arguments and is the node of the backward
+// pass.  It is C++ because these calls are short: a forward and backward pass of a 197-token grid bias
+// takes its kernels 9 us and the call 75, 94 with the same nodes in Python (q/k norm of small heads: 94
+// and 145; one token's, forward alone: 14 and 21).
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <optional>
+#include <tuple>
+#include <utility>
+#include <vector>
+
+#include "kat_position_bias.h"
+#include "kat_qk_norm_rope.h"
+#include "kat_rational.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+struct Entries {
+  decltype(&kat_rational_strerror) strerror;
+  decltype(&kat_qk_norm_rope_fwd) qk_fwd;
+  decltype(&kat_qk_norm_rope_bwd_workspace_bytes) qk_bwd_bytes;
+  decltype(&kat_qk_norm_rope_bwd) qk_bwd;
+  decltype(&kat_distance_bias_fwd) distance_fwd;
+  decltype(&kat_distance_bias_bwd_workspace_bytes) distance_bwd_bytes;
+  decltype(&kat_distance_bias_bwd) distance_bwd;
+  decltype(&kat_index_bias_fwd) index_fwd;
+  decltype(&kat_index_bias_bwd_workspace_bytes) index_bwd_bytes;
+  decltype(&kat_index_bias_bwd) index_bwd;
+};
+Entries entries{};
+
+void check(const char* name, int status) {
+  TORCH_CHECK(status == KAT_OK, name, " failed: ", entries.strerror(status), " (status ", status, ")");
+}
+
+int32_t code_of(at::ScalarType type) {
+  switch (type) {
+    case at::kFloat: return KAT_DTYPE_F32;
+    case at::kHalf: return KAT_DTYPE_F16;
+    case at::kBFloat16: return KAT_DTYPE_BF16;
+    default: TORCH_CHECK(false, "expected float32, float16 or bfloat16, got ", type);
+  }
+}
+at::ScalarType type_of(int64_t code) {
+  return code == KAT_DTYPE_F32 ? at::kFloat : code == KAT_DTYPE_F16 ? at::kHalf : at::kBFloat16;
+}
+
+// The current stream of a tensor's device, which is the current device meanwhile.
+struct On {
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit On(const Tensor& t)
+      : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+
+Tensor bytes_like(const Tensor& t, size_t bytes) {
+  return at::empty({int64_t(bytes)}, t.options().dtype(at::kByte));
+}
+
+bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// Gradients have no gradient: under create_graph they hang on a node that says so.
+struct Once : Function<Once> {
+  static Tensor forward(AutogradContext*, const Tensor& result, const Tensor&) {
+    return result.alias();
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "this operator's gradient cannot be differentiated again");
+  }
+};
+variable_list once(variable_list results, const variable_list& from) {
+  if (!at::GradMode::is_enabled()) return results;
+  for (const Tensor& anchor : from) {
+    if (!anchor.defined() || !anchor.requires_grad()) continue;
+    for (Tensor& r : results)
+      if (r.defined()) r = Once::apply(r, anchor);
+    break;
+  }
+  return results;
+}
+
+// ---------------------------------------------------------------------------
+// Norm of queries and keys with the rotation.
+// ---------------------------------------------------------------------------
+
+using Maybe = std::optional<Tensor>;
+
+struct Rope {   // undefined tensors: none
+  Tensor cos, sin, positions;
+  double eps;
+  bool interleaved;
+};
+
+const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+// The same values with a head's D values one after the other.
+Tensor heads_of(const Tensor& t) {
+  return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
+}
+
+kat_head_problem problem_of(int64_t batch, int64_t tokens, int64_t head_dim, at::ScalarType type,
+                            const Tensor& q_weight, const Tensor& k_weight, const Rope& rope) {
+  kat_head_problem p{};
+  p.batch = batch;
+  p.tokens = tokens;
+  p.head_dim = int32_t(head_dim);
+  p.dtype = code_of(type);
+  const Tensor& weight = q_weight.defined() ? q_weight : k_weight;
+  p.weight_dtype = weight.defined() ? code_of(weight.scalar_type()) : 0;
+  p.eps = float(rope.eps);
+  if (rope.cos.defined()) {
+    p.rot_dim = int32_t(2 * rope.cos.size(1));
+    p.interleaved = rope.interleaved;
+    p.cos_table = rope.cos.const_data_ptr<float>();
+    p.sin_table = rope.sin.const_data_ptr<float>();
+    p.table_rows = rope.cos.size(0);
+    if (rope.positions.defined()) {
+      p.positions = rope.positions.const_data_ptr<int64_t>();
+      p.position_stride[0] = rope.positions.stride(0);
+      p.position_stride[1] = rope.positions.stride(1);
+    }
+  }
+  return p;
+}
+
+struct Strides {
+  int64_t batch, token, head;
+};
+Strides strides_of(const Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
+void put(int64_t (&to)[3], const Strides& s) {
+  to[0] = s.batch;
+  to[1] = s.token;
+  to[2] = s.head;
+}
+// `offset` elements behind a tensor's first, where it has any.
+const void* behind(const Tensor& t, int64_t offset) {
+  const char* p = static_cast<const char*>(t.const_data_ptr());
+  return p == nullptr ? nullptr : p + offset * int64_t(t.element_size());
+}
+
+kat_head_stream stream_of(const void* x, const Strides& xs, const void* out, const Strides& os,
+                          const Tensor& weight, int64_t heads) {
+  kat_head_stream s{};
+  s.x = x;
+  put(s.x_stride, xs);
+  s.out = const_cast<void*>(out);
+  put(s.out_stride, os);
+  s.weight = pointer(weight);
+  s.heads = int32_t(heads);
+  return s;
+}
+void put_grad(kat_head_stream& s, const Tensor& dy, const Tensor& dweight) {
+  s.dy = dy.const_data_ptr();
+  put(s.dy_stride, strides_of(dy));
+  s.dweight = dweight.defined() ? dweight.mutable_data_ptr<float>() : nullptr;
+}
+
+Tensor dweight_of(const Tensor& weight) {
+  return weight.defined() && weight.requires_grad()
+             ? at::empty(weight.sizes(), weight.options().dtype(at::kFloat).requires_grad(false))
+             : Tensor();
+}
+Tensor as(const Tensor& grad, const Tensor& like) {
+  return grad.defined() ? grad.to(like.scalar_type()) : grad;
+}
+
+void run_backward(const kat_head_problem& p, const kat_head_stream* streams, int count,
+                  const Tensor& like) {
+  const On on(like);
+  const size_t bytes = entries.qk_bwd_bytes(p.head_dim, count, like.device().index());
+  TORCH_CHECK(bytes > 0, "kat_qk_norm_rope_bwd_workspace_bytes returned 0");
+  const Tensor ws = bytes_like(like, bytes);
+  check("kat_qk_norm_rope_bwd",
+        entries.qk_bwd(&p, streams, count, ws.mutable_data_ptr(), bytes, on.stream));
+}
+
+variable_list saved_of(const Tensor& a, const Tensor& b, const Tensor& q_weight,
+                       const Tensor& k_weight, const Rope& rope) {
+  return {a, b, q_weight, k_weight, rope.cos, rope.sin, rope.positions};
+}
+Rope rope_of(AutogradContext* ctx, const variable_list& saved) {
+  return {saved[4], saved[5], saved[6], ctx->saved_data["eps"].toDouble(),
+          ctx->saved_data["interleaved"].toBool()};
+}
+void keep_rope(AutogradContext* ctx, const Rope& rope) {
+  ctx->saved_data["eps"] = rope.eps;
+  ctx->saved_data["interleaved"] = rope.interleaved;
+}
+
+variable_list qk_forward(const Tensor& q, const Tensor& k, const Tensor& q_weight,
+                         const Tensor& k_weight, const Rope& rope) {
+  const On on(q);
+  const Tensor out_q = at::empty(q.sizes(), q.options().requires_grad(false));
+  const Tensor out_k = at::empty(k.sizes(), k.options().requires_grad(false));
+  const auto p = problem_of(q.size(0), q.size(1), q.size(3), q.scalar_type(), q_weight, k_weight, rope);
+  const kat_head_stream s[2] = {
+      stream_of(q.const_data_ptr(), strides_of(q), out_q.const_data_ptr(), strides_of(out_q), q_weight,
+                q.size(2)),
+      stream_of(k.const_data_ptr(), strides_of(k), out_k.const_data_ptr(), strides_of(out_k), k_weight,
+                k.size(2))};
+  check("kat_qk_norm_rope_fwd", entries.qk_fwd(&p, s, 2, on.stream));
+  return {out_q, out_k};
+}
+
+struct QkNormRope : Function<QkNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in,
+                               const Maybe& q_maybe, const Maybe& k_maybe, const Rope& rope) {
+    const Tensor q = heads_of(q_in), k = heads_of(k_in);
+    const Tensor q_weight = q_maybe.value_or(Tensor()), k_weight = k_maybe.value_or(Tensor());
+    ctx->save_for_backward(saved_of(q, k, q_weight, k_weight, rope));
+    keep_rope(ctx, rope);
+    return qk_forward(q, k, q_weight, k_weight, rope);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &q_weight = saved[2], &k_weight = saved[3];
+    const Rope rope = rope_of(ctx, saved);
+    const Tensor gq = heads_of(grads[0]), gk = heads_of(grads[1]);
+    const Tensor dq = at::empty(q.sizes(), q.options().requires_grad(false));
+    const Tensor dk = at::empty(k.sizes(), k.options().requires_grad(false));
+    const Tensor dwq = dweight_of(q_weight), dwk = dweight_of(k_weight);
+    const auto p =
+        problem_of(q.size(0), q.size(1), q.size(3), q.scalar_type(), q_weight, k_weight, rope);
+    kat_head_stream s[2] = {
+        stream_of(q.const_data_ptr(), strides_of(q), dq.const_data_ptr(), strides_of(dq), q_weight,
+                  q.size(2)),
+        stream_of(k.const_data_ptr(), strides_of(k), dk.const_data_ptr(), strides_of(dk), k_weight,
+                  k.size(2))};
+    put_grad(s[0], gq, dwq);
+    put_grad(s[1], gk, dwk);
+    run_backward(p, s, 2, q);
+    return once({dq, dk, as(dwq, q_weight), as(dwk, k_weight), Tensor()},
+                {grads[0], grads[1], q, k, q_weight, k_weight});
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
+                                        const Maybe& q_weight,
+                                        const Maybe& k_weight,
+                                        const Maybe& cos,
+                                        const Maybe& sin,
+                                        const Maybe& positions, double eps,
+                                        bool interleaved) {
+  const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
+  const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
+  const variable_list out = wants_grad({&q, &k, &wq, &wk})
+                                ? QkNormRope::apply(q, k, q_weight, k_weight, rope)
+                                : qk_forward(heads_of(q), heads_of(k), wq, wk, rope);
+  return {out[0], out[1]};
+}
+
+Tensor packed_of(const Tensor& qkv) {
+  return qkv.stride(2) == 1 || qkv.size(2) == 1 ? qkv : qkv.contiguous();
+}
+
+// q', k' and v, a view of x.
+variable_list qkv_forward(const Tensor& x, int64_t hq, int64_t hk, const Tensor& q_weight,
+                          const Tensor& k_weight, const Rope& rope) {
+  const On on(x);
+  const int64_t B = x.size(0), L = x.size(1), D = x.size(2) / (hq + 2 * hk);
+  const auto options = x.options().requires_grad(false);
+  const Tensor out_q = at::empty({B, L, hq, D}, options), out_k = at::empty({B, L, hk, D}, options);
+  const Strides xs{x.stride(0), x.stride(1), D};
+  const auto p = problem_of(B, L, D, x.scalar_type(), q_weight, k_weight, rope);
+  const kat_head_stream s[2] = {
+      stream_of(behind(x, 0), xs, out_q.const_data_ptr(), strides_of(out_q), q_weight, hq),
+      stream_of(behind(x, hq * D), xs, out_k.const_data_ptr(), strides_of(out_k), k_weight, hk)};
+  check("kat_qk_norm_rope_fwd", entries.qk_fwd(&p, s, 2, on.stream));
+  return {out_q, out_k,
+          x.as_strided({B, L, hk, D}, {x.stride(0), x.stride(1), D, 1},
+                       x.storage_offset() + (hq + hk) * D)};
+}
+
+struct QkvNormRope : Function<QkvNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& qkv, const Maybe& q_maybe,
+                               const Maybe& k_maybe, int64_t hq, int64_t hk, const Rope& rope) {
+    const Tensor x = packed_of(qkv);
+    const Tensor q_weight = q_maybe.value_or(Tensor()), k_weight = k_maybe.value_or(Tensor());
+    ctx->save_for_backward(saved_of(x, Tensor(), q_weight, k_weight, rope));
+    keep_rope(ctx, rope);
+    ctx->saved_data["hq"] = hq;
+    ctx->saved_data["hk"] = hk;
+    return qkv_forward(x, hq, hk, q_weight, k_weight, rope);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &q_weight = saved[2], &k_weight = saved[3];
+    const Rope rope = rope_of(ctx, saved);
+    const int64_t hq = ctx->saved_data["hq"].toInt(), hk = ctx->saved_data["hk"].toInt();
+    const Tensor gq = heads_of(grads[0]), gk = heads_of(grads[1]), gv = heads_of(grads[2]);
+    const int64_t width = x.size(2), L = x.size(1), D = width / (hq + 2 * hk);
+    const Tensor dx = at::empty(x.sizes(), x.options().requires_grad(false));
+    const Tensor dwq = dweight_of(q_weight), dwk = dweight_of(k_weight);
+    const Strides xs{x.stride(0), x.stride(1), D}, os{L * width, width, D};
+    const auto p = problem_of(x.size(0), L, D, x.scalar_type(), q_weight, k_weight, rope);
+    kat_head_stream s[3] = {
+        stream_of(behind(x, 0), xs, behind(dx, 0), os, q_weight, hq),
+        stream_of(behind(x, hq * D), xs, behind(dx, hq * D), os, k_weight, hk),
+        stream_of(nullptr, {0, 0, 0}, behind(dx, (hq + hk) * D), os, Tensor(), hk)};
+    put_grad(s[0], gq, dwq);
+    put_grad(s[1], gk, dwk);
+    put_grad(s[2], gv, Tensor());
+    run_backward(p, s, 3, x);
+    return once({dx, as(dwq, q_weight), as(dwk, k_weight), Tensor(), Tensor(), Tensor()},
+                {grads[0], grads[1], grads[2], x, q_weight, k_weight});
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, int64_t q_heads, int64_t k_heads,
+                                                 const Maybe& q_weight,
+                                                 const Maybe& k_weight,
+                                                 const Maybe& cos,
+                                                 const Maybe& sin,
+                                                 const Maybe& positions, double eps,
+                                                 bool interleaved) {
+  const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
+  const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
+  const variable_list out = wants_grad({&qkv, &wq, &wk})
+                                ? QkvNormRope::apply(qkv, q_weight, k_weight, q_heads, k_heads, rope)
+                                : qkv_forward(packed_of(qkv), q_heads, k_heads, wq, wk, rope);
+  return {out[0], out[1], out[2]};
+}
+
+// ---------------------------------------------------------------------------
+// Position biases.
+// ---------------------------------------------------------------------------
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Rows padded to multiples of 8, and the view of their lk columns.
+std::pair<Tensor, Tensor> rows_of(const Tensor& table, int64_t lq, int64_t lk, int64_t type) {
+  const Tensor out = at::empty({table.size(1), lq, round8(lk)},
+                               table.options().dtype(type_of(type)).requires_grad(false));
+  return {out, lk % 8 == 0 ? out : out.narrow(2, 0, lk)};
+}
+Tensor dtable_of(const Tensor& grad, int64_t buckets, at::ScalarType type) {
+  return at::empty({buckets, grad.size(0)}, grad.options().dtype(type).requires_grad(false));
+}
+
+struct Distance {
+  Tensor bucket_of, run_begin, run_end;
+  int64_t buckets, reach, lq, lk, offset, causal, type;
+};
+
+Tensor distance_forward(const Tensor& table_in, const Distance& a) {
+  const On on(table_in);
+  const Tensor table = table_in.contiguous();
+  const auto out = rows_of(table, a.lq, a.lk, a.type);
+  check("kat_distance_bias_fwd",
+        entries.distance_fwd(table.const_data_ptr(), code_of(table.scalar_type()), int32_t(a.buckets),
+                             int32_t(table.size(1)), a.bucket_of.const_data_ptr<int32_t>(),
+                             int32_t(a.reach), a.lq, a.lk, a.offset, int32_t(a.causal),
+                             out.first.mutable_data_ptr(), int32_t(a.type), on.stream));
+  return out.second;
+}
+
+struct DistanceBias : Function<DistanceBias> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Distance& a) {
+    ctx->saved_data["runs"] = std::vector<Tensor>{a.run_begin, a.run_end};
+    ctx->saved_data["sizes"] = std::vector<int64_t>{a.buckets, a.lq, a.lk, a.offset, a.causal,
+                                                    int64_t(table.scalar_type())};
+    return distance_forward(table, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor& grad = grads[0];
+    const auto runs = ctx->saved_data["runs"].toTensorVector();
+    const auto n = ctx->saved_data["sizes"].toIntVector();
+    const On on(grad);
+    const int32_t heads = int32_t(grad.size(0));
+    const auto type = at::ScalarType(n[5]);
+    const Tensor d = dtable_of(grad, n[0], type);
+    const size_t bytes = entries.distance_bwd_bytes(heads, n[1], n[2]);
+    const Tensor ws = bytes_like(grad, bytes);
+    check("kat_distance_bias_bwd",
+          entries.distance_bwd(grad.const_data_ptr(), code_of(grad.scalar_type()),
+                               grad.strides().data(), int32_t(n[0]), heads,
+                               runs[0].const_data_ptr<int32_t>(), runs[1].const_data_ptr<int32_t>(),
+                               n[1], n[2], n[3], int32_t(n[4]), d.mutable_data_ptr(), code_of(type),
+                               ws.mutable_data_ptr(), bytes, on.stream));
+    return once({d, Tensor()}, {grad});
+  }
+};
+
+Tensor distance_bias(const Tensor& table, at::TensorList plan, int64_t buckets, int64_t reach,
+                     int64_t lq, int64_t lk, int64_t offset, bool causal, int64_t type) {
+  TORCH_CHECK(plan.size() == 3, "distance_bias: a plan has 3 tensors");
+  const Distance a{plan[0], plan[1], plan[2], buckets, reach, lq, lk, offset, causal, type};
+  return wants_grad({&table}) ? DistanceBias::apply(table, a) : distance_forward(table, a);
+}
+
+struct Index {
+  at::TensorList plan;   // index, cells, padded_cells, seg_begin, slab_begin, seg_place, bucket_begin
+  int64_t buckets, lq, lk, slab_rows, slabs, segments, type;
+};
+
+Tensor index_forward(const Tensor& table_in, const Index& a) {
+  const On on(table_in);
+  const Tensor table = table_in.contiguous();
+  const auto out = rows_of(table, a.lq, a.lk, a.type);
+  check("kat_index_bias_fwd",
+        entries.index_fwd(table.const_data_ptr(), code_of(table.scalar_type()), int32_t(a.buckets),
+                          int32_t(table.size(1)), a.plan[0].const_data_ptr<int32_t>(), a.lq, a.lk,
+                          out.first.mutable_data_ptr(), int32_t(a.type), on.stream));
+  return out.second;
+}
+
+struct IndexBias : Function<IndexBias> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Index& a) {
+    ctx->saved_data["plan"] = a.plan.vec();
+    ctx->saved_data["sizes"] = std::vector<int64_t>{a.buckets, a.lq, a.lk, a.slab_rows, a.slabs,
+                                                    a.segments, int64_t(table.scalar_type())};
+    return index_forward(table, a);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor& grad = grads[0];
+    const auto plan = ctx->saved_data["plan"].toTensorVector();
+    const auto n = ctx->saved_data["sizes"].toIntVector();
+    const On on(grad);
+    const int32_t heads = int32_t(grad.size(0));
+    const auto type = at::ScalarType(n[6]);
+    const Tensor d = dtable_of(grad, n[0], type);
+    const size_t bytes = entries.index_bwd_bytes(heads, n[5]);
+    const Tensor ws = bytes_like(grad, bytes);
+    auto ints = [&](int i) { return plan[i].const_data_ptr<int32_t>(); };
+    auto cells = [&](int i) { return static_cast<const uint16_t*>(plan[i].const_data_ptr()); };
+    check("kat_index_bias_bwd",
+          entries.index_bwd(grad.const_data_ptr(), code_of(grad.scalar_type()), grad.strides().data(),
+                            int32_t(n[0]), heads, n[1], n[2], cells(1), cells(2), ints(3), n[5], ints(4),
+                            n[4], int32_t(n[3]), ints(5), ints(6), d.mutable_data_ptr(), code_of(type),
+                            ws.mutable_data_ptr(), bytes, on.stream));
+    return once({d, Tensor()}, {grad});
+  }
+};
+
+Tensor index_bias(const Tensor& table, at::TensorList plan, int64_t buckets, int64_t lq, int64_t lk,
+                  int64_t slab_rows, int64_t slabs, int64_t segments, int64_t type) {
+  TORCH_CHECK(plan.size() == 7, "index_bias: a plan has 7 tensors");
+  const Index a{plan, buckets, lq, lk, slab_rows, slabs, segments, type};
+  return wants_grad({&table}) ? IndexBias::apply(table, a) : index_forward(table, a);
+}
+
+}  // namespace
+
+// The addresses of libkat_rational.so's entries, in the order of `Entries`.
+extern "C" __attribute__((visibility("default"))) void kat_torch_bind(const Entries* from) {
+  entries = *from;
+}
+
+TORCH_LIBRARY(rational_kat_cu_b200, m) {
+  m.def("qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? cos, Tensor? sin, "
+        "Tensor? positions, float eps, bool interleaved) -> (Tensor, Tensor)", &qk_norm_rope);
+  m.def("qkv_norm_rope(Tensor(a) qkv, int q_heads, int k_heads, Tensor? q_weight, Tensor? k_weight, "
+        "Tensor? cos, Tensor? sin, Tensor? positions, float eps, bool interleaved) -> "
+        "(Tensor, Tensor, Tensor(a))", &qkv_norm_rope);
+  m.def("distance_bias(Tensor table, Tensor[] plan, int buckets, int reach, int lq, int lk, int offset, "
+        "bool causal, int type) -> Tensor", &distance_bias);
+  m.def("index_bias(Tensor table, Tensor[] plan, int buckets, int lq, int lk, int slab_rows, int slabs, "
+        "int segments, int type) -> Tensor", &index_bias);
+}

@@ -4,28 +4,25 @@ Every head's vector x [D] of a token becomes n = x w / sqrt(mean(x^2) + eps), an
 its first `rot_dim` values are turned by their angles:
 (y_a, y_b) = (n_a cos - n_b sin, n_a sin + n_b cos).  Pairs are (i, i + rot_dim / 2), or
 (2i, 2i + 1) with `interleaved`.  Forward and backward run on the sm_100a kernels of
-libkat_rational.so (include/kat_qk_norm_rope.h): a head is read once and written once, and queries
-and keys share a launch.  Arithmetic is fp32; outputs are rounded once.
+libkat_rational.so (include/kat_qk_norm_rope.h), called by the torch operators of libkat_torch.so
+(csrc/kat_torch.cpp): a head is read once and written once, and queries and keys share a launch.  Arithmetic is fp32; outputs are rounded once.
 
   qk_norm_rope    queries [B, L, Hq, D] and keys [B, L, Hk, D], any strides
   qkv_norm_rope   one projection's output [B, L, (Hq + 2 Hk) D]; its gradient is written whole,
                   the values' part included, by the same kernel
   rope_table, rope_grid_table   cos and sin of the angles, computed in 64 bits
 
-There is no CPU implementation: CPU tensors raise, and a missing library raises on first use.
+A gradient cannot be differentiated again (it raises).  There is no CPU implementation: CPU tensors
+raise, and a missing library raises on first use.
 """
 
 from __future__ import annotations
 
-import ctypes
-import functools
-import struct
 from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -64,215 +61,6 @@ def rope_grid_table(rows: int, cols: int, rot_dim: int, prefix: int = 0, base: f
     tables = [_turns(torch.cat([place, p]), rot_dim // 4, base) for p in (y, x)]
     return (torch.cat([tables[0][0], tables[1][0]], 1),
             torch.cat([tables[0][1], tables[1][1]], 1))
-
-
-class _Stream(ctypes.Structure):
-    """Mirror of `kat_head_stream`."""
-
-    _fields_ = [("x", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("out", ctypes.c_void_p),
-                ("weight", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
-                ("x_stride", ctypes.c_int64 * 3), ("dy_stride", ctypes.c_int64 * 3),
-                ("out_stride", ctypes.c_int64 * 3), ("heads", ctypes.c_int32)]
-
-
-class _Problem(ctypes.Structure):
-    """Mirror of `kat_head_problem`."""
-
-    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64),
-                ("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
-                ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32),
-                ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
-                ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
-                ("table_rows", ctypes.c_int64), ("positions", ctypes.c_void_p),
-                ("position_stride", ctypes.c_int64 * 2)]
-
-
-# The same as `_Stream` and `_Problem`, packed at once: filling ctypes fields one by one costs several
-# microseconds a call, as much as a small launch.
-_PACK_STREAM = struct.Struct("=5Q9qi4x")
-_PACK_PROBLEM = struct.Struct("=2q5if2QqQ2q")
-assert _PACK_STREAM.size == ctypes.sizeof(_Stream)
-assert _PACK_PROBLEM.size == ctypes.sizeof(_Problem)
-_NO_STRIDE = (0, 0, 0)
-
-
-def _pack(x: int, dy: int, out: int, weight: Optional[Tensor], dweight: Optional[Tensor], xs, ds,
-          os, heads: int) -> bytes:
-    """A stream from addresses (0: none) and strides."""
-    return _PACK_STREAM.pack(x, dy, out, 0 if weight is None else weight.data_ptr(),
-                             0 if dweight is None else dweight.data_ptr(), *xs, *ds, *os, heads)
-
-
-def _pack_problem(batch: int, tokens: int, head_dim: int, dtype: torch.dtype,
-                  q_weight: Optional[Tensor], k_weight: Optional[Tensor], cos: Optional[Tensor],
-                  sin: Optional[Tensor], positions: Optional[Tensor], eps: float,
-                  interleaved: bool) -> bytes:
-    weight = q_weight if q_weight is not None else k_weight
-    wdtype = 0 if weight is None else DTYPES[weight.dtype]
-    pos, ps = (0, (0, 0)) if positions is None else (positions.data_ptr(), positions.stride())
-    if cos is None:
-        return _PACK_PROBLEM.pack(batch, tokens, head_dim, 0, 0, DTYPES[dtype], wdtype, eps, 0, 0,
-                                  0, 0, 0, 0)
-    rows, pairs = cos.shape
-    return _PACK_PROBLEM.pack(batch, tokens, head_dim, 2 * pairs, int(interleaved), DTYPES[dtype],
-                              wdtype, eps, cos.data_ptr(), sin.data_ptr(), rows, pos, *ps)
-
-
-def _heads(t: Tensor) -> Tensor:
-    """The same values with a head's D values one after the other."""
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
-
-
-def _forward(problem: bytes, streams: bytes, count: int, device: torch.device) -> None:
-    _native.check("kat_qk_norm_rope_fwd",
-                  _native.on_stream(device, _native.lib().kat_qk_norm_rope_fwd, problem, streams, count))
-
-
-@functools.lru_cache(maxsize=None)
-def _workspace_bytes(head_dim: int, count: int, device_index: int) -> int:
-    n = _native.lib().kat_qk_norm_rope_bwd_workspace_bytes(head_dim, count, device_index)
-    if n == 0:
-        raise RuntimeError("kat_qk_norm_rope_bwd_workspace_bytes returned 0")
-    return n
-
-
-def _backward(problem: bytes, streams: bytes, count: int, head_dim: int,
-              device: torch.device) -> None:
-    n = _workspace_bytes(head_dim, count, device.index)
-    ws = torch.empty(n, device=device, dtype=torch.uint8)
-    _native.check("kat_qk_norm_rope_bwd",
-                  _native.on_stream(device, _native.lib().kat_qk_norm_rope_bwd, problem, streams, count,
-                          ws.data_ptr(), n))
-
-
-def _dweight(weight: Optional[Tensor], wanted: bool) -> Optional[Tensor]:
-    if weight is None or not wanted:
-        return None
-    return torch.empty(weight.shape, device=weight.device, dtype=torch.float32)
-
-
-def _as(grad: Optional[Tensor], like: Optional[Tensor]) -> Optional[Tensor]:
-    return grad if grad is None or grad.dtype == like.dtype else grad.to(like.dtype)
-
-
-def _qk_forward(q: Tensor, k: Tensor, q_weight, k_weight, cos, sin, positions, eps: float,
-                interleaved: bool):
-    """(q', k') and the queries and keys as the kernels read them."""
-    q, k = _heads(q), _heads(k)
-    B, L, Hq, D = q.shape
-    Hk = k.shape[2]
-    device, dtype = q.device, q.dtype
-    out_q = torch.empty((B, L, Hq, D), device=device, dtype=dtype)
-    out_k = torch.empty((B, L, Hk, D), device=device, dtype=dtype)
-    _forward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, eps,
-                           interleaved),
-             _pack(q.data_ptr(), 0, out_q.data_ptr(), q_weight, None, q.stride()[:3], _NO_STRIDE,
-                   (L * Hq * D, Hq * D, D), Hq)
-             + _pack(k.data_ptr(), 0, out_k.data_ptr(), k_weight, None, k.stride()[:3],
-                     _NO_STRIDE, (L * Hk * D, Hk * D, D), Hk), 2, device)
-    return out_q, out_k, q, k
-
-
-class QKNormRopeFunction(torch.autograd.Function):
-    """(q, k) -> (q', k'); gradients for q, k and the two weights."""
-
-    @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor, q_weight: Optional[Tensor],
-                k_weight: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor],
-                positions: Optional[Tensor], eps: float, interleaved: bool):
-        out_q, out_k, q, k = _qk_forward(q, k, q_weight, k_weight, cos, sin, positions, eps,
-                                         interleaved)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.eps, ctx.interleaved = eps, interleaved
-        return out_q, out_k
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq: Tensor, gk: Tensor):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        gq, gk = _heads(gq), _heads(gk)
-        B, L, Hq, D = q.shape
-        Hk = k.shape[2]
-        device, dtype = q.device, q.dtype
-        dq = torch.empty((B, L, Hq, D), device=device, dtype=dtype)
-        dk = torch.empty((B, L, Hk, D), device=device, dtype=dtype)
-        dwq, dwk = _dweight(q_weight, need[2]), _dweight(k_weight, need[3])
-        _backward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, ctx.eps,
-                                ctx.interleaved),
-                  _pack(q.data_ptr(), gq.data_ptr(), dq.data_ptr(), q_weight, dwq,
-                        q.stride()[:3], gq.stride()[:3], (L * Hq * D, Hq * D, D), Hq)
-                  + _pack(k.data_ptr(), gk.data_ptr(), dk.data_ptr(), k_weight, dwk,
-                          k.stride()[:3], gk.stride()[:3], (L * Hk * D, Hk * D, D), Hk), 2, D,
-                  device)
-        return (dq, dk, _as(dwq, q_weight), _as(dwk, k_weight), None, None, None, None, None)
-
-
-def _qkv_forward(qkv: Tensor, Hq: int, Hk: int, q_weight, k_weight, cos, sin, positions,
-                 eps: float, interleaved: bool):
-    """(q', k', v) and the projection's output as the kernels read it."""
-    if qkv.stride(2) != 1 and qkv.shape[2] != 1:
-        qkv = qkv.contiguous()
-    B, L, width = qkv.shape
-    D = width // (Hq + 2 * Hk)
-    device, dtype, size = qkv.device, qkv.dtype, qkv.element_size()
-    sb, sl = qkv.stride()[:2]
-    at, xs = qkv.data_ptr(), (sb, sl, D)
-    out_q = torch.empty((B, L, Hq, D), device=device, dtype=dtype)
-    out_k = torch.empty((B, L, Hk, D), device=device, dtype=dtype)
-    v = qkv.as_strided((B, L, Hk, D), (sb, sl, D, 1), qkv.storage_offset() + (Hq + Hk) * D)
-    _forward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, eps,
-                           interleaved),
-             _pack(at, 0, out_q.data_ptr(), q_weight, None, xs, _NO_STRIDE,
-                   (L * Hq * D, Hq * D, D), Hq)
-             + _pack(at and at + Hq * D * size, 0, out_k.data_ptr(), k_weight, None, xs,
-                     _NO_STRIDE, (L * Hk * D, Hk * D, D), Hk), 2, device)
-    return out_q, out_k, v, qkv
-
-
-class QKVNormRopeFunction(torch.autograd.Function):
-    """qkv [B, L, (Hq + 2 Hk) D] -> (q', k', v), v a view of qkv; one gradient for qkv, all of it
-    written by the backward kernel."""
-
-    @staticmethod
-    def forward(ctx, qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Tensor],
-                k_weight: Optional[Tensor], cos: Optional[Tensor], sin: Optional[Tensor],
-                positions: Optional[Tensor], eps: float, interleaved: bool):
-        out_q, out_k, v, x = _qkv_forward(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
-                                          positions, eps, interleaved)
-        ctx.save_for_backward(x, q_weight, k_weight, cos, sin, positions)
-        ctx.heads, ctx.eps, ctx.interleaved = (q_heads, k_heads), eps, interleaved
-        return out_q, out_k, v
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq: Tensor, gk: Tensor, gv: Tensor):
-        x, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        Hq, Hk = ctx.heads
-        need = ctx.needs_input_grad
-        gq, gk, gv = _heads(gq), _heads(gk), _heads(gv)
-        B, L, width = x.shape
-        D = width // (Hq + 2 * Hk)
-        device, dtype, size = x.device, x.dtype, x.element_size()
-        dx = torch.empty((B, L, width), device=device, dtype=dtype)
-        dwq, dwk = _dweight(q_weight, need[3]), _dweight(k_weight, need[4])
-        sb, sl = x.stride()[:2]
-        at, xs = x.data_ptr(), (sb, sl, D)
-        to, os = dx.data_ptr(), (L * width, width, D)
-        k_off, v_off = Hq * D * size, (Hq + Hk) * D * size
-        _backward(_pack_problem(B, L, D, dtype, q_weight, k_weight, cos, sin, positions, ctx.eps,
-                                ctx.interleaved),
-                  _pack(at, gq.data_ptr(), to, q_weight, dwq, xs, gq.stride()[:3], os, Hq)
-                  + _pack(at and at + k_off, gk.data_ptr(), to and to + k_off, k_weight, dwk, xs,
-                          gk.stride()[:3], os, Hk)
-                  + _pack(0, gv.data_ptr(), to and to + v_off, None, None, _NO_STRIDE,
-                          gv.stride()[:3], os, Hk), 3, D, device)
-        return (dx, None, None, _as(dwq, q_weight), _as(dwk, k_weight), None, None, None, None,
-                None)
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _check_rest(name: str, x: Tensor, head_dim: int, q_weight, k_weight, cos, sin, positions):
@@ -354,10 +142,8 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None,
         raise TypeError(f"qk_norm_rope: q is {q.dtype} on {q.device}, k {k.dtype} on {k.device}")
     positions = _check_rest("qk_norm_rope", q, q.shape[3], q_weight, k_weight, cos, sin,
                             positions)
-    if not _wants_grad(q, k, q_weight, k_weight):
-        return _qk_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)[:2]
-    return QKNormRopeFunction.apply(q, k, q_weight, k_weight, cos, sin, positions, eps,
-                                    interleaved)
+    return _native.ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                      interleaved)
 
 
 def qkv_norm_rope(qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Tensor] = None,
@@ -377,11 +163,8 @@ def qkv_norm_rope(qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Te
                          f"{k_heads} heads, got {tuple(qkv.shape)}")
     positions = _check_rest("qkv_norm_rope", qkv, qkv.shape[2] // (q_heads + 2 * k_heads),
                             q_weight, k_weight, cos, sin, positions)
-    if not _wants_grad(qkv, q_weight, k_weight):
-        return _qkv_forward(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin, positions, eps,
-                            interleaved)[:3]
-    return QKVNormRopeFunction.apply(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
-                                     positions, eps, interleaved)
+    return _native.ops().qkv_norm_rope(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
+                                       positions, eps, interleaved)
 
 
 class QKNormRope(nn.Module):

@@ -8,22 +8,19 @@ bucket of each (query, key).  Two kinds of bucket:
   IndexBuckets      of an index matrix [Lq, Lk], as `grid_index` makes one for a grid of patches
 
 `distance_bias` and `index_bias` evaluate them on the sm_100a kernels of libkat_rational.so
-(include/kat_position_bias.h), forward and backward; RelativePositionBias and GridPositionBias
-hold the table.  A bias is returned as a view whose rows start at multiples of 16 bytes (its row
+(include/kat_position_bias.h), forward and backward, called by the torch operators of libkat_torch.so
+(csrc/kat_torch.cpp); RelativePositionBias and GridPositionBias hold the table.  A bias is returned as a view whose rows start at multiples of 16 bytes (its row
 stride is Lk rounded up to 8), ready to be an attention kernel's mask.  There is no CPU
 implementation: CPU tables raise, and a missing library raises on first use.
 """
 
 from __future__ import annotations
 
-import functools
-import struct
 from typing import Dict, List, Optional, Tuple
 
 import torch
 import torch.nn as nn
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -36,7 +33,6 @@ MAX_DISTANCE_BUCKETS = 1024   # their borders are exact, in integers of that man
 MAX_LENGTH = (1 << 31) - 64
 MAX_REACH = 1 << 24
 INT32_MIN, INT32_MAX = -(1 << 31), (1 << 31) - 1
-_PACK_STRIDE = struct.Struct("=3q")
 
 
 def _round8(n: int) -> int:
@@ -244,94 +240,6 @@ def _check_table(name: str, table: Tensor, num_buckets: int, dtype: torch.dtype)
                          f"{tuple(table.shape)}")
 
 
-def _stride(t: Tensor) -> bytes:
-    return _PACK_STRIDE.pack(*t.stride())
-
-
-def _output(heads: int, lq: int, lk: int, device: torch.device,
-            dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
-    """The padded rows and the view of them that is returned."""
-    out = torch.empty((heads, lq, _round8(lk)), device=device, dtype=dtype)
-    return out, (out if lk % 8 == 0 else out.narrow(2, 0, lk))
-
-
-def _distance_forward(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int,
-                      causal: bool, dtype: torch.dtype) -> Tensor:
-    device, heads = table.device, table.shape[1]
-    table = table.contiguous()
-    out, view = _output(heads, lq, lk, device, dtype)
-    _native.check("kat_distance_bias_fwd", _native.on_stream(
-        device, _native.lib().kat_distance_bias_fwd, table.data_ptr(), DTYPES[table.dtype],
-        buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), buckets.reach, lq, lk,
-        offset, causal, out.data_ptr(), DTYPES[dtype]))
-    return view
-
-
-@functools.lru_cache(maxsize=4096)
-def _distance_workspace(heads: int, lq: int, lk: int) -> int:
-    return _native.lib().kat_distance_bias_bwd_workspace_bytes(heads, lq, lk)
-
-
-class DistanceBiasFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int,
-                causal: bool, dtype: torch.dtype) -> Tensor:
-        ctx.args = (buckets, table.shape[1], lq, lk, offset, causal, table.dtype)
-        return _distance_forward(table, buckets, lq, lk, offset, causal, dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad: Tensor):
-        buckets, heads, lq, lk, offset, causal, dtype = ctx.args
-        lib, device = _native.lib(), grad.device
-        _, begin, end = buckets.on(device)
-        nb = buckets.num_buckets
-        d = torch.empty((nb, heads), device=device, dtype=dtype)
-        size = _distance_workspace(heads, lq, lk)
-        ws = torch.empty(size, device=device, dtype=torch.uint8)
-        _native.check("kat_distance_bias_bwd", _native.on_stream(
-            device, lib.kat_distance_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
-            nb, heads, begin.data_ptr(), end.data_ptr(), lq, lk, offset, causal, d.data_ptr(),
-            DTYPES[dtype], ws.data_ptr(), size))
-        return d, None, None, None, None, None, None
-
-
-def _index_forward(table: Tensor, buckets: IndexBuckets, dtype: torch.dtype) -> Tensor:
-    device, heads = table.device, table.shape[1]
-    lq, lk = buckets.shape
-    table = table.contiguous()
-    out, view = _output(heads, lq, lk, device, dtype)
-    _native.check("kat_index_bias_fwd", _native.on_stream(
-        device, _native.lib().kat_index_bias_fwd, table.data_ptr(), DTYPES[table.dtype],
-        buckets.num_buckets, heads, buckets.on(device)[0].data_ptr(), lq, lk, out.data_ptr(),
-        DTYPES[dtype]))
-    return view
-
-
-class IndexBiasFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table: Tensor, buckets: IndexBuckets, dtype: torch.dtype) -> Tensor:
-        ctx.args = (buckets, table.shape[1], table.dtype)
-        return _index_forward(table, buckets, dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad: Tensor):
-        b, heads, dtype = ctx.args
-        lib, device = _native.lib(), grad.device
-        _, cells, padded, seg_begin, slab_begin, seg_place, bucket_begin = b.on(device)
-        d = torch.empty((b.num_buckets, heads), device=device, dtype=dtype)
-        size = 4 * heads * b.segments    # kat_index_bias_bwd_workspace_bytes
-        ws = torch.empty(size, device=device, dtype=torch.uint8)
-        _native.check("kat_index_bias_bwd", _native.on_stream(
-            device, lib.kat_index_bias_bwd, grad.data_ptr(), DTYPES[grad.dtype], _stride(grad),
-            b.num_buckets, heads, b.shape[0], b.shape[1], cells.data_ptr(),
-            padded.data_ptr(), seg_begin.data_ptr(), b.segments, slab_begin.data_ptr(), b.slabs,
-            b.slab_rows, seg_place.data_ptr(), bucket_begin.data_ptr(), d.data_ptr(),
-            DTYPES[dtype], ws.data_ptr(), size))
-        return d, None, None
-
-
 def distance_bias(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int = 0,
                   causal: bool = False, dtype: Optional[torch.dtype] = None) -> Tensor:
     """bias[h, i, j] = table[bucket(j - i - offset), h], [heads, lq, lk] of type `dtype` (default:
@@ -343,9 +251,9 @@ def distance_bias(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, off
     if not (0 <= lq <= MAX_LENGTH and 0 <= lk <= MAX_LENGTH and abs(offset) <= MAX_LENGTH):
         raise ValueError(f"distance_bias: lq, lk and |offset| must be 0..{MAX_LENGTH}, got "
                          f"{lq}, {lk} and {offset}")
-    if not (table.requires_grad and torch.is_grad_enabled()):
-        return _distance_forward(table, buckets, lq, lk, offset, causal, dtype)
-    return DistanceBiasFunction.apply(table, buckets, lq, lk, offset, causal, dtype)
+    return _native.ops().distance_bias(table, buckets.on(table.device), buckets.num_buckets,
+                                       buckets.reach, lq, lk, offset, bool(causal),
+                                       DTYPES[dtype])
 
 
 def index_bias(table: Tensor, buckets: IndexBuckets,
@@ -354,9 +262,9 @@ def index_bias(table: Tensor, buckets: IndexBuckets,
     table's)."""
     dtype = dtype or table.dtype
     _check_table("index_bias", table, buckets.num_buckets, dtype)
-    if not (table.requires_grad and torch.is_grad_enabled()):
-        return _index_forward(table, buckets, dtype)
-    return IndexBiasFunction.apply(table, buckets, dtype)
+    return _native.ops().index_bias(table, buckets.on(table.device), buckets.num_buckets,
+                                    *buckets.shape, buckets.slab_rows, buckets.slabs,
+                                    buckets.segments, DTYPES[dtype])
 
 
 class RelativePositionBias(nn.Module):

@@ -229,6 +229,19 @@ def test_streams_graphs_and_repeats(cuda_device):
             assert all(torch.equal(a, b) for a, b in zip(first, c))
 
 
+def test_gradients_are_differentiated_once(cuda_device):
+    table = normal(8, 2).requires_grad_()
+    up = normal(2, 3, 3, seed=1).requires_grad_()
+    index = torch.arange(9).view(3, 3) % 8
+    for out in (kat.distance_bias(table, kat.DistanceBuckets(8, 20), 3, 3),
+                kat.index_bias(table, kat.IndexBuckets(index, 8))):
+        plain = torch.autograd.grad(out, table, up, retain_graph=True)[0]
+        grad = torch.autograd.grad(out, table, up, create_graph=True)[0]
+        assert torch.equal(grad, plain) and grad.requires_grad
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(grad.sum(), up)
+
+
 def test_refusals(cuda_device):
     b = kat.DistanceBuckets(8, 20)
     for table, error in ((normal(7, 2), ValueError), (normal(8, 2)[0], ValueError),

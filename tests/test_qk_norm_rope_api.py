@@ -11,30 +11,51 @@ import rational_kat_cu_b200 as kat
 from rational_kat_cu_b200 import _native, head_norm
 
 
+class Stream(ctypes.Structure):
+    """`kat_head_stream`."""
+
+    _fields_ = [("x", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64 * 3), ("dy_stride", ctypes.c_int64 * 3),
+                ("out_stride", ctypes.c_int64 * 3), ("heads", ctypes.c_int32)]
+
+
+class Problem(ctypes.Structure):
+    """`kat_head_problem`."""
+
+    _fields_ = [("batch", ctypes.c_int64), ("tokens", ctypes.c_int64),
+                ("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+                ("table_rows", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                ("position_stride", ctypes.c_int64 * 2)]
+
+
 def problem(**kw):
     base = dict(batch=2, tokens=3, head_dim=64, rot_dim=64, interleaved=0, dtype=0, weight_dtype=0,
                 eps=1e-6, cos_table=256, sin_table=256, table_rows=3, positions=None,
                 position_stride=(0, 0))
     base.update(kw)
-    return head_norm._Problem(*base.values())
+    return Problem(*base.values())
 
 
 def stream(**kw):
     base = dict(x=256, dy=256, out=256, weight=None, dweight=None, x_stride=(0, 0, 0),
                 dy_stride=(0, 0, 0), out_stride=(0, 0, 0), heads=2)
     base.update(kw)
-    return head_norm._Stream(*base.values())
+    return Stream(*base.values())
 
 
 def fwd(p, *streams, count=None):
     return _native.lib().kat_qk_norm_rope_fwd(
-        ctypes.byref(p), (head_norm._Stream * len(streams))(*streams),
+        ctypes.byref(p), (Stream * len(streams))(*streams),
         len(streams) if count is None else count, None)
 
 
 def bwd(p, *streams, ws=None, size=0):
     return _native.lib().kat_qk_norm_rope_bwd(
-        ctypes.byref(p), (head_norm._Stream * len(streams))(*streams), len(streams), ws, size,
+        ctypes.byref(p), (Stream * len(streams))(*streams), len(streams), ws, size,
         None)
 
 

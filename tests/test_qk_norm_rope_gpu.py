@@ -308,6 +308,36 @@ def test_streams_graphs_and_repeats(cuda_device):
     assert torch.equal(alive[0], first[0])
 
 
+def test_gradients_are_differentiated_once(cuda_device):
+    qkv = normal(2, 3, 4 * 16).requires_grad_()
+    w = torch.ones(16, device="cuda", requires_grad=True)
+    for outs in (kat.qkv_norm_rope(qkv, 2, 1, w, None),
+                 kat.qk_norm_rope(qkv.view(2, 3, 4, 16), qkv.view(2, 3, 4, 16), None, w)):
+        ups = [normal(*o.shape, seed=i) for i, o in enumerate(outs)]
+        plain = torch.autograd.grad(outs, (qkv, w), ups, retain_graph=True)
+        grads = torch.autograd.grad(outs, (qkv, w), ups, create_graph=True)
+        for a, b in zip(grads, plain):
+            assert torch.equal(a, b) and a.requires_grad
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                torch.autograd.grad(a.sum(), qkv, retain_graph=True)
+
+
+def test_views_and_frozen_inputs(cuda_device):
+    """Values are a view of the projection's output; weights alone, or inputs alone, may train."""
+    qkv = normal(2, 3, 3 * 32)
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    q, k, v = kat.qkv_norm_rope(qkv, 1, 1, w, w)
+    assert v.data_ptr() == qkv.data_ptr() + 2 * 32 * 4 and not kat.qkv_norm_rope(qkv, 1, 1)[0].requires_grad
+    both = torch.autograd.grad((q, k), w, (q.detach(), k.detach()))[0]
+    assert both.isfinite().all()
+    with torch.no_grad():
+        assert not kat.qkv_norm_rope(qkv, 1, 1, w, w)[0].requires_grad
+    x = qkv.clone().requires_grad_()
+    q, k, v = kat.qkv_norm_rope(x, 1, 1, w.detach(), None)
+    dv = torch.autograd.grad(v, x, torch.ones_like(v))[0]       # of the values alone
+    assert not dv[..., :64].any() and (dv[..., 64:] == 1).all()
+
+
 def test_refusals(cuda_device):
     q = normal(1, 2, 3, 64)
     for k, error in ((q.half(), TypeError), (q[..., :32], ValueError), (q[:, :1], ValueError),
