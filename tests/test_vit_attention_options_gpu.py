@@ -131,7 +131,7 @@ def test_muon_updates_the_matrices(cuda_device, strict_fp32):
         # weight's rounding 2^-24, thrice
         moved = float((want - old.double()).norm())
         assert moved > 0
-        assert float((p.double() - want).norm()) <= 1e-4 * moved + 2.0 ** -22 * float(want.norm())
+        assert float((p.detach().double() - want).norm()) <= 1e-4 * moved + 2.0 ** -22 * float(want.norm())
     assert muon.device_status() == 0
 
 
