@@ -10,6 +10,7 @@ other (at most 200 here: 2^-16.3) after those errors: 2^-15 of the sum of magnit
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import rational_kat_cu_b200 as kat
 
@@ -336,6 +337,30 @@ def test_views_and_frozen_inputs(cuda_device):
     q, k, v = kat.qkv_norm_rope(x, 1, 1, w.detach(), None)
     dv = torch.autograd.grad(v, x, torch.ones_like(v))[0]       # of the values alone
     assert not dv[..., :64].any() and (dv[..., 64:] == 1).all()
+
+
+def test_recomputed_moved_and_overwritten_inputs(cuda_device):
+    """Saved tensors may be recomputed or kept elsewhere; one that was written over is refused."""
+    x = normal(2, 5, 3 * 64).requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+
+    def f(x):
+        return kat.qkv_norm_rope(x, 1, 1, w, w)[0]
+
+    want = torch.autograd.grad(f(x).square().sum(), (x, w))
+    again = torch.utils.checkpoint.checkpoint(f, x, use_reentrant=False)
+    with torch.autograd.graph.save_on_cpu():
+        moved = f(x)
+    for out in (again, moved):
+        got = torch.autograd.grad(out.square().sum(), (x, w))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y = x.clone()
+    out = f(y)
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    with pytest.raises(RuntimeError, match="view"):
+        kat.qkv_norm_rope(x.clone(), 1, 1, w, w)[2].mul_(2.0)
 
 
 def test_refusals(cuda_device):
