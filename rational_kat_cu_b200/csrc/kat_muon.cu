@@ -56,8 +56,8 @@ constexpr int kTM = 128;   // operand rows of a CTA: its tile rows, and its shar
 constexpr int kTK = 64;    // k-block: 64 fp16 = one 128-byte swizzle row
 constexpr int kUmmaK = 16;
 constexpr uint32_t kPlaneBytes = kTM * kTK * 2;        // one operand plane of a stage
-constexpr uint32_t kRingBytes = 12 * kPlaneBytes;      // stages: 3 of P and Q in two planes, 6 in one
-constexpr int kMaxStages = 8;                          // (half tiles: 4 and 8)
+constexpr uint32_t kRingBytes = 12 * kPlaneBytes;      // stages: 3 of P and Q in two planes
+constexpr int kMaxStages = 4;                          // (half tiles: 4)
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kPiece = 32;         // rows and columns an epilogue warp handles at once
@@ -318,7 +318,7 @@ template <auto V> struct Const { static constexpr auto value = V; };
 // depend on run-time values each MMA took 270 cycles to issue, four times its execution.  And the whole
 // warp comes here: in a branch of one lane each took 83 cycles, now 65 at most (one [768,768] bf16: 168
 // -> 145 us).
-template <int kPair, int kCols, bool kMnP, bool kMnQ, int kPlanes>
+template <int kPair, int kCols, bool kMnP, bool kMnQ>
 __device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, uint32_t step_p,
                                             uint32_t step_q, bool accumulate, uint32_t leader) {
   const uint64_t p_hi = kMnP ? desc_mn(p) : desc_k(p), q_hi = kMnQ ? desc_mn(q) : desc_k(q);
@@ -331,10 +331,8 @@ __device__ __forceinline__ void issue_block(uint32_t d, uint32_t p, uint32_t q, 
   for (int k = 0; k < kTK / kUmmaK; ++k) {
     umma_f16<kPair>(d, p_hi + k * kStepP, q_hi + k * kStepQ, idesc, accumulate || k != 0 ? 1u : 0u,
                     leader);
-    if constexpr (kPlanes == 2) {
-      umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u, leader);
-      umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u, leader);
-    }
+    umma_f16<kPair>(d, p_hi + k * kStepP, q_lo + k * kStepQ, idesc, 1u, leader);
+    umma_f16<kPair>(d, p_lo + k * kStepP, q_hi + k * kStepQ, idesc, 1u, leader);
   }
 }
 
@@ -567,7 +565,6 @@ struct GemmArgs {
   int32_t set_tiles;       // of all matrices of one set of operands
   int32_t total_tiles;     // of both sets
   int32_t k_blocks;
-  int32_t planes;          // 2: hi and lo of each operand and output, 1: hi alone
   float mult[2];           // accumulator -> plane (or, last, output) value, by set
   const __half* in;        // poly: planes of A
   int64_t ld, plane;
@@ -633,8 +630,9 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
   const uint32_t rank = kPair == 2 ? cluster_rank() : 0u;
   const int slot0 = int(blockIdx.x) / kPair, slots = int(gridDim.x) / kPair;
 
-  const int planes = args.planes, stages = (kParts == 1 ? 6 : 8) / planes;
-  const uint32_t stage_bytes = uint32_t(planes) * (kPlaneBytes + kQBytes);
+  constexpr int stages = kParts == 1 ? 3 : 4;
+  constexpr uint32_t stage_bytes = 2 * (kPlaneBytes + kQBytes);
+  static_assert(stages <= kMaxStages && stages * stage_bytes <= kRingBytes, "ring");
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(full + s, 1);
@@ -709,8 +707,8 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
         const bool inside = r < args.m && c < int(args.ld);   // ld is a multiple of 8
         const __half* at = args.in + int64_t(mat) * 2 * args.plane + int64_t(r) * args.ld + c;
         in_v[0][i] = inside ? *reinterpret_cast<const uint4*>(at) : make_uint4(0u, 0u, 0u, 0u);
-        in_v[1][i] = inside && args.planes == 2 ? *reinterpret_cast<const uint4*>(at + args.plane)
-                                                : make_uint4(0u, 0u, 0u, 0u);
+        in_v[1][i] = inside ? *reinterpret_cast<const uint4*>(at + args.plane)
+                            : make_uint4(0u, 0u, 0u, 0u);
       }
     } else if constexpr (kMode == kFinal) {
       if (args.has_momentum) {
@@ -797,8 +795,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       if (lane == 0 && row0 < args.m && col0 < args.n) {   // TMA leaves out what lies beyond
         const CUtensorMap* out = set ? &tm_out1 : &tm_out0;
         tma_store_3d(out, stage_out, col0, row0, 2 * mat);
-        if (args.planes == 2)
-          tma_store_3d(out, stage_out + kStagingBytes / 2, col0, row0, 2 * mat + 1);
+        tma_store_3d(out, stage_out + kStagingBytes / 2, col0, row0, 2 * mat + 1);
         bulk_commit();
       }
     }
@@ -828,14 +825,14 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
           };
           const bool mn_p = kSymP && kb * kTK / kTile > tr;
           const bool mn_q = kColsQ || (kSymQ && kb * kTK / kTile > tc);
-          for (int h = 0; h < planes; ++h) {
+          for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {   // boxes of 64 x 64: 64 rows, or 64 columns
               const int p = p0 + b * 64, q = q0 + b * 64, k = kb * kTK;
               load(s + h * kPlaneBytes + b * kBoxBytes, &tm_p, mn_p ? p : k, mn_p ? k : p,
                    2 * tmat + h);
               if (b < kCols / 64)
-                load(s + planes * kPlaneBytes + h * kQBytes + b * kBoxBytes, tm_q, mn_q ? q : k,
+                load(s + 2 * kPlaneBytes + h * kQBytes + b * kBoxBytes, tm_q, mn_q ? q : k,
                      mn_q ? k : q, 2 * tmat + h);
             }
           }
@@ -876,21 +873,16 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
           const uint32_t s = smem_u32(smem) + uint32_t(stage) * stage_bytes;
           const bool mn_p = kSymP && __any_sync(0xffffffffu, kb * kTK / kTile > tr);
           const bool mn_q = kColsQ || (kSymQ && __any_sync(0xffffffffu, kb * kTK / kTile > tc));
-          auto issue = [&](auto mn_p_, auto mn_q_, auto planes_) {
-            issue_block<kPair, kCols, mn_p_.value, mn_q_.value, planes_.value>(
-                d, s, s + planes_.value * kPlaneBytes, kPlaneBytes, kQBytes, kb != 0,
-                leader);
+          auto issue = [&](auto mn_p_, auto mn_q_) {
+            issue_block<kPair, kCols, mn_p_.value, mn_q_.value>(d, s, s + 2 * kPlaneBytes, kPlaneBytes,
+                                                                kQBytes, kb != 0, leader);
           };
-          auto issue_q = [&](auto mn_p_, auto planes_) {
-            if (mn_q) issue(mn_p_, Const<true>{}, planes_);
-            else issue(mn_p_, Const<false>{}, planes_);
+          auto issue_q = [&](auto mn_p_) {
+            if (mn_q) issue(mn_p_, Const<true>{});
+            else issue(mn_p_, Const<false>{});
           };
-          auto issue_p = [&](auto planes_) {
-            if (mn_p) issue_q(Const<true>{}, planes_);
-            else issue_q(Const<false>{}, planes_);
-          };
-          if (planes == 2) issue_p(Const<2>{});
-          else issue_p(Const<1>{});
+          if (mn_p) issue_q(Const<true>{});
+          else issue_q(Const<false>{});
           issued = true;
           if (leader) commit_all(empty + stage);
           if (++stage == stages) { stage = 0; phase ^= 1u; }
@@ -960,7 +952,7 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
 // ---------------------------------------------------------------------------
 
 struct ChainArgs {
-  int32_t m, steps, planes;
+  int32_t m, steps;
 };
 
 constexpr int kChainThreads = 512;
@@ -1013,11 +1005,10 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
   const uint32_t tmem = *tmem_slot;
   pdl_wait_previous();
 
-  const bool two = args.planes == 2;
   if (threadIdx.x == 0) {
     // rows and columns behind m arrive as zeros
-    mbar_expect_tx(loaded, uint32_t(args.planes) * kChainPlane);
-    for (int h = 0; h < args.planes; ++h)
+    mbar_expect_tx(loaded, kChainMatrix);
+    for (int h = 0; h < 2; ++h)
       for (int b = 0; b < 4; ++b)
         tma_load_3d(s_a + h * kChainPlane + b * kBoxBytes, &tm_a, loaded, (b >> 1) * 64,
                     (b & 1) * 64, 2 * mat + h);
@@ -1045,19 +1036,10 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
       const uint32_t leader = elect_lane();
       tc_fence_after();
       const uint32_t sp = smem_u32(p), sq = smem_u32(q);
-      if (two) {
-        issue_block<1, kTM, false, false, 2>(tmem, sp, sq, kChainPlane, kChainPlane, false,
-                                        leader);
-        if (args.m > kTK)
-          issue_block<1, kTM, false, false, 2>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
-                                              kChainPlane, true, leader);
-      } else {
-        issue_block<1, kTM, false, false, 1>(tmem, sp, sq, kChainPlane, kChainPlane, false,
-                                        leader);
-        if (args.m > kTK)
-          issue_block<1, kTM, false, false, 1>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
-                                              kChainPlane, true, leader);
-      }
+      issue_block<1, kTM, false, false>(tmem, sp, sq, kChainPlane, kChainPlane, false, leader);
+      if (args.m > kTK)
+        issue_block<1, kTM, false, false>(tmem, sp + kPlaneBytes, sq + kPlaneBytes, kChainPlane,
+                                          kChainPlane, true, leader);
       if (leader) umma_commit<1>(smem_u32(done));
     }
     ok = __syncthreads_and(wait_all(done, parity)) != 0;
@@ -1075,8 +1057,7 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
       float x[8], v[8];
       if (poly)
         join8(*reinterpret_cast<const uint4*>(s_a + at),
-              two ? *reinterpret_cast<const uint4*>(s_a + kChainPlane + at)
-                  : make_uint4(0u, 0u, 0u, 0u), x);
+              *reinterpret_cast<const uint4*>(s_a + kChainPlane + at), x);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         v[k] = y[g * 8 + k] * mult;
@@ -1120,7 +1101,7 @@ kat_muon_chain_kernel(const __grid_constant__ CUtensorMap tm_a,
   if (threadIdx.x == 0) {
     if (*abort == 0) {
       // Q as it lies: four boxes of 64 x 64, cut at m
-      for (int h = 0; h < args.planes; ++h)
+      for (int h = 0; h < 2; ++h)
         for (int b = 0; b < 4; ++b)
           if ((b >> 1) * 64 < args.m && (b & 1) * 64 < args.m)
             tma_store_3d(&tm_q, s_q + h * kChainPlane + b * kBoxBytes, (b >> 1) * 64, (b & 1) * 64,
@@ -1307,7 +1288,7 @@ int launch_gemm(bool pair, const Maps& m, GemmArgs args, const PtrTable& outs, i
 
 template <typename T>
 int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int64_t rows,
-        int64_t cols, int32_t steps, int late, uint8_t* ws, const Device& dev, bool vec,
+        int64_t cols, int32_t steps, uint8_t* ws, const Device& dev, bool vec,
         cudaStream_t stream) {
   const Layout L(count, rows, cols);
   __half* x[2] = {reinterpret_cast<__half*>(ws + L.x0), reinterpret_cast<__half*>(ws + L.x1)};
@@ -1354,7 +1335,6 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   sq.ld = L.ldm;
   sq.plane = L.plane_a;
   sq.k_blocks = k_m;
-  sq.planes = fin.planes = 2;
   sq.mult[0] = 1.0f / kScale;
   fin.m = int32_t(L.m);
   fin.n = int32_t(L.n);
@@ -1386,10 +1366,6 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
   int cur = 0;
   for (int done = 0; done < steps;) {
     const int block = block_steps(L.m, L.n, steps - done);
-    // the last steps in one plane, if the caller's type leaves them room
-    const bool last = done + block == steps;
-    if (steps - done <= late) sq.planes = 1;
-    fin.planes = sq.planes == 1 || (last && late > 0) ? 1 : 2;
     // gram
     GemmArgs g = sq;
     g.k_blocks = k_n;
@@ -1400,7 +1376,7 @@ int run(const Update& u, const PtrTable& outs, GemmArgs fin, int32_t count, int6
     float q_scale = kScale;
     const bool chained = L.m <= kTM;
     if (chained) {
-      const ChainArgs chain{int32_t(L.m), block, sq.planes};
+      const ChainArgs chain{int32_t(L.m), block};
       if (cudaFuncSetAttribute(kat_muon_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                int(kChainSmemBytes)) != cudaSuccess ||
           !launch_after(kat_muon_chain_kernel, dim3(uint32_t(count)), kChainThreads,
@@ -1501,21 +1477,13 @@ int dispatch(const Update& u, const PtrTable& outs, const GemmArgs& fin, int32_t
                   15u) == 0;
   uint8_t* w = static_cast<uint8_t*>(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // How many of the last steps take single planes.  Rounding their operands to 11 bits is no longer
-  // amplified: the result's error grows from 1e-5 to at most 1e-3 with one such step and 3e-3 with two
-  // (over spectra from flat to 32 strong directions a hundred times the rest).  A bf16 result is
-  // itself rounded by 2e-3; a weight of 16 bits by that much of the weight, of which a step's
-  // update is a small part.
-  const int late = dtype == KAT_DTYPE_F32 ? 0
-                   : fin.has_momentum   ? 2
-                                        : (dtype == KAT_DTYPE_BF16 ? 1 : 0);
   switch (dtype) {
     case KAT_DTYPE_F32:
-      return run<float>(u, outs, fin, count, rows, cols, steps, late, w, d, vec, st);
+      return run<float>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
     case KAT_DTYPE_F16:
-      return run<__half>(u, outs, fin, count, rows, cols, steps, late, w, d, vec, st);
+      return run<__half>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
     default:
-      return run<__nv_bfloat16>(u, outs, fin, count, rows, cols, steps, late, w, d, vec, st);
+      return run<__nv_bfloat16>(u, outs, fin, count, rows, cols, steps, w, d, vec, st);
   }
 }
 

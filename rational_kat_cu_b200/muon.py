@@ -7,10 +7,9 @@ matrix moves by about the same amount.  With X = u / |u|_F, `steps` times
     A = X X^T,   X <- a X + (b A + c A^2) X,   (a, b, c) = (3.4445, -4.7750, 2.0315)
 
 on the tcgen05 kernels of libkat_rational.so (include/kat_muon.h).  Matrices of one shape and
-type share their launches.  Operands are pairs of fp16 planes (22 bits) with fp32 accumulation: the
-result's relative error is about 1e-5, below any 16-bit rounding (the last steps of 16-bit results
-take single planes where their own rounding hides it).  There is no CPU implementation: CPU tensors
-raise, and a missing library raises on first use.
+type share their launches.  Operands are pairs of fp16 planes (22 bits) with fp32 accumulation, whatever the
+matrices' type: the result's relative error is about 1e-5, below any 16-bit rounding.  There is no
+CPU implementation: CPU tensors raise, and a missing library raises on first use.
 """
 
 from __future__ import annotations
