@@ -72,6 +72,15 @@ constexpr long long kWaitCycles = 4000000000LL;
 constexpr float kScale = 16384.0f;
 constexpr int kMaxBlock = 3;   // steps taken on the Gram matrix at once
 
+// k-blocks that one accumulator takes at most.  The tensor cores cut what they add, so a sum loses the
+// more the longer it is (always the same way where its terms have one sign, as on A's diagonal):
+// undivided, five steps of [128,65536] were off by 1e-3, three of [256,65536] by 3.3e-4 and five of
+// [4096,4096] by 1.0e-4; in parts of 16 by 2.2e-5, 4.2e-6 and 2.8e-5.  The parts are added up in fp32, with
+// rounding, while the MMAs wait for their accumulator: nothing up to 1024 terms, 1 % of
+// 12 x [768,2304], 4 % of [4096,4096].  (Parts of 8: half the error from 768 terms on, 3 to 6 %
+// slower everywhere.)
+constexpr int kSumBlocks = 16;
+
 __device__ int g_muon_status;
 
 enum Mode { kGram = 0, kSym = 1, kPoly = 2, kApply = 3, kFinal = 4 };
@@ -273,6 +282,22 @@ __device__ __forceinline__ void pdl_launch_next() {
 }
 __device__ __forceinline__ void pdl_wait_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// 16 values into consecutive columns of this thread's TMEM lane (complete after tmem_st_wait).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+      "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+      "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])), "r"(__float_as_uint(v[8])),
+      "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])),
+      "r"(__float_as_uint(v[15]))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 // 16 consecutive fp32 columns of this thread's TMEM lane, complete on return.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
@@ -565,6 +590,7 @@ struct GemmArgs {
   int32_t set_tiles;       // of all matrices of one set of operands
   int32_t total_tiles;     // of both sets
   int32_t k_blocks;
+  int32_t part_blocks;     // k-blocks of an accumulator (the last one's may be fewer)
   float mult[2];           // accumulator -> plane (or, last, output) value, by set
   const __half* in;        // poly: planes of A
   int64_t ld, plane;
@@ -585,6 +611,17 @@ __device__ __forceinline__ void read_piece(uint32_t taddr, float (&y)[kPiece]) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) y[g * 16 + k] = __uint_as_float(v[k]);
   }
+}
+
+// 32 columns at `from` added to those at `to`.
+__device__ __forceinline__ void add_piece(uint32_t to, uint32_t from) {
+  float y[kPiece], x[kPiece];
+  read_piece(from, y);
+  read_piece(to, x);
+#pragma unroll
+  for (int k = 0; k < kPiece; ++k) x[k] += y[k];
+  tmem_st16(to, x);
+  tmem_st16(to + 16, x + 16);
 }
 
 // Staging of a warp.  Planes: 32 rows of 64 bytes, 16-byte granules swizzled as TMA's 64-byte mode
@@ -854,40 +891,45 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
         return __all_sync(0xffffffffu, wait_phase(bar, parity, abort)) != 0;
       };
       int stage = 0, local = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, used = 0;   // used: how often each accumulator was, modulo 2
       bool issued = false, ok = true;
       auto commit_all = [&](uint64_t* bar) {
         umma_commit<kPair>(kPair == 1 ? smem_u32(bar) : cluster_addr(bar, 0));
         if constexpr (kPair == 2) umma_commit<kPair>(cluster_addr(bar, 1));
       };
       for (int tile = slot0; tile < args.total_tiles && ok; tile += slots, ++local) {
-        const int acc = local & 1;
         int tset, tmat, tr, tc, part;
         locate(tile, tset, tmat, tr, tc, part);
-        if (!wait_warp(tempty + acc, ((local >> 1) & 1) ^ 1u)) break;
-        tc_fence_after();
-        const uint32_t d = tmem_base + uint32_t(acc * kAccCols);
-        for (int kb = 0; kb < args.k_blocks; ++kb) {
-          if (!wait_warp(full + stage, phase)) { ok = false; break; }
+        // a sum's first part goes to one accumulator, all others to the other one
+        for (int kb0 = 0; kb0 < args.k_blocks && ok; kb0 += args.part_blocks) {
+          const int acc = (local & 1) ^ (kb0 != 0 ? 1 : 0);
+          if (!wait_warp(tempty + acc, ((used >> acc) & 1) ^ 1u)) { ok = false; break; }
+          used ^= 1u << acc;
           tc_fence_after();
-          const uint32_t s = smem_u32(smem) + uint32_t(stage) * stage_bytes;
-          const bool mn_p = kSymP && __any_sync(0xffffffffu, kb * kTK / kTile > tr);
-          const bool mn_q = kColsQ || (kSymQ && __any_sync(0xffffffffu, kb * kTK / kTile > tc));
-          auto issue = [&](auto mn_p_, auto mn_q_) {
-            issue_block<kPair, kCols, mn_p_.value, mn_q_.value>(d, s, s + 2 * kPlaneBytes, kPlaneBytes,
-                                                                kQBytes, kb != 0, leader);
-          };
-          auto issue_q = [&](auto mn_p_) {
-            if (mn_q) issue(mn_p_, Const<true>{});
-            else issue(mn_p_, Const<false>{});
-          };
-          if (mn_p) issue_q(Const<true>{});
-          else issue_q(Const<false>{});
-          issued = true;
-          if (leader) commit_all(empty + stage);
-          if (++stage == stages) { stage = 0; phase ^= 1u; }
+          const uint32_t d = tmem_base + uint32_t(acc * kAccCols);
+          const int kb1 = min(kb0 + args.part_blocks, args.k_blocks);
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!wait_warp(full + stage, phase)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t s = smem_u32(smem) + uint32_t(stage) * stage_bytes;
+            const bool mn_p = kSymP && __any_sync(0xffffffffu, kb * kTK / kTile > tr);
+            const bool mn_q = kColsQ || (kSymQ && __any_sync(0xffffffffu, kb * kTK / kTile > tc));
+            auto issue = [&](auto mn_p_, auto mn_q_) {
+              issue_block<kPair, kCols, mn_p_.value, mn_q_.value>(
+                  d, s, s + 2 * kPlaneBytes, kPlaneBytes, kQBytes, kb != kb0, leader);
+            };
+            auto issue_q = [&](auto mn_p_) {
+              if (mn_q) issue(mn_p_, Const<true>{});
+              else issue(mn_p_, Const<false>{});
+            };
+            if (mn_p) issue_q(Const<true>{});
+            else issue_q(Const<false>{});
+            issued = true;
+            if (leader) commit_all(empty + stage);
+            if (++stage == stages) { stage = 0; phase ^= 1u; }
+          }
+          if (ok && leader) commit_all(tfull + acc);
         }
-        if (ok && leader) commit_all(tfull + acc);
       }
       if (issued && leader) {
         // Every MMA has completed before the tensor memory is freed.
@@ -903,6 +945,26 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       step = lr * args.scale;
     }
     int local = 0;
+    uint32_t used = 0;
+    auto wait_acc = [&](int acc) {
+      const uint32_t parity = (used >> acc) & 1u;
+      used ^= 1u << acc;
+      int ok = 1;
+      if (lane == 0) ok = wait_phase(tfull + acc, parity, abort) ? 1 : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (ok) (void)mbar_try(tfull + acc, parity);  // completed: acquire for every lane
+      tc_fence_after();
+      return ok != 0;
+    };
+    // this warp is done with its part of the accumulator: hand it back to the MMA issuer
+    auto hand_back = [&](int acc) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair == 1) mbar_arrive(tempty + acc);
+        else mbar_arrive_cluster(cluster_addr(tempty + acc, 0));
+      }
+    };
     for (int tile = slot0; tile < args.total_tiles; tile += slots, ++local) {
       const int acc = local & 1;
       int tr, tc, part;
@@ -911,25 +973,23 @@ kat_muon_gemm_kernel(const __grid_constant__ CUtensorMap tm_p,
       row = row0 + lane;
       const int col_base = tc * kTile + part + half * (kAccCols / 2);
       prefetch(col_base);
-      int ok = 1;
-      if (lane == 0) ok = wait_phase(tfull + acc, (local >> 1) & 1, abort) ? 1 : 0;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      const uint32_t sums = lane_addr + uint32_t(acc * kAccCols + half * (kAccCols / 2));
+      const uint32_t others = lane_addr + uint32_t((acc ^ 1) * kAccCols + half * (kAccCols / 2));
+      bool ok = wait_acc(acc);
+      for (int kb0 = args.part_blocks; ok && kb0 < args.k_blocks; kb0 += args.part_blocks) {
+        ok = wait_acc(acc ^ 1);
+        if (!ok) break;
+#pragma unroll 1
+        for (int c = 0; c < kPieces; ++c) add_piece(sums + c * kPiece, others + c * kPiece);
+        tmem_st_wait();
+        hand_back(acc ^ 1);
+      }
       if (!ok) break;
-      (void)mbar_try(tfull + acc, (local >> 1) & 1);  // completed: acquire for every lane
-      tc_fence_after();
 #pragma unroll 1
       for (int c = 0; c < kPieces; ++c) {
         float y[kPiece];
-        read_piece(lane_addr + uint32_t(acc * kAccCols + half * (kAccCols / 2) + c * kPiece), y);
-        if (c == kPieces - 1) {
-          // this warp has read its part of the accumulator: hand it back to the MMA issuer
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (kPair == 1) mbar_arrive(tempty + acc);
-            else mbar_arrive_cluster(cluster_addr(tempty + acc, 0));
-          }
-        }
+        read_piece(sums + c * kPiece, y);
+        if (c == kPieces - 1) hand_back(acc);
         const int col0 = col_base + c * kPiece;
         finish(col0, y, c + 1 < kPieces ? col0 + kPiece : -1);
       }
@@ -1274,6 +1334,8 @@ int launch_gemm(bool pair, const Maps& m, GemmArgs args, const PtrTable& outs, i
                 const Device& dev, cudaStream_t stream) {
   const int side = pair ? 2 * kTM : kTM;
   const int tm = (args.m + side - 1) / side, tn = (args.n + side - 1) / side;
+  const int parts = (args.k_blocks + kSumBlocks - 1) / kSumBlocks;
+  args.part_blocks = (args.k_blocks + parts - 1) / parts;
   args.row_tiles = tm;
   args.tiles = kMode != kApply && kMode != kFinal ? tm * (tm + 1) / 2 : tm * tn;
   args.set_tiles = args.tiles * count;

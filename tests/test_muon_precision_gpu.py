@@ -1,11 +1,12 @@
 """How exact the orthogonalised updates are, on every way a product takes: a block of steps in one
-CTA, half tiles, whole tiles, CTA pairs and blocks on the Gram matrix.
+CTA, half tiles, whole tiles, CTA pairs, blocks on the Gram matrix, and sums of any length.
 
 Tolerances.  Operands of 22 bits leave 2^-22 of a product's operands.  The tensor cores cut their
-sums: adding 16 terms at a time of three products, a sum of 1024 terms is cut 192 times, each
+sums: adding 16 terms at a time of three products, a sum of at most 1024 terms is cut 192 times, each
 time by at most 2^-23 of what it has grown to, on average half of that of half of the sum: 192 / 4
-x 2^-23 = 6e-6 of |P| |Q|.  Five steps pass this on about eightfold: 5e-5, and 1e-4 is asserted.
-Operands that lose their second plane leave 1e-3.
+x 2^-23 = 6e-6 of |P| |Q| (longer sums are added up from such parts with rounding).  Five steps pass
+this on about eightfold: 5e-5, and 1e-4 is asserted.  Operands that lose their second plane leave
+1e-3, a sum cut 12288 times (65536 terms) 7e-4.
 
 A 16-bit result is the fp32 one, rounded once.  Of an element off by d before the rounding, the
 neighbour of the right one is taken with probability d / step, and is a step off then; the steps
@@ -60,6 +61,26 @@ def test_fp32(cuda_device, shape):
     for i in {0, shape[0] - 1}:
         assert apart(out[i], polar(x[i])) <= 1e-4
     assert muon.device_status() == 0
+
+
+@pytest.mark.parametrize("shape", [(1, 100, 65536), (2, 128, 16384), (1, 256, 16400), (2, 256, 65536),
+                                   (1, 20000, 300), (6, 700, 5000), (1, 2048, 2100),
+                                   (1, 1100, 65536)])
+@pytest.mark.parametrize("steps", [3, 5])
+def test_long_sums(cuda_device, shape, steps):
+    """Sums of more than 1024 terms, in single CTAs and pairs, several tiles to a block."""
+    x = normal(*shape, seed=shape[2])
+    out = kat.orthogonalize(x, steps=steps)
+    for i in {0, shape[0] - 1}:
+        assert apart(out[i], polar(x[i], steps)) <= 1e-4
+    assert muon.device_status() == 0
+    assert torch.equal(out, kat.orthogonalize(x, steps=steps))
+
+
+def test_long_sums_of_one_direction(cuda_device):
+    """Rows that agree: every term of a sum has one sign."""
+    x = 1 + 0.1 * normal(64, 40000)
+    assert apart(kat.orthogonalize(x), polar(x)) <= 1e-4
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
