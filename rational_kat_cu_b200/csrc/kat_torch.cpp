@@ -71,7 +71,14 @@ Tensor bytes_like(const Tensor& t, size_t bytes) {
   return at::empty({int64_t(bytes)}, t.options().dtype(at::kByte));
 }
 
+// There is no forward-mode derivative: a tangent raises, also where no gradient is wanted.
+void refuse_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                              "this operator has no forward-mode derivative");
+}
+
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) refuse_tangent(*t);
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;
@@ -88,6 +95,7 @@ struct Once : Function<Once> {
   }
 };
 variable_list once(variable_list results, const variable_list& from) {
+  for (const Tensor& anchor : from) refuse_tangent(anchor);
   if (!at::GradMode::is_enabled()) return results;
   for (const Tensor& anchor : from) {
     if (!anchor.defined() || !anchor.requires_grad()) continue;
@@ -262,7 +270,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
                                         bool interleaved) {
   const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
   const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
-  const variable_list out = wants_grad({&q, &k, &wq, &wk})
+  const variable_list out = wants_grad({&q, &k, &wq, &wk, &rope.cos, &rope.sin})
                                 ? QkNormRope::apply(q, k, q_weight, k_weight, rope)
                                 : qk_forward(heads_of(q), heads_of(k), wq, wk, rope);
   return {out[0], out[1]};
@@ -334,7 +342,7 @@ std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, int64_t q_he
                                                  bool interleaved) {
   const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
   const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
-  const variable_list out = wants_grad({&qkv, &wq, &wk})
+  const variable_list out = wants_grad({&qkv, &wq, &wk, &rope.cos, &rope.sin})
                                 ? QkvNormRope::apply(qkv, q_weight, k_weight, q_heads, k_heads, rope)
                                 : qkv_forward(packed_of(qkv), q_heads, k_heads, wq, wk, rope);
   return {out[0], out[1], out[2]};

@@ -1,0 +1,51 @@
+"""Calls of the attention-input operators around their values: forward-mode tangents, in-place use of
+their results, plans made ahead and copied, tracing, and tensors with a pending negation."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+import rational_kat_cu_b200 as kat
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(*shape, seed=0, dtype=torch.float32):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def grid_plan():
+    return kat.IndexBuckets(*kat.grid_index(3, 4, prefix=1))
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("which", ["q", "k", "weight", "qkv", "packed weight", "distance", "index"])
+def test_forward_mode_raises(cuda_device, which, requires_grad, no_grad):
+    """No tangent is dropped without a word."""
+    shape = {"q": (2, 3, 4, 16), "k": (2, 3, 2, 16), "weight": (16,), "packed weight": (16,),
+             "qkv": (2, 3, 64), "distance": (32, 2), "index": (38, 2)}[which]
+    x = normal(*shape).requires_grad_(requires_grad)
+    q, k, qkv, w = (normal(2, 3, 4, 16), normal(2, 3, 2, 16), normal(2, 3, 64), normal(16))
+    with fwd.dual_level(), torch.set_grad_enabled(not no_grad):
+        d = fwd.make_dual(x, normal(*shape, seed=1))
+        call = {"q": lambda: kat.qk_norm_rope(d, k, w, w),
+                "k": lambda: kat.qk_norm_rope(q, d, w, w),
+                "weight": lambda: kat.qk_norm_rope(q, k, None, d),
+                "qkv": lambda: kat.qkv_norm_rope(d, 2, 1, w, w),
+                "packed weight": lambda: kat.qkv_norm_rope(qkv, 2, 1, d, w),
+                "distance": lambda: kat.distance_bias(d, kat.DistanceBuckets(), 5, 6),
+                "index": lambda: kat.index_bias(d, grid_plan())}[which]
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call()
+
+
+def test_forward_mode_of_gradients_raises(cuda_device):
+    table, x = normal(32, 2).requires_grad_(), normal(2, 3, 64).requires_grad_()
+    outs = (kat.distance_bias(table, kat.DistanceBuckets(), 5, 6), kat.qkv_norm_rope(x, 2, 1)[0])
+    with fwd.dual_level():
+        for out, leaf in zip(outs, (table, x)):
+            up = fwd.make_dual(normal(*out.shape, seed=2), normal(*out.shape, seed=3))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                torch.autograd.grad(out, leaf, up)
