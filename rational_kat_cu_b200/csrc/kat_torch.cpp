@@ -8,6 +8,7 @@
 // block at batch 128: 104 and 156; one token's, forward alone: 14 and 21).
 
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -354,11 +355,14 @@ std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, int64_t q_he
 
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// Rows padded to multiples of 8, and the view of their lk columns.
+// Rows padded to multiples of 8, and their lk columns as a tensor of its own: autograd does not know it
+// as a view, which could not be changed in place outside the node that made it.
 std::pair<Tensor, Tensor> rows_of(const Tensor& table, int64_t lq, int64_t lk, int64_t type) {
   const Tensor out = at::empty({table.size(1), lq, round8(lk)},
                                table.options().dtype(type_of(type)).requires_grad(false));
-  return {out, lk % 8 == 0 ? out : out.narrow(2, 0, lk)};
+  if (lk % 8 == 0) return {out, out};
+  const at::AutoDispatchBelowADInplaceOrView no_views;
+  return {out, out.narrow(2, 0, lk)};
 }
 Tensor dtable_of(const Tensor& grad, int64_t buckets, at::ScalarType type) {
   return at::empty({buckets, grad.size(0)}, grad.options().dtype(type).requires_grad(false));

@@ -49,3 +49,31 @@ def test_forward_mode_of_gradients_raises(cuda_device):
             up = fwd.make_dual(normal(*out.shape, seed=2), normal(*out.shape, seed=3))
             with pytest.raises((RuntimeError, NotImplementedError)):
                 torch.autograd.grad(out, leaf, up)
+
+
+@pytest.mark.parametrize("lk", [197, 200, 1, 8])
+@pytest.mark.parametrize("kind", ["distance", "index"])
+def test_results_change_in_place(cuda_device, kind, lk):
+    """A mask added to or written into a bias that needs a gradient, at any length."""
+    lq = 5
+    if kind == "distance":
+        b = kat.DistanceBuckets(8, 20)
+        make = lambda t: kat.distance_bias(t, b, lq, lk)  # noqa: E731
+    else:
+        b = kat.IndexBuckets((torch.arange(lq)[:, None] + torch.arange(lk)) % 8, 8)
+        make = lambda t: kat.index_bias(t, b)  # noqa: E731
+    table = normal(8, 3).requires_grad_()
+    mask = torch.rand(lq, lk, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) < 0.5
+    grad = normal(3, lq, lk, seed=2)
+    plain = make(table)
+    want = torch.where(mask, -1.0, 2 * (plain + 1))
+    want_grad, = torch.autograd.grad(want, table, grad)
+    bias = make(table)
+    bias += 1
+    bias.mul_(2).masked_fill_(mask, -1.0)
+    assert torch.equal(bias, want)
+    assert torch.equal(torch.autograd.grad(bias, table, grad)[0], want_grad)
+    with torch.no_grad():
+        bias = make(table)
+        bias[:, 0] = 3.0
+    assert bias.stride(1) % 8 == 0 and (bias[:, 0] == 3).all()
