@@ -39,6 +39,18 @@ def _round8(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
+def _kept_on(kept: Dict[torch.device, Tuple[Tensor, ...]], tensors: Tuple[Tensor, ...],
+             device: torch.device) -> Tuple[Tensor, ...]:
+    """The copies of `tensors` that `kept` holds for `device` ("cuda" is the current device), made
+    if it has none."""
+    if device not in kept:
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if device not in kept:
+            kept[device] = _copied(tensors, device)
+    return kept[device]
+
+
 def _copied(tensors: Tuple[Tensor, ...], device: torch.device) -> Tuple[Tensor, ...]:
     """Copies on `device` that any stream may use."""
     copies = tuple(t.to(device) for t in tensors)
@@ -126,9 +138,7 @@ class DistanceBuckets:
     def on(self, device: torch.device) -> Tuple[Tensor, Tensor, Tensor]:
         """(bucket_of, run_begin, run_end) on `device`, kept there (the first use on a device
         copies them: not inside a graph capture)."""
-        if device not in self._on:
-            self._on[device] = _copied((self._of, self._begin, self._end), device)
-        return self._on[device]
+        return _kept_on(self._on, (self._of, self._begin, self._end), device)
 
     def __repr__(self) -> str:
         return (f"DistanceBuckets(num_buckets={self.num_buckets}, "
@@ -200,9 +210,7 @@ class IndexBuckets:
     def on(self, device: torch.device) -> Tuple[Tensor, ...]:
         """(index, cells, padded_cells, seg_begin, slab_begin, seg_place, bucket_begin) on `device`,
         kept there (the first use on a device copies them: not inside a graph capture)."""
-        if device not in self._on:
-            self._on[device] = _copied(self._tensors, device)
-        return self._on[device]
+        return _kept_on(self._on, self._tensors, device)
 
     def __repr__(self) -> str:
         return f"IndexBuckets(shape={self.shape}, num_buckets={self.num_buckets})"

@@ -77,3 +77,22 @@ def test_results_change_in_place(cuda_device, kind, lk):
         bias = make(table)
         bias[:, 0] = 3.0
     assert bias.stride(1) % 8 == 0 and (bias[:, 0] == 3).all()
+
+
+def test_plans_made_for_cuda_are_ready(cuda_device):
+    """device="cuda" is the current device: the first use copies nothing and may be captured."""
+    b = kat.DistanceBuckets(32, 128, device="cuda")
+    assert all(t.device == torch.device("cuda", 0) for t in b.on(torch.device("cuda")))
+    assert b.on(torch.device("cuda"))[0] is b.on(torch.device("cuda", 0))[0]
+    plan = grid_plan()
+    plan.on(torch.device("cuda"))
+    table, cells = normal(32, 2), normal(38, 2)
+    kat.distance_bias(table, kat.DistanceBuckets(), 3, 3)      # the library is loaded
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = kat.distance_bias(table, b, 40, 50), kat.index_bias(cells, plan)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], kat.distance_bias(table, b, 40, 50))
+    assert torch.equal(got[1], kat.index_bias(cells, plan))
