@@ -59,7 +59,18 @@ def _copied(tensors: Tuple[Tensor, ...], device: torch.device) -> Tuple[Tensor, 
     return copies
 
 
-class DistanceBuckets:
+class _Plan:
+    """What bucket plans share.  A plan does not change once made: copies of a module share it.  Its copies
+    on devices are not stored with it, since torch.load may put those on any device."""
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "_on": {}}
+
+    def __deepcopy__(self, memo) -> "_Plan":
+        return self
+
+
+class DistanceBuckets(_Plan):
     """Buckets of a distance d = key - query.
 
     bidirectional: half of the buckets for d <= 0, half for d > 0, by |d|; otherwise all of them
@@ -145,7 +156,7 @@ class DistanceBuckets:
                 f"max_distance={self.max_distance}, bidirectional={self.bidirectional})")
 
 
-class IndexBuckets:
+class IndexBuckets(_Plan):
     """Buckets of an index matrix [Lq, Lk] with values in [0, num_buckets); -1 marks cells without
     a bias (0, and no gradient).  Keeps the cells sorted by bucket, for the gradient: make it
     once.  Lk is at most 16384 (long sequences go by distance)."""

@@ -1,6 +1,9 @@
 """Calls of the attention-input operators around their values: forward-mode tangents, in-place use of
 their results, plans made ahead and copied, tracing, and tensors with a pending negation."""
 
+import copy
+import io
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -96,3 +99,21 @@ def test_plans_made_for_cuda_are_ready(cuda_device):
     torch.cuda.synchronize()
     assert torch.equal(got[0], kat.distance_bias(table, b, 40, 50))
     assert torch.equal(got[1], kat.index_bias(cells, plan))
+
+
+@pytest.mark.parametrize("kind", ["distance", "index"])
+def test_stored_plans_hold_no_device_copies(cuda_device, kind):
+    """torch.load may put a stored tensor on another device than the one it was kept for."""
+    b = kat.DistanceBuckets() if kind == "distance" else grid_plan()
+    dev = torch.device("cuda", 0)
+    want = b.on(dev)
+    buffer = io.BytesIO()
+    torch.save(b, buffer)
+    for where in ("cpu", None):
+        buffer.seek(0)
+        back = torch.load(buffer, map_location=where, weights_only=False)
+        got = back.on(dev)
+        assert all(t.device == dev for t in got)
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
+    # a copied model's plans are as ready as the model's
+    assert copy.deepcopy(b).on(dev)[0] is want[0]
