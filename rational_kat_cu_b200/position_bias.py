@@ -66,6 +66,9 @@ class _Plan:
     def __getstate__(self) -> dict:
         return {**self.__dict__, "_on": {}}
 
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state, _on={})
+
     def __deepcopy__(self, memo) -> "_Plan":
         return self
 
