@@ -124,6 +124,7 @@ def _need_cuda(name: str, t: Tensor) -> None:
                            f"implementation")
 
 
+@_native.untraced
 def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None,
                  k_weight: Optional[Tensor] = None, cos: Optional[Tensor] = None,
                  sin: Optional[Tensor] = None, positions: Optional[Tensor] = None,
@@ -146,6 +147,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None,
                                       interleaved)
 
 
+@_native.untraced
 def qkv_norm_rope(qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Tensor] = None,
                   k_weight: Optional[Tensor] = None, cos: Optional[Tensor] = None,
                   sin: Optional[Tensor] = None, positions: Optional[Tensor] = None,

@@ -66,6 +66,7 @@ def _runs(count: int, rows: int, cols: int):
         yield start, n, lib.kat_muon_workspace_bytes(n, rows, cols)
 
 
+@_native.untraced
 @torch.no_grad()
 def orthogonalize(x: Tensor, steps: int = 5) -> Tensor:
     """The Newton-Schulz polar factor of each matrix of x [..., rows, cols], in x's type.  Zero
@@ -129,6 +130,7 @@ def _check_step_lists(weights, grads, momenta) -> None:
                 raise ValueError("muon_step: a gradient shares memory with a weight or momentum")
 
 
+@_native.untraced
 @torch.no_grad()
 def muon_step(weights: Sequence[Tensor], grads: Sequence[Tensor], momenta: Sequence[Tensor],
               lr: Union[float, Tensor], momentum: float = 0.95, nesterov: bool = True,

@@ -262,6 +262,7 @@ def _check_table(name: str, table: Tensor, num_buckets: int, dtype: torch.dtype)
                          f"{tuple(table.shape)}")
 
 
+@_native.untraced
 def distance_bias(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, offset: int = 0,
                   causal: bool = False, dtype: Optional[torch.dtype] = None) -> Tensor:
     """bias[h, i, j] = table[bucket(j - i - offset), h], [heads, lq, lk] of type `dtype` (default:
@@ -278,6 +279,7 @@ def distance_bias(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, off
                                        DTYPES[dtype])
 
 
+@_native.untraced
 def index_bias(table: Tensor, buckets: IndexBuckets,
                dtype: Optional[torch.dtype] = None) -> Tensor:
     """bias[h, i, j] = table[index[i, j], h], [heads, Lq, Lk] of type `dtype` (default: the

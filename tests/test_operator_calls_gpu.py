@@ -9,6 +9,7 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 import rational_kat_cu_b200 as kat
+from rational_kat_cu_b200 import grkan_vit as gv
 
 pytestmark = pytest.mark.gpu
 
@@ -117,3 +118,52 @@ def test_stored_plans_hold_no_device_copies(cuda_device, kind):
         assert all(torch.equal(s, t) for s, t in zip(got, want))
     # a copied model's plans are as ready as the model's
     assert copy.deepcopy(b).on(dev)[0] is want[0]
+
+
+def test_compiled_callers_go_on(cuda_device):
+    """torch.compile leaves the operators out of its graphs, as it does rat_cuda."""
+    torch._dynamo.reset()
+    b, plan = kat.DistanceBuckets(device="cuda"), grid_plan()
+    cos, sin = kat.rope_table(7, 16, device="cuda")
+
+    def attention(x, w, table, cells):
+        q, k, v = kat.qkv_norm_rope(x * 2, 2, 1, w, w, cos, sin)
+        q, k = kat.qk_norm_rope(q + 1, k, w, None)
+        return (q.sum() + k.sum() * v.sum() + kat.distance_bias(table, b, 7, 5).square().sum()
+                + kat.index_bias(cells, plan).square().sum())
+
+    args = [t.requires_grad_() for t in (normal(2, 7, 64), normal(16), normal(32, 2), normal(38, 2))]
+    want = attention(*args)
+    got = torch.compile(attention, backend="eager")(*args)
+    assert torch.equal(got, want)
+    for g, w in zip(torch.autograd.grad(got, args), torch.autograd.grad(want, args)):
+        assert torch.equal(g, w)
+
+
+def test_compiled_updates_go_on(cuda_device):
+    torch._dynamo.reset()
+    w, g = normal(24, 40), normal(24, 40, seed=1)
+    other = w.clone()
+    m, n = torch.zeros(2, 24, 40, device="cuda")
+
+    def update(w, g, m):
+        kat.muon_step([w], [g * 2], [m], lr=0.1)
+        return kat.orthogonalize(g + 1) + 1
+
+    want = update(w, g, m)
+    assert torch.equal(torch.compile(update, backend="eager")(other, g, n), want)
+    assert torch.equal(w, other) and torch.equal(m, n)
+
+
+def test_compiled_attention_options(cuda_device):
+    """The options of the attention blocks (KAT_Group itself cannot be traced: plain MLPs)."""
+    torch._dynamo.reset()
+    cfg = gv.ViTConfig(image_size=32, patch_size=16, num_classes=5, embed_dim=64, depth=1,
+                       num_heads=2, act="gelu", qk_norm=True, rope=True, rel_pos_bias=True)
+    torch.manual_seed(0)
+    model = gv.GRKANViT(cfg).cuda()
+    images, labels = gv.synthetic_batch(2, cfg, dtype=torch.float32, seed=1)
+    images, labels = images.cuda(), labels.cuda()
+    want = model(images)
+    got = torch.compile(model, backend="eager")(images)
+    assert torch.equal(got, want)
