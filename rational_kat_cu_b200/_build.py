@@ -86,7 +86,10 @@ def build_torch(force: bool = False) -> str:
            "-I", os.path.join(REPO_DIR, "include"), "-isystem", os.path.join(base, "include"),
            "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
            "-isystem", os.path.join(cuda, "include"), TORCH_SOURCE, "-o", TORCH_LIBRARY + ".tmp",
-           "-L", os.path.join(base, "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           "-L", os.path.join(base, "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           # torch's own C++ runtime, also where the compiler would link a static copy: with two in a
+           # process, an error message with a number in it ends the process
+           "-l:libstdc++.so.6"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
