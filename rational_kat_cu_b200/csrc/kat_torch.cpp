@@ -60,6 +60,22 @@ at::ScalarType type_of(int64_t code) {
   return code == KAT_DTYPE_F32 ? at::kFloat : code == KAT_DTYPE_F16 ? at::kHalf : at::kBFloat16;
 }
 
+// What an operator takes, checked here too: torch.ops reaches it past the Python functions.
+bool known_type(at::ScalarType type) {
+  return type == at::kFloat || type == at::kHalf || type == at::kBFloat16;
+}
+bool plain(const Tensor& t) { return t.layout() == at::kStrided && !t._is_zerotensor(); }
+bool whole(const Tensor& t, const Tensor& like) {
+  return plain(t) && t.device() == like.device() && t.is_contiguous();
+}
+// `n` values of `type`, one after the other, where `like` is.
+bool run_of(const Tensor& t, const Tensor& like, at::ScalarType type, int64_t n) {
+  return t.scalar_type() == type && t.numel() == n && whole(t, like);
+}
+void need_cuda(const char* name, const Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), name, ": expected CUDA tensors, got ", t.device());
+}
+
 // The current stream of a tensor's device, which is the current device meanwhile.
 struct On {
   c10::cuda::CUDAGuard guard;
@@ -118,6 +134,41 @@ struct Rope {   // undefined tensors: none
   double eps;
   bool interleaved;
 };
+
+void check_rope(const char* name, const Tensor& x, int64_t head_dim, const Tensor& q_weight,
+                const Tensor& k_weight, const Rope& rope) {
+  TORCH_CHECK(known_type(x.scalar_type()) && plain(x), name,
+              ": queries and keys must be dense float32, float16 or bfloat16");
+  TORCH_CHECK(head_dim >= 1 && head_dim <= 1024, name, ": head size must be 1..1024, got ", head_dim);
+  for (const Tensor* w : {&q_weight, &k_weight})
+    TORCH_CHECK(!w->defined() || (known_type(w->scalar_type()) && w->dim() == 1 &&
+                                  w->numel() == head_dim && whole(*w, x)),
+                name, ": a weight must be a contiguous [", head_dim, "] on ", x.device());
+  TORCH_CHECK(!q_weight.defined() || !k_weight.defined() ||
+                  q_weight.scalar_type() == k_weight.scalar_type(),
+              name, ": the weights' types differ");
+  TORCH_CHECK(rope.cos.defined() == rope.sin.defined(), name, ": cos and sin come together");
+  if (!rope.cos.defined()) {
+    TORCH_CHECK(!rope.positions.defined(), name, ": positions without a table");
+    return;
+  }
+  TORCH_CHECK(rope.cos.dim() == 2 && rope.cos.sizes() == rope.sin.sizes() &&
+                  2 * rope.cos.size(1) <= head_dim &&
+                  run_of(rope.cos, x, at::kFloat, rope.cos.numel()) &&
+                  run_of(rope.sin, x, at::kFloat, rope.cos.numel()) && !rope.cos.requires_grad() &&
+                  !rope.sin.requires_grad(),
+              name, ": cos and sin must be contiguous float32 [rows, at most ", head_dim / 2, "] on ",
+              x.device(), ", without a gradient");
+  if (rope.positions.defined()) {
+    TORCH_CHECK(rope.positions.scalar_type() == at::kLong && plain(rope.positions) &&
+                    rope.positions.device() == x.device() && rope.positions.dim() == 2 &&
+                    rope.positions.size(0) == x.size(0) && rope.positions.size(1) == x.size(1),
+                name, ": positions must be int64 [", x.size(0), ", ", x.size(1), "] on ", x.device());
+  } else {
+    TORCH_CHECK(rope.cos.size(0) >= x.size(1), name, ": ", x.size(1), " tokens, and a table of ",
+                rope.cos.size(0), " rows");
+  }
+}
 
 const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
@@ -271,6 +322,12 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
                                         bool interleaved) {
   const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
   const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+                  q.size(3) == k.size(3) && q.scalar_type() == k.scalar_type() &&
+                  q.device() == k.device() && plain(k),
+              "qk_norm_rope: expected q [B, L, Hq, D] and k [B, L, Hk, D] of one type on one device");
+  check_rope("qk_norm_rope", q, q.size(3), wq, wk, rope);
+  need_cuda("qk_norm_rope", q);
   const variable_list out = wants_grad({&q, &k, &wq, &wk, &rope.cos, &rope.sin})
                                 ? QkNormRope::apply(q, k, q_weight, k_weight, rope)
                                 : qk_forward(heads_of(q), heads_of(k), wq, wk, rope);
@@ -343,6 +400,12 @@ std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, int64_t q_he
                                                  bool interleaved) {
   const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
   const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
+  constexpr int64_t most = int64_t(1) << 31;
+  TORCH_CHECK(qkv.dim() == 3 && q_heads >= 1 && k_heads >= 1 && q_heads < most && k_heads < most &&
+                  qkv.size(2) > 0 && qkv.size(2) % (q_heads + 2 * k_heads) == 0,
+              "qkv_norm_rope: expected [B, L, (q_heads + 2 k_heads) D]");
+  check_rope("qkv_norm_rope", qkv, qkv.size(2) / (q_heads + 2 * k_heads), wq, wk, rope);
+  need_cuda("qkv_norm_rope", qkv);
   const variable_list out = wants_grad({&qkv, &wq, &wk, &rope.cos, &rope.sin})
                                 ? QkvNormRope::apply(qkv, q_weight, k_weight, q_heads, k_heads, rope)
                                 : qkv_forward(packed_of(qkv), q_heads, k_heads, wq, wk, rope);
@@ -366,6 +429,20 @@ std::pair<Tensor, Tensor> rows_of(const Tensor& table, int64_t lq, int64_t lk, i
 }
 Tensor dtable_of(const Tensor& grad, int64_t buckets, at::ScalarType type) {
   return at::empty({buckets, grad.size(0)}, grad.options().dtype(type).requires_grad(false));
+}
+
+constexpr int64_t kMaxLength = (int64_t(1) << 31) - 64;   // as the entries have it
+
+// The values of a plan are those DistanceBuckets or IndexBuckets made; its sizes are checked.
+void check_table(const char* name, const Tensor& table, int64_t buckets, int64_t lq, int64_t lk,
+                 int64_t type) {
+  TORCH_CHECK(table.dim() == 2 && plain(table) && known_type(table.scalar_type()) && buckets >= 1 &&
+                  table.size(0) == buckets && buckets <= (int64_t(1) << 24) && table.size(1) <= 65535,
+              name, ": expected a dense float32, float16 or bfloat16 table [", buckets, ", heads]");
+  TORCH_CHECK(lq >= 0 && lk >= 0 && lq <= kMaxLength && lk <= kMaxLength, name,
+              ": lengths must be 0..", kMaxLength, ", got ", lq, " and ", lk);
+  TORCH_CHECK(type == KAT_DTYPE_F32 || type == KAT_DTYPE_F16 || type == KAT_DTYPE_BF16, name,
+              ": unknown type ", type);
 }
 
 struct Distance {
@@ -414,7 +491,14 @@ struct DistanceBias : Function<DistanceBias> {
 
 Tensor distance_bias(const Tensor& table, at::TensorList plan, int64_t buckets, int64_t reach,
                      int64_t lq, int64_t lk, int64_t offset, bool causal, int64_t type) {
-  TORCH_CHECK(plan.size() == 3, "distance_bias: a plan has 3 tensors");
+  check_table("distance_bias", table, buckets, lq, lk, type);
+  TORCH_CHECK(offset >= -kMaxLength && offset <= kMaxLength, "distance_bias: |offset| must be 0..",
+              kMaxLength, ", got ", offset);
+  TORCH_CHECK(plan.size() == 3 && reach >= 0 && reach <= (int64_t(1) << 24) &&
+                  run_of(plan[0], table, at::kInt, 2 * reach + 1) &&
+                  run_of(plan[1], table, at::kInt, buckets) && run_of(plan[2], table, at::kInt, buckets),
+              "distance_bias: the plan has another reach, number of buckets or device");
+  need_cuda("distance_bias", table);
   const Distance a{plan[0], plan[1], plan[2], buckets, reach, lq, lk, offset, causal, type};
   return wants_grad({&table}) ? DistanceBias::apply(table, a) : distance_forward(table, a);
 }
@@ -465,7 +549,18 @@ struct IndexBias : Function<IndexBias> {
 
 Tensor index_bias(const Tensor& table, at::TensorList plan, int64_t buckets, int64_t lq, int64_t lk,
                   int64_t slab_rows, int64_t slabs, int64_t segments, int64_t type) {
-  TORCH_CHECK(plan.size() == 7, "index_bias: a plan has 7 tensors");
+  check_table("index_bias", table, buckets, lq, lk, type);
+  TORCH_CHECK(plan.size() == 7 && slabs >= 0 && segments >= 0 && slab_rows >= 1 &&
+                  lk <= KAT_BIAS_SLAB_CELLS &&
+                  run_of(plan[0], table, at::kInt, lq * round8(lk)) &&
+                  run_of(plan[1], table, at::kUInt16, plan[1].numel()) &&
+                  run_of(plan[2], table, at::kUInt16, plan[1].numel()) &&
+                  run_of(plan[3], table, at::kInt, segments + 1) &&
+                  run_of(plan[4], table, at::kInt, slabs + 1) &&
+                  run_of(plan[5], table, at::kInt, segments) &&
+                  run_of(plan[6], table, at::kInt, buckets + 1),
+              "index_bias: the plan has another shape, number of buckets or device");
+  need_cuda("index_bias", table);
   const Index a{plan, buckets, lq, lk, slab_rows, slabs, segments, type};
   return wants_grad({&table}) ? IndexBias::apply(table, a) : index_forward(table, a);
 }

@@ -63,6 +63,9 @@ def rope_grid_table(rows: int, cols: int, rot_dim: int, prefix: int = 0, base: f
             torch.cat([tables[0][1], tables[1][1]], 1))
 
 
+# The torch operators check their arguments.  What they refuse, or positions that are to be spread
+# first, comes here for an error that says what is wrong.
+
 def _check_rest(name: str, x: Tensor, head_dim: int, q_weight, k_weight, cos, sin, positions):
     """Checks what both functions share; returns positions as the kernels read them."""
     if x.dtype not in DTYPES:
@@ -134,6 +137,19 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None,
     q_weight, k_weight: [D] or None (no scaling).  cos, sin: [rows, rot_dim / 2] fp32, or None
     (no rotation); token t takes row t, or positions [B, L] (broadcast) says which.  A position
     outside the table makes that token's heads NaN."""
+    if positions is None or (positions.dtype == torch.int64 and positions.shape == q.shape[:2]):
+        try:
+            return _native.ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                              interleaved)
+        except RuntimeError:
+            _check_qk(q, k, q_weight, k_weight, cos, sin, positions)
+            raise
+    positions = _check_qk(q, k, q_weight, k_weight, cos, sin, positions)
+    return _native.ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                      interleaved)
+
+
+def _check_qk(q, k, q_weight, k_weight, cos, sin, positions):
     _need_cuda("qk_norm_rope", q)
     _need_cuda("qk_norm_rope", k)
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
@@ -141,10 +157,7 @@ def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor] = None,
                          f"{tuple(q.shape)} and {tuple(k.shape)}")
     if q.dtype != k.dtype or q.device != k.device:
         raise TypeError(f"qk_norm_rope: q is {q.dtype} on {q.device}, k {k.dtype} on {k.device}")
-    positions = _check_rest("qk_norm_rope", q, q.shape[3], q_weight, k_weight, cos, sin,
-                            positions)
-    return _native.ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps,
-                                      interleaved)
+    return _check_rest("qk_norm_rope", q, q.shape[3], q_weight, k_weight, cos, sin, positions)
 
 
 @_native.untraced
@@ -156,6 +169,19 @@ def qkv_norm_rope(qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Te
     """`qk_norm_rope` of a projection's output qkv [B, L, (q_heads + 2 k_heads) D], the queries'
     heads first, then the keys', then the values'.  Returns (q, k, v) as [B, L, heads, D]; v is a
     view of qkv."""
+    if positions is None or (positions.dtype == torch.int64 and positions.shape == qkv.shape[:2]):
+        try:
+            return _native.ops().qkv_norm_rope(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
+                                               positions, eps, interleaved)
+        except RuntimeError:
+            _check_qkv(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin, positions)
+            raise
+    positions = _check_qkv(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin, positions)
+    return _native.ops().qkv_norm_rope(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
+                                       positions, eps, interleaved)
+
+
+def _check_qkv(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin, positions):
     _need_cuda("qkv_norm_rope", qkv)
     if q_heads < 1 or k_heads < 1:
         raise ValueError(f"qkv_norm_rope: need at least one head of each, got {q_heads} and "
@@ -163,10 +189,8 @@ def qkv_norm_rope(qkv: Tensor, q_heads: int, k_heads: int, q_weight: Optional[Te
     if qkv.dim() != 3 or qkv.shape[2] == 0 or qkv.shape[2] % (q_heads + 2 * k_heads):
         raise ValueError(f"qkv_norm_rope: expected [B, L, (Hq + 2 Hk) D] for {q_heads} and "
                          f"{k_heads} heads, got {tuple(qkv.shape)}")
-    positions = _check_rest("qkv_norm_rope", qkv, qkv.shape[2] // (q_heads + 2 * k_heads),
-                            q_weight, k_weight, cos, sin, positions)
-    return _native.ops().qkv_norm_rope(qkv, q_heads, k_heads, q_weight, k_weight, cos, sin,
-                                       positions, eps, interleaved)
+    return _check_rest("qkv_norm_rope", qkv, qkv.shape[2] // (q_heads + 2 * k_heads),
+                       q_weight, k_weight, cos, sin, positions)
 
 
 class QKNormRope(nn.Module):

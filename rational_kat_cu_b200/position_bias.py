@@ -250,6 +250,9 @@ def grid_index(rows: int, cols: int, prefix: int = 0) -> Tuple[Tensor, int]:
     return index, pairs + (3 if prefix else 0)
 
 
+# The torch operators check their arguments; what they refuse comes here for an error that says what
+# is wrong.
+
 def _check_table(name: str, table: Tensor, num_buckets: int, dtype: torch.dtype) -> None:
     if not table.is_cuda:
         raise RuntimeError(f"{name}: the table must be a CUDA tensor; there is no CPU "
@@ -270,13 +273,20 @@ def distance_bias(table: Tensor, buckets: DistanceBuckets, lq: int, lk: int, off
     last queries of a sequence, the cache's length for new tokens).  With `causal`, keys ahead of
     their query get -infinity and take no part in the gradient."""
     dtype = dtype or table.dtype
+    try:
+        return _native.ops().distance_bias(table, buckets.on(table.device), buckets.num_buckets,
+                                           buckets.reach, lq, lk, offset, bool(causal),
+                                           DTYPES.get(dtype, -1))
+    except RuntimeError:
+        _check_distance(table, buckets, lq, lk, offset, dtype)
+        raise
+
+
+def _check_distance(table, buckets, lq, lk, offset, dtype) -> None:
     _check_table("distance_bias", table, buckets.num_buckets, dtype)
     if not (0 <= lq <= MAX_LENGTH and 0 <= lk <= MAX_LENGTH and abs(offset) <= MAX_LENGTH):
         raise ValueError(f"distance_bias: lq, lk and |offset| must be 0..{MAX_LENGTH}, got "
                          f"{lq}, {lk} and {offset}")
-    return _native.ops().distance_bias(table, buckets.on(table.device), buckets.num_buckets,
-                                       buckets.reach, lq, lk, offset, bool(causal),
-                                       DTYPES[dtype])
 
 
 @_native.untraced
@@ -285,10 +295,13 @@ def index_bias(table: Tensor, buckets: IndexBuckets,
     """bias[h, i, j] = table[index[i, j], h], [heads, Lq, Lk] of type `dtype` (default: the
     table's)."""
     dtype = dtype or table.dtype
-    _check_table("index_bias", table, buckets.num_buckets, dtype)
-    return _native.ops().index_bias(table, buckets.on(table.device), buckets.num_buckets,
-                                    *buckets.shape, buckets.slab_rows, buckets.slabs,
-                                    buckets.segments, DTYPES[dtype])
+    try:
+        return _native.ops().index_bias(table, buckets.on(table.device), buckets.num_buckets,
+                                        *buckets.shape, buckets.slab_rows, buckets.slabs,
+                                        buckets.segments, DTYPES.get(dtype, -1))
+    except RuntimeError:
+        _check_table("index_bias", table, buckets.num_buckets, dtype)
+        raise
 
 
 class RelativePositionBias(nn.Module):
