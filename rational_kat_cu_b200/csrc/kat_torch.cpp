@@ -72,6 +72,10 @@ bool whole(const Tensor& t, const Tensor& like) {
 bool run_of(const Tensor& t, const Tensor& like, at::ScalarType type, int64_t n) {
   return t.scalar_type() == type && t.numel() == n && whole(t, like);
 }
+// The tensor with its values as they lie in memory (a conjugate's imaginary part is a view whose values
+// are still to be negated).
+Tensor settled(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor settled(const std::optional<Tensor>& t) { return t ? settled(*t) : Tensor(); }
 void need_cuda(const char* name, const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), name, ": expected CUDA tensors, got ", t.device());
 }
@@ -128,6 +132,7 @@ variable_list once(variable_list results, const variable_list& from) {
 // ---------------------------------------------------------------------------
 
 using Maybe = std::optional<Tensor>;
+Maybe given(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
 struct Rope {   // undefined tensors: none
   Tensor cos, sin, positions;
@@ -173,7 +178,8 @@ void check_rope(const char* name, const Tensor& x, int64_t head_dim, const Tenso
 const void* pointer(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 
 // The same values with a head's D values one after the other.
-Tensor heads_of(const Tensor& t) {
+Tensor heads_of(const Tensor& t_in) {
+  const Tensor t = settled(t_in);
   return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
 }
 
@@ -320,8 +326,8 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
                                         const Maybe& sin,
                                         const Maybe& positions, double eps,
                                         bool interleaved) {
-  const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
-  const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
+  const Tensor wq = settled(q_weight), wk = settled(k_weight);
+  const Rope rope{settled(cos), settled(sin), settled(positions), eps, interleaved};
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
                   q.size(3) == k.size(3) && q.scalar_type() == k.scalar_type() &&
                   q.device() == k.device() && plain(k),
@@ -329,12 +335,13 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
   check_rope("qk_norm_rope", q, q.size(3), wq, wk, rope);
   need_cuda("qk_norm_rope", q);
   const variable_list out = wants_grad({&q, &k, &wq, &wk, &rope.cos, &rope.sin})
-                                ? QkNormRope::apply(q, k, q_weight, k_weight, rope)
+                                ? QkNormRope::apply(q, k, given(wq), given(wk), rope)
                                 : qk_forward(heads_of(q), heads_of(k), wq, wk, rope);
   return {out[0], out[1]};
 }
 
-Tensor packed_of(const Tensor& qkv) {
+Tensor packed_of(const Tensor& qkv_in) {
+  const Tensor qkv = settled(qkv_in);
   return qkv.stride(2) == 1 || qkv.size(2) == 1 ? qkv : qkv.contiguous();
 }
 
@@ -398,8 +405,8 @@ std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, int64_t q_he
                                                  const Maybe& sin,
                                                  const Maybe& positions, double eps,
                                                  bool interleaved) {
-  const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none);
-  const Rope rope{cos.value_or(none), sin.value_or(none), positions.value_or(none), eps, interleaved};
+  const Tensor wq = settled(q_weight), wk = settled(k_weight);
+  const Rope rope{settled(cos), settled(sin), settled(positions), eps, interleaved};
   constexpr int64_t most = int64_t(1) << 31;
   TORCH_CHECK(qkv.dim() == 3 && q_heads >= 1 && k_heads >= 1 && q_heads < most && k_heads < most &&
                   qkv.size(2) > 0 && qkv.size(2) % (q_heads + 2 * k_heads) == 0,
@@ -407,7 +414,7 @@ std::tuple<Tensor, Tensor, Tensor> qkv_norm_rope(const Tensor& qkv, int64_t q_he
   check_rope("qkv_norm_rope", qkv, qkv.size(2) / (q_heads + 2 * k_heads), wq, wk, rope);
   need_cuda("qkv_norm_rope", qkv);
   const variable_list out = wants_grad({&qkv, &wq, &wk, &rope.cos, &rope.sin})
-                                ? QkvNormRope::apply(qkv, q_weight, k_weight, q_heads, k_heads, rope)
+                                ? QkvNormRope::apply(qkv, given(wq), given(wk), q_heads, k_heads, rope)
                                 : qkv_forward(packed_of(qkv), q_heads, k_heads, wq, wk, rope);
   return {out[0], out[1], out[2]};
 }
@@ -452,7 +459,7 @@ struct Distance {
 
 Tensor distance_forward(const Tensor& table_in, const Distance& a) {
   const On on(table_in);
-  const Tensor table = table_in.contiguous();
+  const Tensor table = settled(table_in).contiguous();
   const auto out = rows_of(table, a.lq, a.lk, a.type);
   check("kat_distance_bias_fwd",
         entries.distance_fwd(table.const_data_ptr(), code_of(table.scalar_type()), int32_t(a.buckets),
@@ -470,7 +477,7 @@ struct DistanceBias : Function<DistanceBias> {
     return distance_forward(table, a);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor& grad = grads[0];
+    const Tensor grad = settled(grads[0]);
     const auto runs = ctx->saved_data["runs"].toTensorVector();
     const auto n = ctx->saved_data["sizes"].toIntVector();
     const On on(grad);
@@ -510,7 +517,7 @@ struct Index {
 
 Tensor index_forward(const Tensor& table_in, const Index& a) {
   const On on(table_in);
-  const Tensor table = table_in.contiguous();
+  const Tensor table = settled(table_in).contiguous();
   const auto out = rows_of(table, a.lq, a.lk, a.type);
   check("kat_index_bias_fwd",
         entries.index_fwd(table.const_data_ptr(), code_of(table.scalar_type()), int32_t(a.buckets),
@@ -527,7 +534,7 @@ struct IndexBias : Function<IndexBias> {
     return index_forward(table, a);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor& grad = grads[0];
+    const Tensor grad = settled(grads[0]);
     const auto plan = ctx->saved_data["plan"].toTensorVector();
     const auto n = ctx->saved_data["sizes"].toIntVector();
     const On on(grad);

@@ -81,7 +81,7 @@ def orthogonalize(x: Tensor, steps: int = 5) -> Tensor:
     out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     if x.numel() == 0:
         return out
-    src = x.detach().contiguous().view(-1, rows, cols)
+    src = x.detach().resolve_neg().contiguous().view(-1, rows, cols)
     dst = out.view(-1, rows, cols)
     size = rows * cols * x.element_size()
     with torch.cuda.device(x.device):
@@ -111,9 +111,9 @@ def _check_step_lists(weights, grads, momenta) -> None:
         if m.shape != w.shape or m.dtype != torch.float32 or m.device != w.device:
             raise ValueError(f"muon_step: momenta must be float32 and have the weights' shapes "
                              f"and devices, got {tuple(m.shape)} {m.dtype} on {m.device}")
-        if not (w.is_contiguous() and m.is_contiguous()):
+        if not (w.is_contiguous() and m.is_contiguous()) or w.is_neg() or m.is_neg():
             raise ValueError("muon_step: weights and momenta are updated in place and must be "
-                             "contiguous")
+                             "contiguous, without a pending negation")
         if w.numel():
             written.append((w.data_ptr(), w.numel() * w.element_size()))
             written.append((m.data_ptr(), m.numel() * 4))
@@ -175,7 +175,7 @@ def muon_step(weights: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seque
             for start, n, ws_bytes in _runs(len(members), rows, cols):
                 at = members[start:start + n]
                 ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8)
-                gs = [grads[i].contiguous() for i in at]
+                gs = [grads[i].resolve_neg().contiguous() for i in at]
                 st = _native.lib().kat_muon_step(
                     _pointers([weights[i] for i in at]), _pointers(gs),
                     _pointers([momenta[i] for i in at]), n, rows, cols, DTYPES[dtype], lr_value,

@@ -167,3 +167,49 @@ def test_compiled_attention_options(cuda_device):
     want = model(images)
     got = torch.compile(model, backend="eager")(images)
     assert torch.equal(got, want)
+
+
+def test_pending_negations(cuda_device):
+    """The imaginary part of a conjugate is a view whose values are still to be negated."""
+    def negated(*shape, seed=0):
+        z = torch.complex(normal(*shape, seed=seed), normal(*shape, seed=seed + 1))
+        return z.conj().imag
+
+    q, k, w = negated(2, 3, 4, 16), negated(2, 3, 2, 16, seed=2), negated(16, seed=4)
+    assert q.is_neg()
+    for got, want in zip(kat.qk_norm_rope(q, k, w.clone(), w.clone()),
+                         kat.qk_norm_rope(q.resolve_neg(), k.resolve_neg(), w.resolve_neg().clone(),
+                                          w.resolve_neg().clone())):
+        assert torch.equal(got, want)
+    x = torch._neg_view(normal(2, 3, 64))
+    wn = torch._neg_view(normal(16))
+    tables = [torch._neg_view(t) for t in kat.rope_table(3, 16, device="cuda")]
+    for got, want in zip(kat.qkv_norm_rope(x, 2, 1, wn, wn, *tables),
+                         kat.qkv_norm_rope(x.resolve_neg(), 2, 1, wn.resolve_neg(), wn.resolve_neg(),
+                                           *[t.resolve_neg() for t in tables])):
+        assert torch.equal(got, want)
+    table, b, plan = torch._neg_view(normal(32, 2)), kat.DistanceBuckets(), grid_plan()
+    assert torch.equal(kat.distance_bias(table, b, 5, 6),
+                       kat.distance_bias(table.resolve_neg(), b, 5, 6))
+    cells = torch._neg_view(normal(38, 2))
+    assert torch.equal(kat.index_bias(cells, plan), kat.index_bias(cells.resolve_neg(), plan))
+    # gradients
+    leaves = [normal(32, 2).requires_grad_(), normal(38, 2).requires_grad_(),
+              normal(2, 3, 64).requires_grad_()]
+    outs = [kat.distance_bias(leaves[0], b, 5, 8), kat.index_bias(leaves[1], plan),
+            *kat.qkv_norm_rope(leaves[2], 2, 1)]
+    ups = [torch._neg_view(normal(*o.shape, seed=i)) for i, o in enumerate(outs)]
+    got = torch.autograd.grad(outs, leaves, ups, retain_graph=True)
+    want = torch.autograd.grad(outs, leaves, [u.resolve_neg() for u in ups])
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    # updates
+    u = torch._neg_view(normal(24, 40))
+    assert torch.equal(kat.orthogonalize(u), kat.orthogonalize(u.resolve_neg()))
+    ws, ms = normal(2, 24, 40), torch.zeros(2, 24, 40, device="cuda")
+    ws[1] = ws[0]
+    kat.muon_step([ws[0]], [u], [ms[0]], lr=0.1)
+    kat.muon_step([ws[1]], [u.resolve_neg()], [ms[1]], lr=0.1)
+    assert torch.equal(ws[0], ws[1]) and torch.equal(ms[0], ms[1])
+    for a, c in ((torch._neg_view(ws[0]), ms[0]), (ws[0], torch._neg_view(ms[0]))):
+        with pytest.raises(ValueError, match="negat"):
+            kat.muon_step([a], [u], [c], lr=0.1)
