@@ -208,6 +208,8 @@ class QKNormRope(nn.Module):
         self.q_weight = nn.Parameter(torch.ones(head_dim))
         self.k_weight = nn.Parameter(torch.ones(head_dim))
         cos, sin = table if table is not None else (None, None)
+        if any(t is not None and t.is_meta for t in (cos, sin)):
+            raise ValueError("QKNormRope: the table has no values (made on the meta device)")
         self.register_buffer("cos", cos, persistent=False)
         self.register_buffer("sin", sin, persistent=False)
 
@@ -217,8 +219,12 @@ class QKNormRope(nn.Module):
         tables = (self.cos, self.sin)
         super()._apply(fn, recurse)
         for name, t in zip(("cos", "sin"), tables):
-            if t is not None and not t.is_meta:
-                setattr(self, name, t.to(getattr(self, name).device))
+            if t is None:
+                continue
+            if t.is_meta and not getattr(self, name).is_meta:
+                raise RuntimeError("QKNormRope: the table's values were left on the meta device; "
+                                   "make the module again")
+            setattr(self, name, t.to(getattr(self, name).device))
         return self
 
     def forward(self, qkv: Tensor,

@@ -29,6 +29,22 @@ def test_stored_plans_hold_no_device_copies(make):
     assert module.buckets.num_buckets == 35
 
 
+def test_tables_without_values_are_refused():
+    """A table is not stored: one that the meta device lost would come back as whatever memory held."""
+    with torch.device("meta"):
+        with pytest.raises(ValueError, match="no values"):
+            kat.QKNormRope(16, 2, table=kat.rope_table(4, 16))
+        plain = kat.QKNormRope(16, 2)
+        kept = kat.QKNormRope(16, 2, table=kat.rope_table(4, 16, device="cpu"))
+    plain.to_empty(device="cpu")
+    table = kat.rope_table(4, 16)
+    kept.to_empty(device="cpu").half()
+    assert torch.equal(kept.cos, table[0]) and torch.equal(kept.sin, table[1])
+    kept.to("meta")
+    with pytest.raises(RuntimeError, match="left on the meta device"):
+        kept.to_empty(device="cpu")
+
+
 def operators():
     return _native.ops()
 
