@@ -154,7 +154,7 @@ def muon_step(weights: Sequence[Tensor], grads: Sequence[Tensor], momenta: Seque
     lr_ptr, lr_value = None, 0.0
     if isinstance(lr, Tensor):
         if lr.is_cuda:
-            if lr.numel() != 1 or lr.dtype != torch.float32:
+            if lr.numel() != 1 or lr.dtype != torch.float32 or lr.is_neg():
                 raise ValueError(f"muon_step: a CUDA lr must be one float32, got "
                                  f"{tuple(lr.shape)} {lr.dtype}")
             if any(w.device != lr.device for w in weights):

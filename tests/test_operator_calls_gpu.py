@@ -213,3 +213,5 @@ def test_pending_negations(cuda_device):
     for a, c in ((torch._neg_view(ws[0]), ms[0]), (ws[0], torch._neg_view(ms[0]))):
         with pytest.raises(ValueError, match="negat"):
             kat.muon_step([a], [u], [c], lr=0.1)
+    with pytest.raises(ValueError, match="lr"):
+        kat.muon_step([ws[0]], [u], [ms[0]], lr=torch._neg_view(torch.ones(1, device="cuda")))
