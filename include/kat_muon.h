@@ -17,9 +17,9 @@
  * Small singular values grow by a^steps, and with them the rounding of the operands.  Every
  * matrix is therefore held as two fp16 planes (value x 2^14 = hi + lo, 22 bits), and a product
  * is hi hi + hi lo + lo hi in an fp32 accumulator; sums of more than 1024 terms are added up from
- * parts.  The result's relative error is 1e-5 to 8e-5 for any type and size (4e-6 with fp32
- * products, whose sums are rounded where the tensor cores' are cut; 2e-3 with single fp16 or bf16
- * operands).
+ * parts.  After five steps the result's relative error is about 1e-5 and at most 1e-4, for any type
+ * and size (2e-6 and 7e-6 with fp32 products, whose sums are rounded where the tensor cores' are cut;
+ * 2e-3 with single fp16 or bf16 operands).
  *
  * Conventions as in kat_rational.h: the caller owns every buffer, nothing is allocated, work is
  * enqueued on `stream` of the current device, argument errors are reported before anything is

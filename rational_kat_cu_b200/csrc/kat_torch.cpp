@@ -2,10 +2,11 @@
 // (libkat_torch.so, loaded by _native.ops()).
 //
 // Everything is computed by libkat_rational.so through its C entries, whose addresses kat_torch_bind
-// takes.  What is here allocates outputs, fills the entries' arguments and is the node of the backward
-// pass.  It is C++ because these calls are short: a forward and backward pass of a 197-token grid bias
-// takes its kernels 9 us and the call 69, 94 with the same nodes in Python (packed q/k norm of the ViT-B/16
-// block at batch 128: 104 and 156; one token's, forward alone: 14 and 21).
+// takes.  What is here checks the arguments, allocates outputs, fills the entries' arguments and is the
+// node of the backward pass.  It is C++ because these calls are short: a forward and backward pass of a
+// 197-token grid bias takes its kernels 9 us and the call 67, 94 with the same nodes in Python (packed q/k
+// norm of the ViT-B/16 block at batch 128: 97 and 156; one token's, forward alone: 11 and 21, and 14 with
+// the checks in Python).
 
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>

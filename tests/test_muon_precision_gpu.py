@@ -77,6 +77,29 @@ def test_long_sums(cuda_device, shape, steps):
     assert torch.equal(out, kat.orthogonalize(x, steps=steps))
 
 
+@pytest.mark.parametrize("shape", [(12, 768, 2304), (3, 1500, 4000), (1, 4000, 4100), (2, 3000, 2050)])
+def test_long_sums_in_pairs(cuda_device, shape):
+    """CTA pairs: parts of the Gram matrix alone, of every product, several tiles to a pair."""
+    x = normal(*shape, seed=shape[2])
+    out = kat.orthogonalize(x)
+    for i in {0, shape[0] - 1}:
+        assert apart(out[i], polar(x[i])) <= 1e-4
+    assert muon.device_status() == 0
+    assert torch.equal(out, kat.orthogonalize(x))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1100, 1100), (2, 2600, 2700), (1, 3000, 1300)])
+def test_long_sums_of_16_bit_weights(cuda_device, shape, dtype):
+    gs = [normal(*shape[1:], seed=i, dtype=dtype) for i in range(shape[0])]
+    ws = [torch.zeros_like(g) for g in gs]
+    ms = [torch.zeros_like(g, dtype=torch.float32) for g in gs]
+    kat.muon_step(ws, gs, ms, lr=0.5, momentum=0.5, nesterov=False)
+    scale = 0.5 * 0.2 * math.sqrt(max(shape[1:]))
+    for w, g in zip(ws, gs):
+        assert apart(w, (-scale * polar(g)).to(dtype)) <= math.sqrt(torch.finfo(dtype).eps * 5e-5)
+
+
 def test_long_sums_of_one_direction(cuda_device):
     """Rows that agree: every term of a sum has one sign."""
     x = 1 + 0.1 * normal(64, 40000)
