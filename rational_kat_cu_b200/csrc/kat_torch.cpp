@@ -65,7 +65,11 @@ at::ScalarType type_of(int64_t code) {
 bool known_type(at::ScalarType type) {
   return type == at::kFloat || type == at::kHalf || type == at::kBFloat16;
 }
-bool plain(const Tensor& t) { return t.layout() == at::kStrided && !t._is_zerotensor(); }
+// Its values lie where it says (not so in a subclass that wraps other tensors).
+bool plain(const Tensor& t) {
+  return t.layout() == at::kStrided && !t._is_zerotensor() &&
+         !t.unsafeGetTensorImpl()->is_python_dispatch();
+}
 bool whole(const Tensor& t, const Tensor& like) {
   return plain(t) && t.device() == like.device() && t.is_contiguous();
 }

@@ -172,3 +172,37 @@ def test_operators_check_their_plans():
     for plan in other_plans(index_args()["plan"]):
         with pytest.raises(RuntimeError, match="^index_bias: the plan"):
             operators().index_bias(**index_args(plan=plan))
+
+
+class Wrapped(torch.Tensor):
+    """A tensor whose values lie in another one, as distributed tensors' do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype,
+                                                   device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+
+@pytest.mark.parametrize("which", ["q", "k", "q_weight", "k_weight", "cos", "sin", "positions"])
+def test_wrapped_tensors_are_refused(which):
+    """They have no values of their own: a weight without an address would count as none."""
+    args = qk_args()
+    args[which] = Wrapped(args[which])
+    with pytest.raises(RuntimeError, match="^qk_norm_rope: (?!expected CUDA)"):
+        operators().qk_norm_rope(**args)
+    if which in ("q", "k"):
+        return
+    del args["q"], args["k"]
+    with pytest.raises(RuntimeError, match="^qkv_norm_rope: (?!expected CUDA)"):
+        operators().qkv_norm_rope(torch.zeros(2, 3, 64), 2, 1, **args)
+
+
+def test_wrapped_tables_are_refused():
+    with pytest.raises(RuntimeError, match="^distance_bias: (?!expected CUDA)"):
+        operators().distance_bias(**distance_args(table=Wrapped(torch.zeros(8, 2))))
+    with pytest.raises(RuntimeError, match="^index_bias: (?!expected CUDA)"):
+        operators().index_bias(**index_args(table=Wrapped(torch.zeros(35, 2))))
